@@ -204,6 +204,13 @@ def _context():
     return ctx
 
 
+def _scratch(st, name, *sizes):
+    """The scratch memory that a caller keeps for an entry point."""
+    if "scratch" not in st:
+        st["scratch"] = torch.empty(_context().scratch_bytes(name, *sizes), dtype=torch.uint8, device="cuda")
+    return st["scratch"]
+
+
 def _pair(ts):
     return ts[0], (ts[1] if len(ts) > 1 else None)
 
@@ -231,7 +238,8 @@ def _plain_embed(st):
 
 def _own_embed_grad(st):
     (g0, g1), (d0, d1) = _pair(st["x"]), _pair(st["out"])
-    _context().call("ring_embed_grad", g0, g1, st["ids"], st["n"], st["vocab"], st["dim"], st["scale"], st["shift"], 0, d0, d1)
+    ws = _scratch(st, "ring_embed_grad", st["n"], st["vocab"], st["dim"])
+    _context().call("ring_embed_grad", g0, g1, st["ids"], st["n"], st["vocab"], st["dim"], st["scale"], st["shift"], 0, ws, d0, d1)
     return st["out"]
 
 
@@ -244,7 +252,8 @@ def _plain_embed_grad(st):
 
 def _own_norm(st):
     ns = [t.numel() for t in st["x0"]]
-    _context().call("aby3_sqnorm_local", st["x0"], st["x1"], ns, len(ns), SEED_NEXT, st["pop"], SEED_PREV, st["pop"], st["z"])
+    ws = _scratch(st, "aby3_sqnorm", len(ns))
+    _context().call("aby3_sqnorm_local", st["x0"], st["x1"], ns, len(ns), SEED_NEXT, st["pop"], SEED_PREV, st["pop"], ws, st["z"])
     return st["z"]
 
 
@@ -269,8 +278,9 @@ def _plain_clip(st):
 
 def _own_logprobs(st):
     logp, ent, top_ids, top_logp, row_max, log_sum = st["out"]
+    ws = _scratch(st, "reveal_logprobs", st["rows"], st["vocab"], st["top"])
     _context().call("reveal_logprobs", *_three(st["shares_of"]), st["rows"], st["vocab"], FRAC, st["ids"], st["per_row"],
-                    st["top"], logp, ent, top_ids, top_logp, row_max, log_sum)
+                    st["top"], ws, logp, ent, top_ids, top_logp, row_max, log_sum)
     return st["out"]
 
 
