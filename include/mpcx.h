@@ -421,6 +421,70 @@ int mpcx_my_bit_inject_party_post(mpcx_ctx *ctx, int party, uint64_t seed2, uint
 /* reveal_vec_bools (:777-807): out = a ^ b, one byte per boolean */
 int mpcx_xor_bools(mpcx_ctx *ctx, const int8_t *a, const int8_t *b, int8_t *out, uint64_t n);
 
+/* ---- language models on shares (no counterpart in the reference) ----
+ * A model whose weights stay shared, run and trained on public text.  Token ids are public int64 words, so the rows of a
+ * shared table are looked up, and its gradient gathered, locally on every share; the logits are opened
+ * (ABY3Engine.cpp:145-158) and the log probabilities, and the error that the loss sends back, are formed from the opened
+ * words; the global norm of shared gradients is one opened word.  Matrices are row-major and contiguous; reals are fixed
+ * point, a word w standing for w 2^-frac.  Outputs must not overlap inputs.  Scratch memory is the caller's, 8-byte
+ * aligned, of at least the bytes that the _scratch function next to the call names; its contents need not be
+ * kept between calls and two calls may share it when they are ordered (two graphs that may run at once need one each).
+ * All calls can be captured into a graph once the context has the generator words they use.
+ *
+ * E_k[t] = (scale * T_k[ids[t]]) >> shift, t < n: rows of a vocab x dim table, a zero row for an id outside [0, vocab)
+ * (padding).  T1 / E1 are the second replicated share, or both NULL for additive shares.  shift (arithmetic, as
+ * benchmark/benchmark1.cpp:106-112 truncates additive shares locally) must be 0 with replicated shares, whose product
+ * goes through the trunc protocol instead (mpcx_aby3_trunc_local). */
+int mpcx_ring_embed(mpcx_ctx *ctx, const int64_t *T0, const int64_t *T1, uint64_t vocab, uint64_t dim, const int64_t *ids,
+                    uint64_t n, int64_t scale, int shift, int64_t *E0, int64_t *E1);
+/* The gradient of that lookup with respect to the table: dT_k[v] (+)= (scale * sum of G_k[t] over ids[t] = v) >> shift,
+ * all vocab rows (zero where no token falls; left as they were there with accumulate != 0).  Sums mod 2^64 do not depend
+ * on the order of the tokens. */
+uint64_t mpcx_ring_embed_grad_scratch(uint64_t n, uint64_t vocab, uint64_t dim);
+int mpcx_ring_embed_grad(mpcx_ctx *ctx, const int64_t *G0, const int64_t *G1, const int64_t *ids, uint64_t n, uint64_t vocab,
+                         uint64_t dim, int64_t scale, int shift, int accumulate, void *scratch, int64_t *dT0, int64_t *dT1);
+/* This party's share of the squared norm of `count` shared tensors taken together, before the round: z0[0] = sum over all
+ * words of X0*X0 + X0*X1 + X1*X0, plus pop(next) - pop(prev) (one word of each stream).  X0, X1 and lens are HOST arrays:
+ * the device pointers of the tensors' shares and their word counts (0 allowed).  The sum of the three parties' z0 is the
+ * squared norm with twice the tensors' fractional bits; it must stay below 2^64. */
+uint64_t mpcx_aby3_sqnorm_scratch(uint64_t count);
+int mpcx_aby3_sqnorm_local(mpcx_ctx *ctx, const int64_t *const *X0, const int64_t *const *X1, const uint64_t *lens,
+                           uint64_t count, uint64_t seed_next, uint64_t pop_next, uint64_t seed_prev, uint64_t pop_prev,
+                           void *scratch, int64_t *z0);
+/* Clips those tensors to the global norm max_norm (a word with `number` fractional bits, like the tensors), before the
+ * round.  S = z_prev + z0 + z1 is the opened squared norm (the three shares, one device word each, read as one unsigned
+ * word); the factor is the largest c in [0, 2^number] with c^2 S <= (max_norm 2^number)^2, in exact integers, and Y0 is
+ * the trunc segment (ABY3Engine.cpp:480-503) of c * X by `number` bits: the message to the previous party, the tensors
+ * one after the other (the words that parties 1 and 2 pop run through them in the same order).  Party 0 reads X0 only,
+ * party 1 both shares, party 2 none (its X0 / X1 may be NULL).  coef (nullable) receives c.  number <= 31,
+ * max_norm < 2^(62 - number).  Party 0's segment is also the local clip of an additive share. */
+int mpcx_aby3_clip_local(mpcx_ctx *ctx, int party, const int64_t *const *X0, const int64_t *const *X1, const uint64_t *lens,
+                         uint64_t count, const int64_t *z_prev, const int64_t *z0, const int64_t *z1, uint64_t max_norm,
+                         int number, uint64_t seed12, uint64_t pop12, int64_t *Y0, int64_t *coef);
+/* Opened logits x = a + b + c (rows x vocab words with frac fractional bits; c NULL: two additive shares, b and c NULL:
+ * already opened).  Per row, l = x 2^-frac:
+ *   row_max    the largest word                       log_sum   ln sum exp(l - max l)
+ *   logp       ln p of the row's per_row ids (rows x per_row; 0 where an id lies outside [0, vocab))
+ *   entropy    - sum p ln p
+ *   top_ids / top_logp   the `top` likeliest ids (rows x top), equal words by the lower id, and their ln p
+ * Differences of words are exact; the sums are kept in 32-bit floats.  top <= 32, top <= vocab, frac <= 62,
+ * vocab < 2^31.  ids / logp may be NULL when per_row = 0, top_ids / top_logp when top = 0; entropy, row_max and log_sum
+ * may be NULL. */
+uint64_t mpcx_reveal_logprobs_scratch(uint64_t rows, uint64_t vocab, uint64_t top);
+int mpcx_reveal_logprobs(mpcx_ctx *ctx, const int64_t *a, const int64_t *b, const int64_t *c, uint64_t rows, uint64_t vocab,
+                         int frac, const int64_t *ids, uint64_t per_row, uint64_t top, void *scratch, float *logp,
+                         float *entropy, int64_t *top_ids, float *top_logp, int64_t *row_max, float *log_sum);
+/* The gradient of sum_t d_logp[t] logp[t] + d_entropy entropy of every row with respect to its logits:
+ *   grad[j] = sum over t with ids[t] = j of d_logp[t]  -  p_j sum_t d_logp[t]  -  d_entropy p_j (ln p_j + entropy)
+ * (the sums run over ids inside [0, vocab)).  row_max and log_sum are the forward call's, entropy too when d_entropy is
+ * given (d_entropy NULL: no entropy term, entropy may be NULL).  grad (rows x vocab floats) and grad_words (the same
+ * rounded to the nearest word with grad_frac fractional bits, ties to even, saturating) are both optional, one at least
+ * is given. */
+int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b, const int64_t *c, uint64_t rows,
+                              uint64_t vocab, int frac, const int64_t *ids, uint64_t per_row, const float *d_logp,
+                              const float *d_entropy, const int64_t *row_max, const float *log_sum, const float *entropy,
+                              float *grad, int64_t *grad_words, int grad_frac);
+
 /* ---- several GPUs behind one party (no counterpart in the reference, which is single-threaded host code) ----
  * The path shards without any exchange between the devices: matrix_mul by row blocks of X (ABY3Engine.cpp:189-197:
  * Y replicated, the mask words of a block start row0 * c words into both pop streams), the element-wise segments by

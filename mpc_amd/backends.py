@@ -38,6 +38,8 @@ class GpuBackend:
                 dev.append(d)
             elif isinstance(a, np.ndarray):
                 dev.append(ctx.to_device(a))
+            elif isinstance(a, list):  # a host array of device pointers, or of counts
+                dev.append([ctx.to_device(e) if isinstance(e, np.ndarray) else e for e in a])
             else:
                 dev.append(a)
         ctx.call(name, *dev)
@@ -351,6 +353,51 @@ class GpuBackend:
                         None if gamma is None else _c(gamma, np.int64), None if delta is None else _c(delta, np.int64), n,
                         ("out", np.int64, n))
 
+    # ---- language models on shares (a second share of None: additive shares)
+    def _scratch(self, name, *sizes):
+        return self.ctx.empty(np.uint8, self.ctx.scratch_bytes(name, *sizes))
+
+    def ring_embed(self, T0, T1, vocab, dim, ids, scale=1, shift=0):
+        n = ids.size
+        outs = [("out", np.int64, n * dim)] * (1 if T1 is None else 2)
+        return self._go("ring_embed", _c(T0, np.int64), _c(T1, np.int64), vocab, dim, _c(ids, np.int64), n, scale, shift, *outs,
+                        *([None] if T1 is None else []))
+
+    def ring_embed_grad(self, G0, G1, ids, vocab, dim, scale=1, shift=0):
+        n = ids.size
+        outs = [("out", np.int64, vocab * dim)] * (1 if G1 is None else 2)
+        return self._go("ring_embed_grad", _c(G0, np.int64), _c(G1, np.int64), _c(ids, np.int64), n, vocab, dim, scale, shift, 0,
+                        self._scratch("ring_embed_grad", n, vocab, dim), *outs, *([None] if G1 is None else []))
+
+    def aby3_sqnorm_local(self, X0s, X1s, seed_next, pop_next, seed_prev, pop_prev):
+        """X0s, X1s: lists of the tensors' shares."""
+        X0s, X1s = [_c(x, np.int64) for x in X0s], [_c(x, np.int64) for x in X1s]
+        return self._go("aby3_sqnorm_local", X0s, X1s, [x.size for x in X0s], len(X0s), seed_next, pop_next, seed_prev, pop_prev,
+                        self._scratch("aby3_sqnorm", len(X0s)), ("out", np.int64, 1))
+
+    def aby3_clip_local(self, party, X0s, X1s, z_prev, z0, z1, max_norm, number, seed12, pop12):
+        """Returns the message (the tensors one after the other) and the factor."""
+        lens = [x.size for x in X0s]
+        X0s, X1s = [_c(x, np.int64) for x in X0s], [_c(x, np.int64) for x in X1s]
+        return self._go("aby3_clip_local", party, X0s, X1s, lens, len(lens), _c(z_prev, np.int64), _c(z0, np.int64),
+                        _c(z1, np.int64), max_norm, number, seed12, pop12, ("out", np.int64, sum(lens)), ("out", np.int64, 1))
+
+    def reveal_logprobs(self, a, b, c, rows, vocab, frac, ids, top=0):
+        """Returns logp, entropy, top_ids, top_logp, row_max, log_sum (flat)."""
+        per_row = ids.size // rows if rows else 0
+        return self._go("reveal_logprobs", _c(a, np.int64), _c(b, np.int64), _c(c, np.int64), rows, vocab, frac, _c(ids, np.int64),
+                        per_row, top, self._scratch("reveal_logprobs", rows, vocab, top), ("out", np.float32, rows * per_row),
+                        ("out", np.float32, rows), ("out", np.int64, rows * top), ("out", np.float32, rows * top),
+                        ("out", np.int64, rows), ("out", np.float32, rows))
+
+    def reveal_logprobs_grad(self, a, b, c, rows, vocab, frac, ids, d_logp, d_entropy, row_max, log_sum, entropy, grad_frac):
+        """Returns the gradient as floats and as ring words with grad_frac fractional bits (flat)."""
+        per_row = ids.size // rows if rows else 0
+        return self._go("reveal_logprobs_grad", _c(a, np.int64), _c(b, np.int64), _c(c, np.int64), rows, vocab, frac,
+                        _c(ids, np.int64), per_row, _c(d_logp, np.float32), _c(d_entropy, np.float32), _c(row_max, np.int64),
+                        _c(log_sum, np.float32), _c(entropy, np.float32), ("out", np.float32, rows * vocab),
+                        ("out", np.int64, rows * vocab), grad_frac)
+
 
 class ResidentBackend(GpuBackend):
     """GpuBackend whose arrays stay on the device: inputs and outputs are DeviceArrays borrowed from torch's
@@ -362,11 +409,15 @@ class ResidentBackend(GpuBackend):
         super().__init__(ctx)
         self.torch, self.dev = torch, dev
         self._tdt = {np.dtype(np.int64): torch.int64, np.dtype(np.uint64): torch.int64, np.dtype(np.int8): torch.int8,
-                     np.dtype(np.uint16): torch.int16, np.dtype(np.uint32): torch.int32}
+                     np.dtype(np.uint16): torch.int16, np.dtype(np.uint32): torch.int32, np.dtype(np.float32): torch.float32,
+                     np.dtype(np.uint8): torch.uint8}
 
     def empty(self, dtype, n):
         t = self.torch.empty(max(int(n), 1), dtype=self._tdt[np.dtype(dtype)], device=self.dev)
         return self.ctx.wrap(t, dtype).view(0, int(n))
+
+    def _scratch(self, name, *sizes):
+        return self.empty(np.uint8, self.ctx.scratch_bytes(name, *sizes))
 
     def up(self, a):
         a = np.ascontiguousarray(a)

@@ -32,6 +32,8 @@ def load_library():
         _lib.mpcx_last_error.restype = ctypes.c_char_p
         _lib.mpcx_last_error.argtypes = [ctypes.c_void_p]
         _lib.mpcx_get_stream.restype = ctypes.c_void_p
+        for name in ("ring_embed_grad", "aby3_sqnorm", "reveal_logprobs"):
+            getattr(_lib, f"mpcx_{name}_scratch").restype = ctypes.c_uint64
     return _lib
 
 
@@ -93,6 +95,8 @@ def _a(x):
         return ctypes.c_uint64(int(x) & 0xFFFFFFFFFFFFFFFF)
     if hasattr(x, "data_ptr"):  # torch tensor on the device
         return ctypes.c_void_p(x.data_ptr())
+    if isinstance(x, (list, tuple)):  # a host array: of device addresses (arrays, tensors) or of counts
+        return (ctypes.c_uint64 * max(len(x), 1))(*[_a(e).value or 0 for e in x])
     raise TypeError(f"cannot pass {type(x)} to the C ABI")
 
 
@@ -123,6 +127,10 @@ class Context:
     def call(self, name, *args):
         """Calls ``mpcx_<name>(ctx, *args)``; DeviceArrays / tensors / ints are converted."""
         self._call("mpcx_" + name, *[_a(x) for x in args])
+
+    def scratch_bytes(self, name, *sizes):
+        """Bytes of scratch memory that the caller of ``mpcx_<name>`` hands over (mpcx_<name>_scratch)."""
+        return getattr(self.lib, f"mpcx_{name}_scratch")(*[ctypes.c_uint64(s) for s in sizes])
 
     def sync(self):
         self._call("mpcx_sync")

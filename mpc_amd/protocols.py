@@ -175,6 +175,49 @@ def aby3_trunc(w, Xs, number):
     return [(Y0[j], Y0[(j + 1) % 3]) for j in range(3)]
 
 
+# ------------------------------------------------------------------ language models on ABY3 shares, public tokens
+def aby3_embed(w, Ts, vocab, dim, ids, scale=1):
+    """Rows ids of a shared vocab x dim table times a public ring integer; no round."""
+    return [tuple(w.be.ring_embed(Ts[j][0], Ts[j][1], vocab, dim, ids, scale)) for j in range(3)]
+
+
+def aby3_embed_grad(w, Gs, ids, vocab, dim, scale=1):
+    """The shared gradient of that table from the shared gradient of the rows; no round."""
+    return [tuple(w.be.ring_embed_grad(Gs[j][0], Gs[j][1], ids, vocab, dim, scale)) for j in range(3)]
+
+
+def aby3_sqnorm(w, tensors):
+    """tensors: list of share lists.  The three shares of the squared norm of all of them together; party j sends its own
+    to both others (the norm is opened)."""
+    z = []
+    for j in range(3):
+        nx, pv = (j + 1) % 3, (j + 2) % 3
+        z.append(w.be.aby3_sqnorm_local([t[j][0] for t in tensors], [t[j][1] for t in tensors], w.seed(j, nx), w.take(j, nx, 1),
+                                        w.seed(j, pv), w.take(j, pv, 1)))
+        w.rec(f"sqnorm.P{j}", z[j])
+    return z
+
+
+def aby3_clip(w, tensors, max_norm, number):
+    """Clips the tensors to the global norm max_norm (`number` fractional bits, as the tensors).  Two rounds: the opened
+    norm, then trunc's message.  Returns the clipped shares of all tensors as one vector, and the factor."""
+    z = aby3_sqnorm(w, tensors)
+    total = sum(t[0][0].size for t in tensors)
+    pops = [0, w.take(1, 2, total), w.take(2, 1, total)]
+    Y, coef = [], None
+    for j in range(3):
+        y, coef = w.be.aby3_clip_local(j, [t[j][0] for t in tensors], [t[j][1] for t in tensors], z[(j + 2) % 3], z[j],
+                                       z[(j + 1) % 3], max_norm, number, KEY12, pops[j])
+        Y.append(y)
+        w.rec(f"clip.P{j}->P{(j + 2) % 3}", y)
+    return [(Y[j], Y[(j + 1) % 3]) for j in range(3)], coef
+
+
+def aby3_reveal_logprobs(w, Ls, rows, vocab, frac, ids, top=0):
+    """Opens shared logits (ABY3Engine.cpp:145-158) and forms log probabilities from them, on every party."""
+    return [w.be.reveal_logprobs(Ls[(j + 2) % 3][0], Ls[j][0], Ls[j][1], rows, vocab, frac, ids, top) for j in range(3)]
+
+
 # ------------------------------------------------------------------ SecureNN
 def snn_share(w, X, n):
     """SecurennEngine::share (SecurennEngine.cpp:318-334).  Returns [X_0, X_1, zeros]."""

@@ -1,0 +1,129 @@
+"""What the language-model entry points refuse: shapes and pointers are checked on the host before anything is launched, so
+these run without a GPU (no context)."""
+import ctypes
+
+import pytest
+
+U = ctypes.c_uint64
+P = ctypes.c_void_p
+I = ctypes.c_int
+L = ctypes.c_int64
+X = P(4096)  # never read: the call is refused, or there is nothing to do
+N = P(0)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from mpc_amd.lib import load_library
+    return load_library()
+
+
+def refused(lib, name, args, text):
+    assert getattr(lib, name)(N, *args) != 0
+    assert text in lib.mpcx_last_error(None).decode(), lib.mpcx_last_error(None).decode()
+
+
+def host(*v):
+    return (ctypes.c_uint64 * max(len(v), 1))(*v)
+
+
+@pytest.mark.parametrize("args,text", [
+    ((X, N, U(1 << 40), U(1 << 40), X, U(1), L(1), I(0), X, N), "too large"),
+    ((X, N, U(4), U(1 << 40), X, U(1 << 40), L(1), I(0), X, N), "too large"),
+    ((X, N, U(4), U(4), X, U(1), L(1), I(64), X, N), "out of range"),
+    ((X, N, U(4), U(4), X, U(1), L(1), I(-1), X, N), "out of range"),
+    ((X, X, U(4), U(4), X, U(1), L(1), I(0), X, N), "second share"),
+    ((X, N, U(4), U(4), X, U(1), L(1), I(0), X, X), "second share"),
+    ((X, X, U(4), U(4), X, U(1), L(1), I(16), X, X), "not truncated locally"),
+    ((N, N, U(4), U(4), X, U(1), L(1), I(0), X, N), "NULL"),
+    ((X, N, U(4), U(4), N, U(1), L(1), I(0), X, N), "NULL"),
+    ((X, N, U(4), U(4), X, U(1), L(1), I(0), N, N), "NULL"),
+])
+def test_embed(lib, args, text):
+    refused(lib, "mpcx_ring_embed", args, text)
+
+
+def test_nothing_to_do_is_no_error(lib):
+    assert lib.mpcx_ring_embed(N, X, N, U(4), U(4), X, U(0), L(1), I(0), X, N) == 0
+    assert lib.mpcx_ring_embed(N, X, N, U(4), U(0), X, U(3), L(1), I(0), X, N) == 0
+    assert lib.mpcx_ring_embed_grad(N, X, N, X, U(3), U(0), U(4), L(1), I(0), I(0), X, X, N) == 0
+    assert lib.mpcx_reveal_logprobs(N, X, N, N, U(0), U(5), I(16), X, U(1), U(1), X, X, N, X, X, N, N) == 0
+    assert lib.mpcx_reveal_logprobs_grad(N, X, N, N, U(0), U(5), I(16), X, U(1), X, N, X, X, N, X, N, I(0)) == 0
+
+
+@pytest.mark.parametrize("args,text", [
+    ((X, N, X, U(1), U(1 << 40), U(1 << 40), L(1), I(0), I(0), X, X, N), "too large"),
+    ((X, N, X, U(1 << 33), U(4), U(4), L(1), I(0), I(0), X, X, N), "too large"),
+    ((X, N, X, U(1), U(1 << 33), U(4), L(1), I(0), I(0), X, X, N), "too large"),
+    ((X, N, X, U(1), U(4), U(4), L(1), I(64), I(0), X, X, N), "out of range"),
+    ((X, X, X, U(1), U(4), U(4), L(1), I(0), I(0), X, X, N), "second share"),
+    ((X, N, X, U(1), U(4), U(4), L(1), I(0), I(0), X, X, X), "second share"),
+    ((X, X, X, U(1), U(4), U(4), L(1), I(3), I(0), X, X, X), "not truncated locally"),
+    ((N, N, X, U(1), U(4), U(4), L(1), I(0), I(0), X, X, N), "NULL"),
+    ((X, N, N, U(1), U(4), U(4), L(1), I(0), I(0), X, X, N), "NULL"),
+    ((X, N, X, U(1), U(4), U(4), L(1), I(0), I(0), N, X, N), "NULL"),
+    ((X, N, X, U(1), U(4), U(4), L(1), I(0), I(0), X, N, N), "NULL"),
+])
+def test_embed_grad(lib, args, text):
+    refused(lib, "mpcx_ring_embed_grad", args, text)
+
+
+@pytest.mark.parametrize("args,text", [
+    ((host(4096), host(4096), host(8), U(1), U(1), U(0), U(2), U(0), N, X), "NULL"),
+    ((host(4096), host(4096), host(8), U(1), U(1), U(0), U(2), U(0), X, N), "NULL"),
+    ((N, host(4096), host(8), U(1), U(1), U(0), U(2), U(0), X, X), "NULL"),
+    ((host(4096), host(4096), N, U(1), U(1), U(0), U(2), U(0), X, X), "NULL"),
+    ((host(4096, 0), host(4096, 4096), host(8, 8), U(2), U(1), U(0), U(2), U(0), X, X), "tensor 1: NULL"),
+    ((host(4096, 4096), host(0, 4096), host(8, 8), U(2), U(1), U(0), U(2), U(0), X, X), "tensor 0: NULL"),
+    ((host(4096), host(4096), host(1 << 60), U(1), U(1), U(0), U(2), U(0), X, X), "too long"),
+])
+def test_sqnorm(lib, args, text):
+    refused(lib, "mpcx_aby3_sqnorm_local", args, text)
+
+
+def clip(party=0, X0=None, X1=None, lens=None, count=1, z=(X, X, X), max_norm=1 << 16, number=16, Y0=X, coef=X):
+    return (I(party), X0 if X0 is not None else host(4096), X1 if X1 is not None else host(4096), lens or host(8), U(count), *z,
+            U(max_norm), I(number), U(2), U(0), Y0, coef)
+
+
+@pytest.mark.parametrize("args,text", [
+    (clip(party=3), "party 3"), (clip(party=-1), "party -1"),
+    (clip(number=32), "fractional bits"), (clip(number=-1), "fractional bits"),
+    (clip(max_norm=1 << 46), "max_norm"),
+    (clip(z=(N, X, X)), "NULL"), (clip(z=(X, N, X)), "NULL"), (clip(z=(X, X, N)), "NULL"),
+    (clip(Y0=N), "NULL"), (clip(X0=host(0)), "NULL"), (clip(party=1, X1=host(0)), "NULL"), (clip(X0=N), "NULL"),
+    (clip(lens=host(1 << 60)), "too long"),
+])
+def test_clip(lib, args, text):
+    refused(lib, "mpcx_aby3_clip_local", args, text)
+
+
+def lp(a=X, b=X, c=X, rows=3, vocab=5, frac=16, ids=X, per_row=1, top=2, scratch=X, logp=X, top_ids=X, top_logp=X):
+    return (a, b, c, U(rows), U(vocab), I(frac), ids, U(per_row), U(top), scratch, logp, X, top_ids, top_logp, X, X)
+
+
+@pytest.mark.parametrize("args,text", [
+    (lp(vocab=0), "vocabulary"), (lp(vocab=1 << 31), "vocabulary"), (lp(rows=1 << 31), "too large"),
+    (lp(rows=1 << 20, per_row=1 << 50), "too large"), (lp(frac=63), "fractional"), (lp(frac=-1), "fractional"),
+    (lp(top=33, vocab=100), "alternatives"), (lp(top=6), "alternatives"), (lp(b=N), "third share"),
+    (lp(a=N), "NULL"), (lp(ids=N), "NULL"), (lp(logp=N), "NULL"), (lp(scratch=N), "NULL"), (lp(top_ids=N), "NULL"),
+    (lp(top_logp=N), "NULL"),
+])
+def test_logprobs(lib, args, text):
+    refused(lib, "mpcx_reveal_logprobs", args, text)
+
+
+def lg(a=X, b=X, c=X, rows=3, vocab=5, frac=16, ids=X, per_row=1, d_logp=X, d_entropy=X, row_max=X, log_sum=X, entropy=X,
+       grad=X, words=X, grad_frac=16):
+    return (a, b, c, U(rows), U(vocab), I(frac), ids, U(per_row), d_logp, d_entropy, row_max, log_sum, entropy, grad, words,
+            I(grad_frac))
+
+
+@pytest.mark.parametrize("args,text", [
+    (lg(vocab=0), "vocabulary"), (lg(vocab=1 << 31), "vocabulary"), (lg(rows=1 << 31), "too large"), (lg(frac=63), "fractional"),
+    (lg(grad_frac=63), "fractional"), (lg(grad_frac=-1), "fractional"), (lg(b=N), "third share"), (lg(a=N), "NULL"),
+    (lg(ids=N), "NULL"), (lg(d_logp=N), "NULL"), (lg(row_max=N), "NULL"), (lg(log_sum=N), "NULL"), (lg(entropy=N), "NULL"),
+    (lg(grad=N, words=N), "NULL"),
+])
+def test_logprobs_grad(lib, args, text):
+    refused(lib, "mpcx_reveal_logprobs_grad", args, text)
