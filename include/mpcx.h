@@ -456,7 +456,7 @@ int mpcx_aby3_sqnorm_local(mpcx_ctx *ctx, const int64_t *const *X0, const int64_
  * word); the factor is the largest c in [0, 2^number] with c^2 S <= (max_norm 2^number)^2, in exact integers, and Y0 is
  * the trunc segment (ABY3Engine.cpp:480-503) of c * X by `number` bits: the message to the previous party, the tensors
  * one after the other (the words that parties 1 and 2 pop run through them in the same order).  Party 0 reads X0 only,
- * party 1 both shares, party 2 none (its X0 / X1 may be NULL).  coef (nullable) receives c.  number <= 31,
+ * party 1 both shares, party 2 none (its X0 / X1 may be NULL).  coef (one device word) receives c.  number <= 31,
  * max_norm < 2^(62 - number).  Party 0's segment is also the local clip of an additive share. */
 int mpcx_aby3_clip_local(mpcx_ctx *ctx, int party, const int64_t *const *X0, const int64_t *const *X1, const uint64_t *lens,
                          uint64_t count, const int64_t *z_prev, const int64_t *z0, const int64_t *z1, uint64_t max_norm,

@@ -23,11 +23,132 @@ bool lm_fits(u64 a, u64 b) { return a == 0 || b <= (1ull << 60) / a; }
 
 __device__ inline void lm_atomic_add(u64 *p, u64 v) { atomicAdd((unsigned long long *)p, (unsigned long long)v); }
 
-__global__ __launch_bounds__(256) void sqnorm_kernel(const u64 *__restrict__ x0, const u64 *__restrict__ x1, u64 n, u64 *z) {
+// two neighbouring words by one 16-byte access; share arrays are 8-byte aligned only, which the hardware takes
+typedef u64 u64x2 __attribute__((ext_vector_type(2)));
+typedef u64x2 u64x2u __attribute__((aligned(8)));
+__device__ inline u64x2 ld2(const u64 *p) { return *(const u64x2u *)p; }
+__device__ inline void st2(u64 *p, u64x2 v) { *(u64x2u *)p = v; }
+
+// ---- lookup.  A row is copied by 2^lg lanes (8 .. 256) of a workgroup, 16 bytes of each share per lane and step; the
+// four steps of a lane are all requested before the first is used.
+constexpr u32 EMB_STEPS = 4;
+template <bool TWO>
+__global__ __launch_bounds__(256) void embed_kernel(const u64 *__restrict__ T0, const u64 *__restrict__ T1, u64 vocab, u64 dim,
+                                                    const i64 *__restrict__ ids, u64 n, u64 scale, int shift,
+                                                    u64 *__restrict__ E0, u64 *__restrict__ E1, u32 lg) {
+    const u32 lane = threadIdx.x & ((1u << lg) - 1), rows = 256u >> lg;
+    const u64 col0 = 2 * (((u64)blockIdx.y * EMB_STEPS << lg) + lane);
+    for (u64 t = (u64)blockIdx.x * rows + (threadIdx.x >> lg); t < n; t += (u64)gridDim.x * rows) {
+        const u64 v = (u64)ids[t];
+        const bool ok = v < vocab;
+        const u64 *r0 = T0 + v * dim, *r1 = TWO ? T1 + v * dim : nullptr;
+        u64x2 a[EMB_STEPS] = {}, b[EMB_STEPS] = {};
+#pragma unroll
+        for (u32 u = 0; u < EMB_STEPS; u++) {
+            const u64 c = col0 + ((u64)(2 * u) << lg);
+            if (!ok || c >= dim) continue;
+            if (c + 1 < dim) {
+                a[u] = ld2(r0 + c);
+                if (TWO) b[u] = ld2(r1 + c);
+            } else {
+                a[u].x = r0[c];
+                if (TWO) b[u].x = r1[c];
+            }
+        }
+#pragma unroll
+        for (u32 u = 0; u < EMB_STEPS; u++) {
+            const u64 c = col0 + ((u64)(2 * u) << lg);
+            if (c >= dim) continue;
+            u64x2 x, y;
+            if (TWO) {
+                x = a[u] * scale, y = b[u] * scale;
+            } else {
+                x.x = (u64)((i64)(a[u].x * scale) >> shift), x.y = (u64)((i64)(a[u].y * scale) >> shift);
+            }
+            if (c + 1 < dim) {
+                st2(E0 + t * dim + c, x);
+                if (TWO) st2(E1 + t * dim + c, y);
+            } else {
+                E0[t * dim + c] = x.x;
+                if (TWO) E1[t * dim + c] = y.x;
+            }
+        }
+    }
+}
+inline u32 lanes_log2(u64 dim) { // lanes for a row: enough for its 16-byte pieces, 8 .. 256
+    u32 lg = 3;
+    while (lg < 8 && (2ull << lg) < dim) lg++;
+    return lg;
+}
+
+// ---- many tensors in one launch.  The tensors of a call are cut into tiles; up to LM_TENSORS descriptors travel in the
+// kernel's own arguments, so nothing is copied to the device and a captured call keeps its descriptors.  A workgroup
+// finds the tensor of a tile by one comparison per lane and a population count.
+constexpr u32 LM_TENSORS = 96;    // descriptors of 40 bytes: the arguments stay below 4 KiB
+constexpr u64 LM_TILE = 4096;     // words
+// From this many words on party 1's segment of a tensor is one launch that consumes the stream's words where they are
+// regenerated (24 bytes of traffic a word); shorter tensors share a launch that reads the words back (40 bytes).
+constexpr u64 CLIP_FUSED_WORDS = 1 << 18;
+constexpr u32 LM_GRID = 2048;     // eight workgroups of four waves on each of 256 CUs
+struct TensorRef {
+    const u64 *x0, *x1;
+    u64 n, out, tile0; // words, first word in the call's output, first tile
+};
+struct TensorTable {
+    TensorRef t[LM_TENSORS];
+    u32 count;
+    u64 tiles;
+};
+__device__ inline u32 tensor_of(const TensorTable &tab, u64 tile) {
+    const u32 lane = threadIdx.x & 63;
+    const bool a = lane < tab.count && tab.t[lane].tile0 <= tile;
+    const bool b = lane + 64 < tab.count && tab.t[lane + 64 < LM_TENSORS ? lane + 64 : 0].tile0 <= tile;
+    const u32 k = (u32)(__popcll(__ballot(a)) + __popcll(__ballot(b))) - 1;
+    return __builtin_amdgcn_readfirstlane(k);
+}
+
+// sum of x0 (x0 + 2 x1) over the tiles of a workgroup -> part[workgroup]
+__global__ __launch_bounds__(256) void sqnorm_kernel(TensorTable tab, u64 *__restrict__ part) {
+    __shared__ u64 ws[4];
+    const u32 tid = threadIdx.x;
     u64 s = 0;
-    for (u64 i = (u64)blockIdx.x * 256 + threadIdx.x; i < n; i += (u64)gridDim.x * 256) s += x0[i] * (x0[i] + 2 * x1[i]);
+    for (u64 tile = blockIdx.x; tile < tab.tiles; tile += gridDim.x) {
+        const u32 k = tensor_of(tab, tile);
+        const u64 at = (tile - tab.t[k].tile0) * LM_TILE, n = tab.t[k].n - at;
+        const u64 *x0 = tab.t[k].x0 + at, *x1 = tab.t[k].x1 + at;
+        if (n >= LM_TILE) {
+#pragma unroll
+            for (u32 u = 0; u < LM_TILE / 512; u++) {
+                const u64x2 a = ld2(x0 + 512 * u + 2 * tid), b = ld2(x1 + 512 * u + 2 * tid);
+                const u64x2 q = a * (a + 2 * b);
+                s += q.x + q.y;
+            }
+        } else {
+            for (u64 i = tid; i < n; i += 256) s += x0[i] * (x0[i] + 2 * x1[i]);
+        }
+    }
     for (u32 d = 32; d; d >>= 1) s += __shfl_xor((unsigned long long)s, d);
-    if ((threadIdx.x & 63) == 0) lm_atomic_add(z, s);
+    if ((tid & 63) == 0) ws[tid >> 6] = s;
+    __syncthreads();
+    if (tid == 0) part[blockIdx.x] = ws[0] + ws[1] + ws[2] + ws[3];
+}
+// z = the sum of the partial sums + A[tA] - B[tB] (one word of each of two generator streams)
+__global__ __launch_bounds__(256) void sqnorm_join_kernel(const u64 *__restrict__ part, u64 parts, const PrgCk *__restrict__ ckA,
+                                                          const PrgCk *__restrict__ ckB, u64 tA, u64 tB, u64 *__restrict__ z) {
+    __shared__ u64 ws[4];
+    const u32 tid = threadIdx.x;
+    u64 s = 0;
+    for (u64 i = tid; i < parts; i += 256) s += part[i];
+    if (tid == 0 || tid == 64) {
+        PrgCursor g;
+        g.open(tid ? ckB : ckA, tid ? tB : tA, true);
+        const u64 w = g.next();
+        s += tid ? 0 - w : w;
+    }
+    for (u32 d = 32; d; d >>= 1) s += __shfl_xor((unsigned long long)s, d);
+    if ((tid & 63) == 0) ws[tid >> 6] = s;
+    __syncthreads();
+    if (tid == 0) *z = ws[0] + ws[1] + ws[2] + ws[3];
 }
 
 // f to the nearest word, ties to even; beyond the range its ends, 0 for what is no number
@@ -50,6 +171,46 @@ __device__ inline u64 clip_factor(u64 S, u64 R, int f) {
     while (c < one && (u128)((c + 1) * (c + 1)) * S <= R2) c++;
     return c;
 }
+
+struct ClipArgs {
+    const u64 *za, *zb, *zc; // the shares of the squared norm
+    u64 R;
+    int number;
+    __device__ u64 factor() const { return clip_factor(*za + *zb + *zc, R, number); }
+};
+// SUM = false: y = (c x0) >> number (party 0; every workgroup forms the factor, which saves a launch); SUM = true: y =
+// ((c (x0 + x1)) >> number) - y, where y holds the words of the stream (party 1; the factor has been written)
+template <bool SUM>
+__global__ __launch_bounds__(256) void clip_kernel(TensorTable tab, ClipArgs A, i64 *__restrict__ coef, u64 *__restrict__ Y) {
+    const u32 tid = threadIdx.x;
+    const u64 c = SUM ? (u64)*coef : A.factor();
+    if (!SUM && blockIdx.x == 0 && tid == 0) *coef = (i64)c;
+    const int sh = A.number;
+    for (u64 tile = blockIdx.x; tile < tab.tiles; tile += gridDim.x) {
+        const u32 k = tensor_of(tab, tile);
+        const u64 at = (tile - tab.t[k].tile0) * LM_TILE, n = tab.t[k].n - at;
+        const u64 *x0 = tab.t[k].x0 + at, *x1 = SUM ? tab.t[k].x1 + at : nullptr;
+        u64 *y = Y + tab.t[k].out + at;
+        if (n >= LM_TILE) {
+#pragma unroll
+            for (u32 u = 0; u < LM_TILE / 512; u++) {
+                const u32 i = 512 * u + 2 * tid;
+                u64x2 a = ld2(x0 + i);
+                if (SUM) a += ld2(x1 + i);
+                a *= c;
+                u64x2 r = {(u64)((i64)a.x >> sh), (u64)((i64)a.y >> sh)};
+                if (SUM) r -= ld2(y + i);
+                st2(y + i, r);
+            }
+        } else {
+            for (u64 i = tid; i < n; i += 256) {
+                const u64 r = (u64)((i64)((SUM ? x0[i] + x1[i] : x0[i]) * c) >> sh);
+                y[i] = SUM ? r - y[i] : r;
+            }
+        }
+    }
+}
+__global__ void clip_factor_kernel(ClipArgs A, i64 *coef) { *coef = (i64)A.factor(); }
 
 struct LogitIn {
     const u64 *a, *b, *c;
@@ -169,13 +330,20 @@ int mpcx_ring_embed(mpcx_ctx *ctx, const int64_t *T0, const int64_t *T1, uint64_
     if (n == 0 || dim == 0) return 0;
     MPCX_REQUIRE(ids && E0 && (T0 || vocab == 0), "mpcx_ring_embed: NULL pointer");
     MPCX_REQUIRE(ctx, "mpcx_ring_embed: the context is NULL");
-    return lm_ew(ctx, n * dim, [=] __device__(u64 i) {
-        const u64 t = i / dim, j = i % dim;
-        const u64 v = (u64)ids[t];
-        const bool ok = v < vocab;
-        E0[i] = ok ? (i64)((u64)T0[v * dim + j] * (u64)scale) >> shift : 0;
-        if (E1) E1[i] = ok ? (i64)((u64)T1[v * dim + j] * (u64)scale) : 0;
-    });
+    const u32 lg = lanes_log2(dim);
+    const u64 slices = ceil_div(dim, 2 * EMB_STEPS << lg);
+    MPCX_REQUIRE(slices < 65536, "mpcx_ring_embed: rows of %llu words", (unsigned long long)dim);
+    u64 blocks = ceil_div(n, 256u >> lg);
+    if (blocks > MPCX_MAX_GRID) blocks = MPCX_MAX_GRID;
+    const dim3 grid((u32)blocks, (u32)slices), block(256);
+    if (T1)
+        hipLaunchKernelGGL(embed_kernel<true>, grid, block, 0, ctx->stream, (const u64 *)T0, (const u64 *)T1, vocab, dim, ids, n,
+                           (u64)scale, shift, (u64 *)E0, (u64 *)E1, lg);
+    else
+        hipLaunchKernelGGL(embed_kernel<false>, grid, block, 0, ctx->stream, (const u64 *)T0, (const u64 *)nullptr, vocab, dim, ids,
+                           n, (u64)scale, shift, (u64 *)E0, (u64 *)nullptr, lg);
+    MPCX_LAUNCH_CHECK();
+    return 0;
 }
 
 uint64_t mpcx_ring_embed_grad_scratch(uint64_t n, uint64_t vocab, uint64_t dim) { return 2 * 8 * vocab * dim + 8; }
@@ -203,7 +371,22 @@ int mpcx_ring_embed_grad(mpcx_ctx *ctx, const int64_t *G0, const int64_t *G1, co
     });
 }
 
-uint64_t mpcx_aby3_sqnorm_scratch(uint64_t count) { return 8; }
+// the next tensors of a call, from tensor `i` on, as one launch's table; advances i and out
+static TensorTable tensor_table(const int64_t *const *X0, const int64_t *const *X1, const uint64_t *lens, u64 count, u64 limit,
+                                u64 &i, u64 &out) {
+    TensorTable tab;
+    tab.count = 0, tab.tiles = 0;
+    for (; i < count && tab.count < LM_TENSORS && lens[i] < limit; i++) {
+        if (lens[i] == 0) continue;
+        tab.t[tab.count++] = TensorRef{X0 ? (const u64 *)X0[i] : nullptr, X1 ? (const u64 *)X1[i] : nullptr, lens[i], out, tab.tiles};
+        tab.tiles += ceil_div(lens[i], LM_TILE);
+        out += lens[i];
+    }
+    return tab;
+}
+static u32 tensor_grid(const TensorTable &tab) { return (u32)(tab.tiles < LM_GRID ? tab.tiles : LM_GRID); }
+
+uint64_t mpcx_aby3_sqnorm_scratch(uint64_t count) { return (ceil_div(count, LM_TENSORS) * LM_GRID + 1) * 8; }
 int mpcx_aby3_sqnorm_local(mpcx_ctx *ctx, const int64_t *const *X0, const int64_t *const *X1, const uint64_t *lens,
                            uint64_t count, uint64_t seed_next, uint64_t pop_next, uint64_t seed_prev, uint64_t pop_prev,
                            void *scratch, int64_t *z0) {
@@ -213,14 +396,21 @@ int mpcx_aby3_sqnorm_local(mpcx_ctx *ctx, const int64_t *const *X0, const int64_
         MPCX_REQUIRE(lens[i] == 0 || (X0[i] && X1[i]), "mpcx_aby3_sqnorm_local: tensor %llu: NULL pointer", (unsigned long long)i);
     }
     MPCX_REQUIRE(ctx, "mpcx_aby3_sqnorm_local: the context is NULL");
-    MPCX_TRY(prg_fill_diff(ctx, seed_next, PRG_POP_T0 + pop_next, seed_prev, PRG_POP_T0 + pop_prev, 1, nullptr, z0));
-    for (u64 i = 0; i < count; i++) {
-        const u64 *x0 = (const u64 *)X0[i], *x1 = (const u64 *)X1[i];
-        if (lens[i] == 0) continue;
-        const u64 blocks = ceil_div(lens[i], 256);
-        hipLaunchKernelGGL(sqnorm_kernel, dim3((u32)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, ctx->stream, x0, x1, lens[i], (u64 *)z0);
+    const PrgCk *ckA, *ckB;
+    const u64 tA = PRG_POP_T0 + pop_next, tB = PRG_POP_T0 + pop_prev;
+    MPCX_TRY(mpcx_prg_table(ctx, seed_next, 0, tA + 1, &ckA));
+    MPCX_TRY(mpcx_prg_table(ctx, seed_prev, 0, tB + 1, &ckB));
+    u64 *part = (u64 *)scratch, parts = 0, out = 0;
+    for (u64 i = 0; i < count;) {
+        const TensorTable tab = tensor_table(X0, X1, lens, count, ~0ull, i, out);
+        if (tab.count == 0) continue;
+        const u32 grid = tensor_grid(tab);
+        hipLaunchKernelGGL(sqnorm_kernel, dim3(grid), dim3(256), 0, ctx->stream, tab, part + parts);
         MPCX_LAUNCH_CHECK();
+        parts += grid;
     }
+    hipLaunchKernelGGL(sqnorm_join_kernel, dim3(1), dim3(256), 0, ctx->stream, part, parts, ckA, ckB, tA, tB, (u64 *)z0);
+    MPCX_LAUNCH_CHECK();
     return 0;
 }
 
@@ -230,7 +420,7 @@ int mpcx_aby3_clip_local(mpcx_ctx *ctx, int party, const int64_t *const *X0, con
     MPCX_REQUIRE(party >= 0 && party <= 2, "mpcx_aby3_clip_local: party %d", party);
     MPCX_REQUIRE(number >= 0 && number <= 31, "mpcx_aby3_clip_local: %d fractional bits", number);
     MPCX_REQUIRE(max_norm < (1ull << (62 - number)), "mpcx_aby3_clip_local: max_norm does not fit %d fractional bits", number);
-    MPCX_REQUIRE(z_prev && z0 && z1 && (count == 0 || lens), "mpcx_aby3_clip_local: NULL pointer");
+    MPCX_REQUIRE(z_prev && z0 && z1 && coef && (count == 0 || lens), "mpcx_aby3_clip_local: NULL pointer");
     const u64 R = max_norm << number;
     u64 at = 0;
     for (u64 i = 0; i < count; i++) {
@@ -240,23 +430,34 @@ int mpcx_aby3_clip_local(mpcx_ctx *ctx, int party, const int64_t *const *X0, con
         at += lens[i];
     }
     MPCX_REQUIRE(ctx, "mpcx_aby3_clip_local: the context is NULL");
-    auto factor = [=] __device__() { return clip_factor((u64)*z_prev + (u64)*z0 + (u64)*z1, R, number); };
-    if (coef) MPCX_TRY(lm_ew(ctx, 1, [=] __device__(u64) { *coef = (i64)factor(); }));
-    at = 0;
-    for (u64 i = 0; i < count; i++) {
-        i64 *y = Y0 + at;
-        if (party == 0) {
-            const u64 *x0 = (const u64 *)X0[i];
-            MPCX_TRY(lm_ew(ctx, lens[i], [=] __device__(u64 j) { y[j] = (i64)(x0[j] * factor()) >> number; }));
-        } else if (party == 1) {
+    const ClipArgs A{(const u64 *)z_prev, (const u64 *)z0, (const u64 *)z1, R, number};
+    if (party || at == 0) {
+        hipLaunchKernelGGL(clip_factor_kernel, dim3(1), dim3(1), 0, ctx->stream, A, coef);
+        MPCX_LAUNCH_CHECK();
+    }
+    u64 *Y = (u64 *)Y0;
+    if (party == 2) return at ? prg_fill_words(ctx, seed12, 0, PRG_POP_T0 + pop12, at, 1, Y0, nullptr) : 0;
+    u64 out = 0;
+    for (u64 i = 0; i < count;) {
+        if (party == 1 && lens[i] >= CLIP_FUSED_WORDS) {
             const u64 *x0 = (const u64 *)X0[i], *x1 = (const u64 *)X1[i];
-            MPCX_TRY(prg_map1(ctx, seed12, PRG_POP_T0 + pop12 + at, lens[i], [=] __device__(u64 j, u64 w) {
-                y[j] = (i64)((u64)((i64)((x0[j] + x1[j]) * factor()) >> number) - w);
+            u64 *y = Y + out;
+            MPCX_TRY(prg_map1(ctx, seed12, PRG_POP_T0 + pop12 + out, lens[i], [=] __device__(u64 j, u64 w) {
+                y[j] = (u64)((i64)((x0[j] + x1[j]) * (u64)*coef) >> number) - w;
             }));
-        } else if (lens[i]) {
-            MPCX_TRY(prg_fill_words(ctx, seed12, 0, PRG_POP_T0 + pop12 + at, lens[i], 1, y, nullptr));
+            out += lens[i++];
+            continue;
         }
-        at += lens[i];
+        const u64 first = out;
+        const TensorTable tab = tensor_table(X0, party == 1 ? X1 : nullptr, lens, count, party == 1 ? CLIP_FUSED_WORDS : ~0ull, i, out);
+        if (tab.count == 0) continue;
+        if (party == 1) {
+            MPCX_TRY(prg_fill_words(ctx, seed12, 0, PRG_POP_T0 + pop12 + first, out - first, 1, (i64 *)Y + first, nullptr));
+            hipLaunchKernelGGL(clip_kernel<true>, dim3(tensor_grid(tab)), dim3(256), 0, ctx->stream, tab, A, coef, Y);
+        } else {
+            hipLaunchKernelGGL(clip_kernel<false>, dim3(tensor_grid(tab)), dim3(256), 0, ctx->stream, tab, A, coef, Y);
+        }
+        MPCX_LAUNCH_CHECK();
     }
     return 0;
 }

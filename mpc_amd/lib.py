@@ -86,18 +86,27 @@ class DeviceArray:
             pass
 
 
-def _a(x):
+def _word(x, keep):
+    """One argument of the C ABI as the 64-bit word that carries it: an address, a size, or an int (whose callee reads the
+    low half).  `keep` holds what must outlive the call."""
+    t = type(x)
+    if t is int:
+        return x
     if x is None:
-        return ctypes.c_void_p(0)
-    if isinstance(x, DeviceArray):
-        return ctypes.c_void_p(x.ptr)
-    if isinstance(x, (int, np.integer)):
-        return ctypes.c_uint64(int(x) & 0xFFFFFFFFFFFFFFFF)
+        return 0
+    if t is DeviceArray:
+        return x.ptr
     if hasattr(x, "data_ptr"):  # torch tensor on the device
-        return ctypes.c_void_p(x.data_ptr())
+        return x.data_ptr()
+    if isinstance(x, (int, np.integer)):
+        return int(x)
+    if isinstance(x, DeviceArray):
+        return x.ptr
     if isinstance(x, (list, tuple)):  # a host array: of device addresses (arrays, tensors) or of counts
-        return (ctypes.c_uint64 * max(len(x), 1))(*[_a(e).value or 0 for e in x])
-    raise TypeError(f"cannot pass {type(x)} to the C ABI")
+        arr = (ctypes.c_uint64 * max(len(x), 1))(*[_word(e, keep) for e in x])
+        keep.append(arr)
+        return ctypes.addressof(arr)
+    raise TypeError(f"cannot pass {t} to the C ABI")
 
 
 class Context:
@@ -111,6 +120,7 @@ class Context:
             raise MpcxError(self.lib.mpcx_last_error(None).decode())
         self.h = h
         self.device = device
+        self._fns = {}  # (name, number of arguments) -> foreign function taking that many 64-bit words
 
     def close(self):
         if self.h:
@@ -126,7 +136,16 @@ class Context:
 
     def call(self, name, *args):
         """Calls ``mpcx_<name>(ctx, *args)``; DeviceArrays / tensors / ints are converted."""
-        self._call("mpcx_" + name, *[_a(x) for x in args])
+        if not self.h:
+            raise MpcxError(f"mpcx_{name}: the context is closed")
+        fn = self._fns.get((name, len(args)))
+        if fn is None:
+            fn = self.lib["mpcx_" + name]  # an object of its own: its argument types do not touch the shared one's
+            fn.argtypes = [ctypes.c_void_p] + [ctypes.c_uint64] * len(args)
+            self._fns[name, len(args)] = fn
+        keep = []
+        if fn(self.h, *[_word(x, keep) for x in args]):
+            raise MpcxError(f"mpcx_{name}: {self.lib.mpcx_last_error(self.h).decode()}")
 
     def scratch_bytes(self, name, *sizes):
         """Bytes of scratch memory that the caller of ``mpcx_<name>`` hands over (mpcx_<name>_scratch)."""

@@ -206,7 +206,7 @@ def test_sqnorm_of_a_tensor_beyond_four_billion_words(resident):
         y = torch.empty(n, dtype=torch.int64, device=dev)
         zero, four = torch.zeros(1, dtype=torch.int64, device=dev), torch.full((1,), 4 << 32, dtype=torch.int64, device=dev)
         x0 <<= 17
-        ctx.call("aby3_clip_local", 0, [x0], [x1], [n], 1, zero, four, zero, 1 << 16, 16, 0, 0, y, None)  # norm 2, bound 1
+        ctx.call("aby3_clip_local", 0, [x0], [x1], [n], 1, zero, four, zero, 1 << 16, 16, 0, 0, y, torch.empty_like(zero))  # norm 2, bound 1
         assert y[0].item() == 1 << 16 and y[n - 2].item() == 1 << 16 and y[n - 1].item() == -5 << 16
         del x0, x1, y
         torch.cuda.empty_cache()
@@ -595,3 +595,17 @@ def test_two_contexts_at_once(resident):
         want = ref.logprobs(x.cpu().numpy(), 16, np.zeros((3, 0), np.int64), 0)[5]
         assert np.abs(ls.cpu().numpy() - want).max() < (100003 / 64 + 70) * STEP + 4 * STEP * np.abs(want).max()
     other.close()
+
+
+def test_clip_of_tensors_on_both_sides_of_the_fused_size(gpu):
+    """Party 1 takes long tensors one by one and short ones together."""
+    rng = np.random.default_rng(77)
+    lens = [(1 << 18) - 1, 5, 1 << 18, 0, 1, (1 << 18) + 4097, 300, 0]
+    X0, X1 = [rnd(rng, n) for n in lens], [rnd(rng, n) for n in lens]
+    z = [np.array([v], np.int64) for v in (25 << 32, 0, 0)]
+    c = ref.clip_factor(25 << 32, 1 << 16, 16)
+    w = prg_pops(KEY12, 9, sum(lens))
+    with np.errstate(over="ignore"):
+        want = ((((np.concatenate(X0) + np.concatenate(X1)) * c) >> 16) - w)
+    y, coef = gpu.aby3_clip_local(1, X0, X1, *z, 1 << 16, 16, KEY12, 9)
+    assert int(coef[0]) == c and np.array_equal(y, want)

@@ -91,7 +91,7 @@ def clip(party=0, X0=None, X1=None, lens=None, count=1, z=(X, X, X), max_norm=1 
     (clip(number=32), "fractional bits"), (clip(number=-1), "fractional bits"),
     (clip(max_norm=1 << 46), "max_norm"),
     (clip(z=(N, X, X)), "NULL"), (clip(z=(X, N, X)), "NULL"), (clip(z=(X, X, N)), "NULL"),
-    (clip(Y0=N), "NULL"), (clip(X0=host(0)), "NULL"), (clip(party=1, X1=host(0)), "NULL"), (clip(X0=N), "NULL"),
+    (clip(Y0=N), "NULL"), (clip(coef=N), "NULL"), (clip(X0=host(0)), "NULL"), (clip(party=1, X1=host(0)), "NULL"), (clip(X0=N), "NULL"),
     (clip(lens=host(1 << 60)), "too long"),
 ])
 def test_clip(lib, args, text):
