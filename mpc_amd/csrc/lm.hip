@@ -212,84 +212,338 @@ __global__ __launch_bounds__(256) void clip_kernel(TensorTable tab, ClipArgs A, 
 }
 __global__ void clip_factor_kernel(ClipArgs A, i64 *coef) { *coef = (i64)A.factor(); }
 
-struct LogitIn {
+// ---- opened logits.  A word x = a + b + c stands for the logit x 2^-frac; distances from a maximum are differences of
+// words, exact before their one conversion to a float.
+template <int SH> struct LogitIn {
     const u64 *a, *b, *c;
     __device__ i64 at(u64 i) const {
         u64 x = a[i];
-        if (b) x += b[i];
-        if (c) x += c[i];
+        if (SH > 1) x += b[i];
+        if (SH > 2) x += c[i];
         return (i64)x;
     }
+    __device__ u64x2 at2(u64 i) const {
+        u64x2 x = ld2(a + i);
+        if (SH > 1) x += ld2(b + i);
+        if (SH > 2) x += ld2(c + i);
+        return x;
+    }
+};
+// hi - lo >= 0 as a float, off by less than two half steps
+__device__ inline float word_dist(i64 hi, i64 lo) {
+    const u64 d = (u64)hi - (u64)lo;
+    return fmaf((float)(u32)(d >> 32), 4294967296.0f, (float)(u32)d);
+}
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); } // v_exp_f32, within one step
+
+__device__ inline i64 lane_word(i64 v, u32 lane) {
+    const u32 lo = (u32)__builtin_amdgcn_readlane((int)(u32)v, (int)lane), hi = (u32)__builtin_amdgcn_readlane((int)((u64)v >> 32), (int)lane);
+    return (i64)((u64)hi << 32 | lo);
+}
+__device__ inline i64 wave_max(i64 v) {
+    for (u32 d = 32; d; d >>= 1) {
+        const i64 o = (i64)__shfl_xor((long long)v, (int)d);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+// The likeliest `top` <= 32 entries a wavefront has seen, best first: entry l in lane l, in the order value descending,
+// index ascending (all entries differ).  (tv, ti) is the last of them, the border that a new one has to beat.
+struct TopEntry {
+    i64 v;
+    u32 i, pad;
+};
+__device__ inline bool top_better(i64 av, u32 ai, i64 bv, u32 bi) { return av > bv || (av == bv && ai < bi); }
+constexpr u32 TOP_NONE = ~0u; // the index of an entry that is not there (with the lowest value: behind all others)
+struct WaveTop {
+    i64 v = INT64_MIN, tv = INT64_MIN;
+    u32 i = TOP_NONE, ti = TOP_NONE;
+    __device__ void border(u32 top) {
+        tv = lane_word(v, top - 1);
+        ti = (u32)__builtin_amdgcn_readlane((int)i, (int)top - 1);
+    }
+    // one candidate per lane; those that beat the border go in one after the other
+    __device__ void insert(u32 top, bool valid, i64 x, u32 idx) {
+        const u32 lane = threadIdx.x & 63;
+        u64 mask = __ballot(valid && top_better(x, idx, tv, ti));
+        while (mask) {
+            const u32 src = (u32)__builtin_ctzll(mask);
+            const i64 cv = lane_word(x, src);
+            const u32 ci = (u32)__builtin_amdgcn_readlane((int)idx, (int)src);
+            const u32 pos = (u32)__popcll(__ballot(top_better(v, i, cv, ci)));
+            const i64 uv = (i64)__shfl_up((long long)v, 1);
+            const u32 ui = (u32)__shfl_up((int)i, 1);
+            if (lane > pos) v = uv, i = ui;
+            if (lane == pos) v = cv, i = ci;
+            border(top);
+            mask &= mask - 1;
+            mask &= __ballot(top_better(x, idx, tv, ti));
+        }
+    }
+};
+// The first tile of a wavefront: N candidates per lane at once.  A distance D is found by bisection such that at least
+// `top` lanes hold something within D of the maximum; what lies within D (rarely more than a few above `top`) is
+// gathered in LDS and sorted by counting, for each, how many are better.  Where more than 64 lie within D (many equal
+// words), or lanes are few, the candidates are inserted one by one.
+template <u32 N>
+__device__ inline void top_first(WaveTop &t, u32 top, const i64 (&x)[N], const u32 (&idx)[N], const bool (&valid)[N], i64 lane_max,
+                                 bool lane_any, TopEntry *buf) {
+    const u32 lane = threadIdx.x & 63;
+    const i64 m = wave_max(lane_any ? lane_max : INT64_MIN);
+    const float near = lane_any ? word_dist(m, lane_max) : INFINITY;
+    float lo = 0, hi = near;
+    if ((u32)__popcll(__ballot(lane_any)) < top) {
+        hi = INFINITY;
+    } else {
+        if (!lane_any) hi = 0;
+        for (u32 d = 32; d; d >>= 1) hi = fmaxf(hi, __shfl_xor(hi, (int)d));
+        for (u32 r = 0; r < 12; r++) {
+            const float mid = 0.5f * (lo + hi);
+            if ((u32)__popcll(__ballot(near <= mid)) >= top)
+                hi = mid;
+            else
+                lo = mid;
+        }
+    }
+    u32 count = 0;
+    u32 slot[N];
+#pragma unroll
+    for (u32 k = 0; k < N; k++) {
+        const u64 b = __ballot(valid[k] && word_dist(m, x[k]) <= hi);
+        slot[k] = ((b >> lane) & 1) ? count + (u32)__popcll(b & ((1ull << lane) - 1)) : TOP_NONE;
+        count += (u32)__popcll(b);
+    }
+    if (count > 64) {
+#pragma unroll
+        for (u32 k = 0; k < N; k++) t.insert(top, valid[k], x[k], idx[k]);
+        return;
+    }
+#pragma unroll
+    for (u32 k = 0; k < N; k++)
+        if (slot[k] != TOP_NONE) buf[slot[k]] = TopEntry{x[k], idx[k], 0};
+    prg_wave_sync();
+    const i64 v = lane < count ? buf[lane].v : INT64_MIN;
+    const u32 i = lane < count ? buf[lane].i : TOP_NONE;
+    u32 rank = 0;
+    for (u32 k = 0; k < count; k++) rank += top_better(buf[k].v, buf[k].i, v, i);
+    prg_wave_sync();
+    if (lane < count) buf[rank] = TopEntry{v, i, 0};
+    prg_wave_sync();
+    if (lane < count && lane < top) t.v = buf[lane].v, t.i = buf[lane].i;
+    prg_wave_sync();
+    t.border(top);
+}
+// The lists of the W wavefronts of a workgroup (in `lists`, `top` entries each) -> out[0 .. top): every entry counts the
+// better ones.  Entries that are not there stay behind the rest.  All threads call it; ends with a barrier.
+template <u32 W> __device__ inline void top_merge(const TopEntry *lists, TopEntry *out, u32 top) {
+    const u32 tid = threadIdx.x, n = W * top;
+    if (tid < top) out[tid] = TopEntry{INT64_MIN, TOP_NONE, 0};
+    __syncthreads();
+    if (tid < n) {
+        const TopEntry e = lists[tid];
+        u32 rank = 0;
+        for (u32 k = 0; k < n; k++) rank += top_better(lists[k].v, lists[k].i, e.v, e.i);
+        if (rank < top && e.i != TOP_NONE) out[rank] = e;
+    }
+    __syncthreads();
+}
+
+// max, sum of 2^-d and sum of d 2^-d, d = (max - x) in units of 1 / log2(e) 2^-frac, over some of a row's words
+struct RowSums {
+    i64 m = INT64_MIN;
+    float S = 0, T = 0;
+    __device__ void move_to(i64 to, float unit2) { // the same sums relative to a larger maximum
+        const float d = word_dist(to, m) * unit2, f = exp2_fast(-d);
+        T = (T + d * S) * f, S *= f, m = to;
+    }
+    __device__ void wave_join(float unit2) {
+        move_to(wave_max(m), unit2);
+        for (u32 d = 32; d; d >>= 1) S += __shfl_xor(S, (int)d), T += __shfl_xor(T, (int)d);
+    }
+};
+struct RowPart {
+    i64 m;
+    float S, T;
 };
 
-__global__ __launch_bounds__(256) void logprobs_kernel(LogitIn in, u64 vocab, float unit, const i64 *__restrict__ ids,
-                                                       u64 per_row, u32 top, float *__restrict__ logp,
-                                                       float *__restrict__ entropy, i64 *__restrict__ top_ids,
-                                                       float *__restrict__ top_logp, i64 *__restrict__ row_max,
-                                                       float *__restrict__ log_sum) {
-    __shared__ i64 sv[256];
-    __shared__ u64 si[256];
-    __shared__ float ss[256], st[256];
-    const u32 tid = threadIdx.x;
-    const u64 row = blockIdx.x, base = row * vocab;
-    // the best (value, index) below (pv, pi) in the order value descending, index ascending
-    auto best_below = [&](bool first, i64 pv, u64 pi) {
-        i64 bv = INT64_MIN;
-        u64 bi = ~0ull;
-        for (u64 j = tid; j < vocab; j += 256) {
-            const i64 x = in.at(base + j);
-            if (!first && !(x < pv || (x == pv && j > pi))) continue;
-            if (bi == ~0ull || x > bv) bv = x, bi = j;
-        }
-        __syncthreads();
-        sv[tid] = bv, si[tid] = bi;
-        __syncthreads();
-        for (u32 s = 128; s; s >>= 1) {
-            if (tid < s) {
-                const i64 ov = sv[tid + s];
-                const u64 oi = si[tid + s];
-                if (oi != ~0ull && (si[tid] == ~0ull || ov > sv[tid] || (ov == sv[tid] && oi < si[tid]))) sv[tid] = ov, si[tid] = oi;
-            }
-            __syncthreads();
-        }
-    };
-    best_below(true, 0, 0);
-    const i64 m = sv[0];
-    float S = 0, T = 0;
-    for (u64 j = tid; j < vocab; j += 256) {
-        const float d = (float)((u64)m - (u64)in.at(base + j)) * unit, e = expf(-d);
-        S += e, T += d * e;
+struct LogprobArgs {
+    u64 rows, vocab;
+    u64 chunk;  // words of a row that one group of wavefronts reads
+    u32 splits; // groups per row
+    u32 top;
+    float unit, unit2; // 2^-frac, 2^-frac log2(e)
+    const i64 *ids;
+    u64 per_row;
+    float *logp, *entropy;
+    i64 *top_ids;
+    float *top_logp;
+    i64 *row_max;
+    float *log_sum;
+    RowPart *parts;  // splits > 1: rows x splits, then
+    TopEntry *lists; // rows x splits x top
+};
+// a row's outputs, by `n` threads (thread `t` of them); list: the row's sorted entries
+template <int SH>
+__device__ inline void logprobs_finish(const LogitIn<SH> &in, const LogprobArgs &A, u64 row, RowSums s, const TopEntry *list, u32 t, u32 n) {
+    const float ls = logf(s.S);
+    if (t == 0) {
+        if (A.entropy) A.entropy[row] = ls + s.T / s.S * 0.69314718f;
+        if (A.row_max) A.row_max[row] = s.m;
+        if (A.log_sum) A.log_sum[row] = ls;
     }
-    ss[tid] = S, st[tid] = T;
-    __syncthreads();
-    for (u32 s = 128; s; s >>= 1) {
-        if (tid < s) ss[tid] += ss[tid + s], st[tid] += st[tid + s];
-        __syncthreads();
+    for (u64 k = t; k < A.per_row; k += n) {
+        const u64 id = (u64)A.ids[row * A.per_row + k];
+        A.logp[row * A.per_row + k] = id < A.vocab ? -(word_dist(s.m, in.at(row * A.vocab + id)) * A.unit + ls) : 0.0f;
     }
-    const float ls = logf(ss[0]);
-    if (tid == 0) {
-        if (entropy) entropy[row] = ls + st[0] / ss[0];
-        if (row_max) row_max[row] = m;
-        if (log_sum) log_sum[row] = ls;
-    }
-    for (u64 t = tid; t < per_row; t += 256) {
-        const i64 id = ids[row * per_row + t];
-        const bool in_range = id >= 0 && (u64)id < vocab;
-        logp[row * per_row + t] = in_range ? -((float)((u64)m - (u64)in.at(base + (u64)id)) * unit + ls) : 0.0f;
-    }
-    i64 pv = 0;
-    u64 pi = 0;
-    for (u32 k = 0; k < top; k++) {
-        best_below(k == 0, pv, pi);
-        pv = sv[0], pi = si[0];
-        if (tid == 0) {
-            top_ids[row * top + k] = (i64)pi;
-            top_logp[row * top + k] = -((float)((u64)m - (u64)pv) * unit + ls);
-        }
+    if (t < A.top) {
+        A.top_ids[row * A.top + t] = (i64)list[t].i;
+        A.top_logp[row * A.top + t] = -(word_dist(s.m, list[t].v) * A.unit + ls);
     }
 }
 
-__global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn in, u64 vocab, float unit, const i64 *__restrict__ ids,
+// W wavefronts of a workgroup of four read `chunk` words of a row, in tiles of 64 x 8 words each.  A lane keeps its own
+// maximum and sums and moves them when a tile raises its maximum; nothing is exchanged between lanes before the end but
+// the ballots that look for new entries of the top list.
+template <u32 W, int SH> __global__ __launch_bounds__(256) void logprobs_kernel(LogitIn<SH> in, LogprobArgs A) {
+    constexpr u32 U = 4, N = 2 * U, TILE = 64 * N;
+    __shared__ TopEntry buf[4][64];
+    __shared__ TopEntry merged[32];
+    __shared__ RowPart ws[4];
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const u64 group = W == 1 ? (u64)blockIdx.x * 4 + wave : blockIdx.x;
+    const u64 row = group / A.splits, split = group % A.splits;
+    if (W == 1 && row >= A.rows) return; // a wavefront of its own: no barrier follows
+    const u64 base = row * A.vocab, j0 = split * A.chunk, j1 = j0 + A.chunk < A.vocab ? j0 + A.chunk : A.vocab;
+    RowSums s;
+    WaveTop top;
+    bool first = true;
+    for (u64 tile = j0 + (W == 1 ? 0 : wave) * TILE; tile < j1; tile += W * TILE) {
+        i64 x[N];
+        u32 idx[N];
+        bool valid[N];
+        if (tile + TILE <= j1) {
+            u64x2 p[U];
+#pragma unroll
+            for (u32 u = 0; u < U; u++) p[u] = in.at2(base + tile + 128 * u + 2 * lane);
+#pragma unroll
+            for (u32 k = 0; k < N; k++) x[k] = (i64)(k & 1 ? p[k / 2].y : p[k / 2].x), valid[k] = true;
+        } else {
+#pragma unroll
+            for (u32 k = 0; k < N; k++) {
+                const u64 j = tile + 128 * (k / 2) + 2 * lane + (k & 1);
+                valid[k] = j < j1;
+                x[k] = valid[k] ? in.at(base + j) : INT64_MIN;
+            }
+        }
+        i64 m = x[0];
+        bool any = valid[0];
+#pragma unroll
+        for (u32 k = 0; k < N; k++) {
+            m = x[k] > m ? x[k] : m;
+            any |= valid[k];
+            idx[k] = (u32)(tile + 128 * (k / 2) + 2 * lane + (k & 1));
+        }
+        if (m > s.m) s.move_to(m, A.unit2);
+#pragma unroll
+        for (u32 k = 0; k < N; k++) {
+            const float d = word_dist(s.m, x[k]) * A.unit2, e = valid[k] ? exp2_fast(-d) : 0.0f;
+            s.S += e, s.T = fmaf(d, e, s.T);
+        }
+        if (A.top) {
+            if (first) {
+                top_first<N>(top, A.top, x, idx, valid, m, any, buf[wave]);
+                first = false;
+            } else if (__ballot(m >= top.tv)) {
+#pragma unroll
+                for (u32 k = 0; k < N; k++) top.insert(A.top, valid[k], x[k], idx[k]);
+            }
+        }
+    }
+    s.wave_join(A.unit2);
+    if (W == 1) {
+        if (lane < A.top) buf[wave][lane] = TopEntry{top.v, top.i, 0};
+        prg_wave_sync();
+        logprobs_finish(in, A, row, s, buf[wave], lane, 64);
+        return;
+    }
+    if (lane == 0) ws[wave] = RowPart{s.m, s.S, s.T};
+    __syncthreads(); // every wavefront has left its own part of buf
+    TopEntry *lists = &buf[0][0];
+    if (lane < A.top) lists[wave * A.top + lane] = TopEntry{top.v, top.i, 0};
+    for (u32 w = 0; w < 4; w++) {
+        RowSums o;
+        o.m = ws[w].m, o.S = ws[w].S, o.T = ws[w].T;
+        if (w == 0) {
+            s = o;
+            continue;
+        }
+        if (o.m > s.m) s.move_to(o.m, A.unit2);
+        else o.move_to(s.m, A.unit2);
+        s.S += o.S, s.T += o.T;
+    }
+    __syncthreads();
+    if (A.top) top_merge<4>(lists, merged, A.top);
+    if (A.splits == 1) {
+        logprobs_finish(in, A, row, s, merged, tid, 256);
+    } else {
+        if (tid == 0) A.parts[group] = RowPart{s.m, s.S, s.T};
+        if (tid < A.top) A.lists[group * A.top + tid] = merged[tid];
+    }
+}
+// joins the parts of a row: one workgroup per row
+template <int SH> __global__ __launch_bounds__(256) void logprobs_join_kernel(LogitIn<SH> in, LogprobArgs A) {
+    constexpr u32 N = 8;
+    __shared__ TopEntry buf[4][64];
+    __shared__ TopEntry merged[32];
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const u64 row = blockIdx.x;
+    const RowPart *parts = A.parts + row * A.splits;
+    RowSums s;
+    for (u32 k = lane; k < A.splits; k += 64) { // every wavefront for itself
+        RowSums o;
+        o.m = parts[k].m, o.S = parts[k].S, o.T = parts[k].T;
+        if (o.m > s.m) s.move_to(o.m, A.unit2);
+        else o.move_to(s.m, A.unit2);
+        s.S += o.S, s.T += o.T;
+    }
+    s.wave_join(A.unit2);
+    if (A.top) {
+        const TopEntry *lists = A.lists + row * A.splits * A.top;
+        const u32 n = A.splits * A.top;
+        WaveTop top;
+        bool first = true;
+        for (u32 tile = wave * 64 * N; tile < n; tile += 4 * 64 * N) {
+            i64 x[N], m = INT64_MIN;
+            u32 idx[N];
+            bool valid[N], any = false;
+#pragma unroll
+            for (u32 k = 0; k < N; k++) {
+                const u32 j = tile + 64 * k + lane;
+                const TopEntry e = j < n ? lists[j] : TopEntry{INT64_MIN, TOP_NONE, 0};
+                x[k] = e.v, idx[k] = e.i, valid[k] = e.i != TOP_NONE, any |= valid[k];
+                m = e.v > m ? e.v : m;
+            }
+            if (first) {
+                top_first<N>(top, A.top, x, idx, valid, m, any, buf[wave]);
+                first = false;
+            } else if (__ballot(any && m >= top.tv)) {
+#pragma unroll
+                for (u32 k = 0; k < N; k++) top.insert(A.top, valid[k], x[k], idx[k]);
+            }
+        }
+        __syncthreads();
+        TopEntry *all = &buf[0][0];
+        if (lane < A.top) all[wave * A.top + lane] = TopEntry{top.v, top.i, 0};
+        __syncthreads();
+        top_merge<4>(all, merged, A.top);
+    }
+    logprobs_finish(in, A, row, s, merged, tid, 256);
+}
+
+// The gradient: one workgroup per row
+template <int SH>
+__global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, u64 vocab, float unit, const i64 *__restrict__ ids,
                                                             u64 per_row, const float *__restrict__ d_logp,
                                                             const float *__restrict__ d_entropy,
                                                             const i64 *__restrict__ row_max, const float *__restrict__ log_sum,
@@ -315,6 +569,22 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn in, u64 voca
         if (grad) grad[base + j] = g;
         if (grad_words) grad_words[base + j] = nearest_word(g * words);
     }
+}
+
+constexpr u64 LP_GROUPS = 1024; // workgroups that fill the chip: four on each CU
+constexpr u64 LP_CHUNK = 2048;  // words: one tile for each of four wavefronts
+constexpr u64 LP_WAVE_ROW = 1024; // rows up to this length are read by one wavefront each
+template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, const LogprobArgs &A) {
+    if (A.splits == 1 && A.vocab <= LP_WAVE_ROW)
+        hipLaunchKernelGGL((logprobs_kernel<1, SH>), dim3((u32)ceil_div(A.rows, 4)), dim3(256), 0, ctx->stream, in, A);
+    else
+        hipLaunchKernelGGL((logprobs_kernel<4, SH>), dim3((u32)(A.rows * A.splits)), dim3(256), 0, ctx->stream, in, A);
+    MPCX_LAUNCH_CHECK();
+    if (A.splits > 1) {
+        hipLaunchKernelGGL(logprobs_join_kernel<SH>, dim3((u32)A.rows), dim3(256), 0, ctx->stream, in, A);
+        MPCX_LAUNCH_CHECK();
+    }
+    return 0;
 }
 
 } // namespace
@@ -462,7 +732,16 @@ int mpcx_aby3_clip_local(mpcx_ctx *ctx, int party, const int64_t *const *X0, con
     return 0;
 }
 
-uint64_t mpcx_reveal_logprobs_scratch(uint64_t rows, uint64_t vocab, uint64_t top) { return 8; }
+// Groups that share a row: enough that the launch has LP_GROUPS workgroups of work, as long as each reads LP_CHUNK words.
+static u64 logprob_chunk(u64 rows, u64 vocab) {
+    u64 splits = rows >= LP_GROUPS ? 1 : LP_GROUPS / (rows ? rows : 1);
+    if (splits > ceil_div(vocab, LP_CHUNK)) splits = ceil_div(vocab, LP_CHUNK);
+    return ceil_div(ceil_div(vocab, splits ? splits : 1), 2048) * 2048;
+}
+uint64_t mpcx_reveal_logprobs_scratch(uint64_t rows, uint64_t vocab, uint64_t top) {
+    const u64 splits = vocab ? ceil_div(vocab, logprob_chunk(rows, vocab)) : 1;
+    return splits > 1 ? rows * splits * (sizeof(RowPart) + top * sizeof(TopEntry)) : 16;
+}
 int mpcx_reveal_logprobs(mpcx_ctx *ctx, const int64_t *a, const int64_t *b, const int64_t *c, uint64_t rows, uint64_t vocab,
                          int frac, const int64_t *ids, uint64_t per_row, uint64_t top, void *scratch, float *logp,
                          float *entropy, int64_t *top_ids, float *top_logp, int64_t *row_max, float *log_sum) {
@@ -475,11 +754,15 @@ int mpcx_reveal_logprobs(mpcx_ctx *ctx, const int64_t *a, const int64_t *b, cons
     MPCX_REQUIRE(a && scratch && (per_row == 0 || (ids && logp)) && (top == 0 || (top_ids && top_logp)),
                  "mpcx_reveal_logprobs: NULL pointer");
     MPCX_REQUIRE(ctx, "mpcx_reveal_logprobs: the context is NULL");
-    const LogitIn in{(const u64 *)a, (const u64 *)b, (const u64 *)c};
-    hipLaunchKernelGGL(logprobs_kernel, dim3((u32)rows), dim3(256), 0, ctx->stream, in, vocab, ldexpf(1.0f, -frac), ids,
-                       per_row, (u32)top, logp, entropy, top_ids, top_logp, row_max, log_sum);
-    MPCX_LAUNCH_CHECK();
-    return 0;
+    LogprobArgs A{};
+    A.rows = rows, A.vocab = vocab, A.chunk = logprob_chunk(rows, vocab), A.splits = (u32)ceil_div(vocab, A.chunk), A.top = (u32)top;
+    A.unit = ldexpf(1.0f, -frac), A.unit2 = ldexpf(1.44269504f, -frac);
+    A.ids = ids, A.per_row = per_row, A.logp = logp, A.entropy = entropy, A.top_ids = top_ids, A.top_logp = top_logp;
+    A.row_max = row_max, A.log_sum = log_sum;
+    A.parts = (RowPart *)scratch, A.lists = (TopEntry *)(A.parts + rows * A.splits);
+    return c ? logprobs_run<3>(ctx, {(const u64 *)a, (const u64 *)b, (const u64 *)c}, A)
+         : b ? logprobs_run<2>(ctx, {(const u64 *)a, (const u64 *)b, nullptr}, A)
+             : logprobs_run<1>(ctx, {(const u64 *)a, nullptr, nullptr}, A);
 }
 
 int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b, const int64_t *c, uint64_t rows,
@@ -495,11 +778,15 @@ int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b,
     MPCX_REQUIRE(a && row_max && log_sum && (grad || grad_words) && (per_row == 0 || (ids && d_logp)) && (!d_entropy || entropy),
                  "mpcx_reveal_logprobs_grad: NULL pointer");
     MPCX_REQUIRE(ctx, "mpcx_reveal_logprobs_grad: the context is NULL");
-    const LogitIn in{(const u64 *)a, (const u64 *)b, (const u64 *)c};
-    hipLaunchKernelGGL(logprobs_grad_kernel, dim3((u32)rows), dim3(256), 0, ctx->stream, in, vocab, ldexpf(1.0f, -frac), ids,
-                       per_row, d_logp, d_entropy, row_max, log_sum, entropy, grad, grad_words, ldexpf(1.0f, grad_frac));
-    MPCX_LAUNCH_CHECK();
-    return 0;
+    auto run = [&](auto in) -> int {
+        hipLaunchKernelGGL(logprobs_grad_kernel, dim3((u32)rows), dim3(256), 0, ctx->stream, in, vocab, ldexpf(1.0f, -frac), ids,
+                           per_row, d_logp, d_entropy, row_max, log_sum, entropy, grad, grad_words, ldexpf(1.0f, grad_frac));
+        MPCX_LAUNCH_CHECK();
+        return 0;
+    };
+    return c ? run(LogitIn<3>{(const u64 *)a, (const u64 *)b, (const u64 *)c})
+         : b ? run(LogitIn<2>{(const u64 *)a, (const u64 *)b, nullptr})
+             : run(LogitIn<1>{(const u64 *)a, nullptr, nullptr});
 }
 
 } // extern "C"
