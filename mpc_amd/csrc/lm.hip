@@ -6,22 +6,8 @@
 
 namespace {
 
-template <class F> __global__ __launch_bounds__(256) void lm_ew_kernel(u64 n, F f) {
-    for (u64 i = (u64)blockIdx.x * 256 + threadIdx.x; i < n; i += (u64)gridDim.x * 256) f(i);
-}
-template <class F> int lm_ew(mpcx_ctx *ctx, u64 n, F f) {
-    if (n == 0) return 0;
-    u64 blocks = ceil_div(n, 256);
-    if (blocks > MPCX_MAX_GRID) blocks = MPCX_MAX_GRID;
-    hipLaunchKernelGGL(lm_ew_kernel<F>, dim3((u32)blocks), dim3(256), 0, ctx->stream, n, f);
-    MPCX_LAUNCH_CHECK();
-    return 0;
-}
-
 // a product of sizes that stays below 2^60 words (every byte count then fits 64 bits)
 bool lm_fits(u64 a, u64 b) { return a == 0 || b <= (1ull << 60) / a; }
-
-__device__ inline void lm_atomic_add(u64 *p, u64 v) { atomicAdd((unsigned long long *)p, (unsigned long long)v); }
 
 // two neighbouring words by one 16-byte access; share arrays are 8-byte aligned only, which the hardware takes
 typedef u64 u64x2 __attribute__((ext_vector_type(2)));
@@ -79,6 +65,269 @@ inline u32 lanes_log2(u64 dim) { // lanes for a row: enough for its 16-byte piec
     u32 lg = 3;
     while (lg < 8 && (2ull << lg) < dim) lg++;
     return lg;
+}
+
+// ---- gradient of the lookup.  Rows of G whose tokens are equal are added; a wavefront (or 2^lg lanes of it) owns a slice
+// of a row of the table, GRAD_STEPS 16-byte pieces of each share per lane.
+constexpr u32 GRAD_STEPS = 4;
+struct GradArgs {
+    const u64 *G0, *G1;
+    const i64 *ids;
+    u64 n, vocab, dim, scale;
+    int shift, accumulate;
+    u64 *D0, *D1;
+};
+template <bool TWO> struct RowAcc {
+    u64x2 a[GRAD_STEPS], b[TWO ? GRAD_STEPS : 1];
+    __device__ RowAcc() {
+#pragma unroll
+        for (u32 u = 0; u < GRAD_STEPS; u++) {
+            a[u] = 0;
+            if (TWO) b[u] = 0;
+        }
+    }
+    // adds columns c0 + u cs (two words each) of one row of each share
+    __device__ void add(const u64 *r0, const u64 *r1, u64 c0, u64 cs, u64 dim) {
+#pragma unroll
+        for (u32 u = 0; u < GRAD_STEPS; u++) {
+            const u64 c = c0 + u * cs;
+            if (c + 1 < dim) {
+                a[u] += ld2(r0 + c);
+                if (TWO) b[u] += ld2(r1 + c);
+            } else if (c < dim) {
+                a[u].x += r0[c];
+                if (TWO) b[u].x += r1[c];
+            }
+        }
+    }
+    // adds the rows of tokens list[i], i = i0, i0 + step, .. below i1, two at a time
+    template <class L> __device__ void add_tokens(const GradArgs &A, const L *list, u32 i0, u32 i1, u32 step, u64 c0, u64 cs) {
+        u32 i = i0;
+        for (; i + step < i1; i += 2 * step) {
+            const u64 t = (u64)list[i] * A.dim, s = (u64)list[i + step] * A.dim;
+            RowAcc o; // its loads go out together with this one's
+            o.add(A.G0 + s, TWO ? A.G1 + s : nullptr, c0, cs, A.dim);
+            add(A.G0 + t, TWO ? A.G1 + t : nullptr, c0, cs, A.dim);
+            join(o);
+        }
+        if (i < i1) {
+            const u64 t = (u64)list[i] * A.dim;
+            add(A.G0 + t, TWO ? A.G1 + t : nullptr, c0, cs, A.dim);
+        }
+    }
+    __device__ void join(const RowAcc &o) {
+#pragma unroll
+        for (u32 u = 0; u < GRAD_STEPS; u++) {
+            a[u] += o.a[u];
+            if (TWO) b[u] += o.b[u];
+        }
+    }
+    __device__ static void put(u64 *p, u64x2 v, bool pair, int accumulate) {
+        if (pair) {
+            if (accumulate) v += ld2(p);
+            st2(p, v);
+        } else {
+            *p = accumulate ? *p + v.x : v.x;
+        }
+    }
+    __device__ void write(const GradArgs &A, u64 row, u64 c0, u64 cs) {
+#pragma unroll
+        for (u32 u = 0; u < GRAD_STEPS; u++) {
+            const u64 c = c0 + u * cs;
+            if (c >= A.dim) continue;
+            u64x2 x = a[u] * A.scale;
+            if (!TWO) x.x = (u64)((i64)x.x >> A.shift), x.y = (u64)((i64)x.y >> A.shift);
+            put(A.D0 + row * A.dim + c, x, c + 1 < A.dim, A.accumulate);
+            if (TWO) put(A.D1 + row * A.dim + c, b[u] * A.scale, c + 1 < A.dim, A.accumulate);
+        }
+    }
+};
+// the sums of four wavefronts in the first one; all threads call it
+template <bool TWO> __device__ inline void join_waves(RowAcc<TWO> &acc, u64x2 *lds) {
+    constexpr u32 P = TWO ? 2 * GRAD_STEPS : GRAD_STEPS;
+    const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();
+    if (wave) {
+#pragma unroll
+        for (u32 u = 0; u < GRAD_STEPS; u++) {
+            lds[((wave - 1) * P + u) * 64 + lane] = acc.a[u];
+            if (TWO) lds[((wave - 1) * P + GRAD_STEPS + u) * 64 + lane] = acc.b[u];
+        }
+    }
+    __syncthreads();
+    if (wave == 0) {
+        for (u32 w = 0; w < 3; w++)
+#pragma unroll
+            for (u32 u = 0; u < GRAD_STEPS; u++) {
+                acc.a[u] += lds[(w * P + u) * 64 + lane];
+                if (TWO) acc.b[u] += lds[(w * P + GRAD_STEPS + u) * 64 + lane];
+            }
+    }
+}
+
+// Few tokens: one launch.  A workgroup owns GRAD_ROWS rows of the table: it looks through all ids, sorts its own tokens by
+// row in LDS, and adds them -- a row of few tokens by one wavefront, a row of many by all four.
+constexpr u32 GRAD_ROWS = 8, GRAD_SMALL_N = 4096, GRAD_ALONE = 8;
+template <bool TWO> __global__ __launch_bounds__(256) void embed_grad_small_kernel(GradArgs A) {
+    __shared__ u16 list[GRAD_SMALL_N];
+    __shared__ u32 cnt[GRAD_ROWS], off[GRAD_ROWS + 1];
+    __shared__ u64x2 lds[3 * (TWO ? 2 : 1) * GRAD_STEPS * 64];
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = (u32)A.n;
+    const u64 v0 = (u64)blockIdx.x * GRAD_ROWS;
+    const u32 rows = (u32)(A.vocab - v0 < GRAD_ROWS ? A.vocab - v0 : GRAD_ROWS);
+    if (tid < GRAD_ROWS) cnt[tid] = 0;
+    __syncthreads();
+    for (u32 t = tid; t < n; t += 256) {
+        const u64 r = (u64)A.ids[t] - v0;
+        if (r < rows) atomicAdd(&cnt[r], 1u);
+    }
+    __syncthreads();
+    if (tid == 0) {
+        u32 s = 0;
+        for (u32 r = 0; r < GRAD_ROWS; r++) {
+            off[r] = s;
+            s += cnt[r];
+            cnt[r] = off[r];
+        }
+        off[GRAD_ROWS] = s;
+    }
+    __syncthreads();
+    if (off[GRAD_ROWS])
+        for (u32 t = tid; t < n; t += 256) {
+            const u64 r = (u64)A.ids[t] - v0;
+            if (r < rows) list[atomicAdd(&cnt[r], 1u)] = (u16)t;
+        }
+    __syncthreads();
+    const u64 c0 = (u64)blockIdx.y * (128 * GRAD_STEPS) + 2 * lane;
+    for (u32 r = wave; r < rows; r += 4) {
+        const u32 k = off[r + 1] - off[r];
+        if (k > GRAD_ALONE || (k == 0 && A.accumulate)) continue;
+        RowAcc<TWO> acc;
+        acc.add_tokens(A, list, off[r], off[r + 1], 1, c0, 128);
+        acc.write(A, v0 + r, c0, 128);
+    }
+    for (u32 r = 0; r < rows; r++) {
+        if (off[r + 1] - off[r] <= GRAD_ALONE) continue;
+        RowAcc<TWO> acc;
+        acc.add_tokens(A, list, off[r] + wave, off[r + 1], 4, c0, 128);
+        join_waves<TWO>(acc, lds);
+        if (wave == 0) acc.write(A, v0 + r, c0, 128);
+    }
+}
+
+// Many tokens: the tokens are put in the order of their rows first (a counting sort, in which the rows' places are taken
+// as they come: sums mod 2^64 do not depend on it), then every row is added by one group of lanes.  A row of more than
+// GRAD_CHUNK tokens is cut into at most GRAD_MAX_CHUNKS chunks, whose sums go through scratch memory.
+constexpr u32 GRAD_CHUNK = 32, GRAD_MAX_CHUNKS = 256;
+struct GradChunk {
+    u32 first, count; // in the ordered tokens
+};
+struct GradHeavy {
+    u32 row, first, count, pad; // its chunks
+};
+struct GradWork {
+    u32 *cursor; // [0] ordered tokens given out, [1] chunks, [2] heavy rows
+    u32 *count, *start, *rank, *order;
+    GradChunk *chunks;
+    GradHeavy *heavy;
+    u64 *partial; // per chunk: dim words of each share
+};
+__global__ __launch_bounds__(256) void grad_clear_kernel(u32 *p, u64 n) {
+    for (u64 i = (u64)blockIdx.x * 256 + threadIdx.x; i < n; i += (u64)gridDim.x * 256) p[i] = 0;
+}
+__global__ __launch_bounds__(256) void grad_count_kernel(const i64 *__restrict__ ids, u32 n, u64 vocab, GradWork W) {
+    const u32 t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= n) return;
+    const u64 v = (u64)ids[t];
+    if (v < vocab) W.rank[t] = atomicAdd(&W.count[v], 1u);
+}
+__global__ __launch_bounds__(256) void grad_place_kernel(u32 vocab, GradWork W) {
+    __shared__ u32 ws[4], at;
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const u32 v = blockIdx.x * 256 + tid;
+    const u32 c = v < vocab ? W.count[v] : 0;
+    u32 s = c; // inclusive sum over the wavefront
+    for (u32 d = 1; d < 64; d <<= 1) {
+        const u32 o = (u32)__shfl_up((int)s, d);
+        if (lane >= d) s += o;
+    }
+    if (lane == 63) ws[wave] = s;
+    __syncthreads();
+    if (tid == 0) {
+        const u32 total = ws[0] + ws[1] + ws[2] + ws[3];
+        at = total ? atomicAdd(&W.cursor[0], total) : 0;
+    }
+    __syncthreads();
+    u32 first = at + s - c;
+    for (u32 w = 0; w < wave; w++) first += ws[w];
+    if (v < vocab) W.start[v] = first;
+    if (c > GRAD_CHUNK) {
+        u32 size = (c + GRAD_MAX_CHUNKS - 1) / GRAD_MAX_CHUNKS;
+        if (size < GRAD_CHUNK) size = GRAD_CHUNK;
+        const u32 k = (c + size - 1) / size;
+        const u32 slot = atomicAdd(&W.cursor[1], k);
+        W.heavy[atomicAdd(&W.cursor[2], 1u)] = GradHeavy{v, slot, k, 0};
+        for (u32 i = 0; i < k; i++) W.chunks[slot + i] = GradChunk{first + i * size, c - i * size < size ? c - i * size : size};
+    }
+}
+__global__ __launch_bounds__(256) void grad_order_kernel(const i64 *__restrict__ ids, u32 n, u64 vocab, GradWork W) {
+    const u32 t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= n) return;
+    const u64 v = (u64)ids[t];
+    if (v < vocab) W.order[W.start[v] + W.rank[t]] = t;
+}
+// The first `heavy_blocks` workgroups add the chunks of the heavy rows into scratch memory, the others one row of the
+// table per 2^lg lanes.
+template <bool TWO> __global__ __launch_bounds__(256) void grad_rows_kernel(GradArgs A, GradWork W, u32 heavy_blocks, u32 lg, u32 slices) {
+    const u32 tid = threadIdx.x;
+    if (blockIdx.x < heavy_blocks) {
+        const u32 lane = tid & 63;
+        const u64 items = (u64)W.cursor[1] * slices;
+        for (u64 it = (u64)blockIdx.x * 4 + (tid >> 6); it < items; it += (u64)heavy_blocks * 4) {
+            const u32 k = (u32)(it / slices), slice = (u32)(it % slices);
+            const GradChunk ch = W.chunks[k];
+            const u64 cs = 2ull << lg, c0 = (u64)slice * cs * GRAD_STEPS + 2 * lane;
+            if (lane >> lg) continue;
+            RowAcc<TWO> acc;
+            acc.add_tokens(A, W.order + ch.first, 0, ch.count, 1, c0, cs);
+            u64 *p = W.partial + (u64)k * 2 * A.dim;
+#pragma unroll
+            for (u32 u = 0; u < GRAD_STEPS; u++) {
+                const u64 c = c0 + u * cs;
+                if (c >= A.dim) continue;
+                RowAcc<TWO>::put(p + c, acc.a[u], c + 1 < A.dim, 0);
+                if (TWO) RowAcc<TWO>::put(p + A.dim + c, acc.b[u], c + 1 < A.dim, 0);
+            }
+        }
+        return;
+    }
+    const u64 item = (((u64)(blockIdx.x - heavy_blocks) * 256 + tid) >> lg);
+    const u64 v = item / slices;
+    if (v >= A.vocab) return;
+    const u32 c = W.count[v];
+    if (c > GRAD_CHUNK || (c == 0 && A.accumulate)) return;
+    const u32 lane = tid & ((1u << lg) - 1);
+    const u64 cs = 2ull << lg, c0 = (item % slices) * cs * GRAD_STEPS + 2 * lane;
+    RowAcc<TWO> acc;
+    if (c) acc.add_tokens(A, W.order + W.start[v], 0, c, 1, c0, cs);
+    acc.write(A, v, c0, cs);
+}
+template <bool TWO> __global__ __launch_bounds__(256) void grad_heavy_kernel(GradArgs A, GradWork W, u32 lg, u32 slices) {
+    __shared__ u64x2 lds[3 * (TWO ? 2 : 1) * GRAD_STEPS * 64];
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const u64 items = (u64)W.cursor[2] * slices;
+    const u64 cs = 2ull << lg;
+    for (u64 it = blockIdx.x; it < items; it += gridDim.x) {
+        const GradHeavy h = W.heavy[it / slices];
+        const u64 c0 = (lane >> lg) ? A.dim : (it % slices) * cs * GRAD_STEPS + 2 * lane; // idle lanes own no column
+        RowAcc<TWO> acc;
+        for (u32 k = wave; k < h.count; k += 4) {
+            const u64 *p = W.partial + (u64)(h.first + k) * 2 * A.dim;
+            acc.add(p, p + A.dim, c0, cs, A.dim);
+        }
+        join_waves<TWO>(acc, lds);
+        if (wave == 0) acc.write(A, h.row, c0, cs);
+    }
 }
 
 // ---- many tensors in one launch.  The tensors of a call are cut into tiles; up to LM_TENSORS descriptors travel in the
@@ -587,6 +836,55 @@ template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, const LogprobA
     return 0;
 }
 
+constexpr u64 GRAD_SMALL_SCAN = 1 << 24;
+// scratch memory of the many-token form, in 8-byte words from its start
+struct GradLayout {
+    u64 cursor, count, start, rank, order, chunks, heavy, partial, words;
+    GradLayout(u64 n, u64 vocab, u64 dim) {
+        // a heavy row has more than GRAD_CHUNK tokens, and its chunks hold GRAD_CHUNK tokens or more, all but the last one
+        const u64 max_heavy = n / (GRAD_CHUNK + 1), max_chunks = n / GRAD_CHUNK + max_heavy;
+        u64 at = 0;
+        auto take = [&](u64 &where, u64 bytes) { where = at, at += ceil_div(bytes, 16) * 2; };
+        take(cursor, 16);
+        take(count, 4 * vocab); // right behind the cursors: cleared together
+        take(start, 4 * vocab);
+        take(rank, 4 * n);
+        take(order, 4 * n);
+        take(chunks, max_chunks * sizeof(GradChunk));
+        take(heavy, max_heavy * sizeof(GradHeavy));
+        take(partial, max_chunks * 2 * dim * 8);
+        words = at;
+    }
+};
+template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *scratch) {
+    if (A.n <= GRAD_SMALL_N && A.n * A.vocab <= GRAD_SMALL_SCAN) {
+        const u64 slices = ceil_div(A.dim, 128 * GRAD_STEPS);
+        MPCX_REQUIRE(slices < 65536, "mpcx_ring_embed_grad: rows of %llu words", (unsigned long long)A.dim);
+        hipLaunchKernelGGL(embed_grad_small_kernel<TWO>, dim3((u32)ceil_div(A.vocab, GRAD_ROWS), (u32)slices), dim3(256), 0,
+                           ctx->stream, A);
+        MPCX_LAUNCH_CHECK();
+        return 0;
+    }
+    const GradLayout L(A.n, A.vocab, A.dim);
+    u64 *w = (u64 *)scratch;
+    const GradWork W{(u32 *)(w + L.cursor), (u32 *)(w + L.count), (u32 *)(w + L.start), (u32 *)(w + L.rank), (u32 *)(w + L.order),
+                     (GradChunk *)(w + L.chunks), (GradHeavy *)(w + L.heavy), w + L.partial};
+    u32 lg = 3; // lanes of a row: up to a wavefront
+    while (lg < 6 && (2ull * GRAD_STEPS << lg) < A.dim) lg++;
+    const u64 slices = ceil_div(A.dim, 2ull * GRAD_STEPS << lg), heavy_blocks = 512;
+    const u64 blocks = ceil_div(A.vocab * slices, 256u >> lg) + heavy_blocks;
+    MPCX_REQUIRE(blocks < (1ull << 31), "mpcx_ring_embed_grad: table too large for one launch");
+    const u32 n = (u32)A.n, tb = (u32)ceil_div(A.n, 256), vb = (u32)ceil_div(A.vocab, 256);
+    hipLaunchKernelGGL(grad_clear_kernel, dim3(vb), dim3(256), 0, ctx->stream, W.cursor, 4 + A.vocab);
+    if (n) hipLaunchKernelGGL(grad_count_kernel, dim3(tb), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
+    hipLaunchKernelGGL(grad_place_kernel, dim3(vb), dim3(256), 0, ctx->stream, (u32)A.vocab, W);
+    if (n) hipLaunchKernelGGL(grad_order_kernel, dim3(tb), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
+    hipLaunchKernelGGL(grad_rows_kernel<TWO>, dim3((u32)blocks), dim3(256), 0, ctx->stream, A, W, (u32)heavy_blocks, lg, (u32)slices);
+    if (n > GRAD_CHUNK) hipLaunchKernelGGL(grad_heavy_kernel<TWO>, dim3(512), dim3(256), 0, ctx->stream, A, W, lg, (u32)slices);
+    MPCX_LAUNCH_CHECK();
+    return 0;
+}
+
 } // namespace
 
 extern "C" {
@@ -616,7 +914,7 @@ int mpcx_ring_embed(mpcx_ctx *ctx, const int64_t *T0, const int64_t *T1, uint64_
     return 0;
 }
 
-uint64_t mpcx_ring_embed_grad_scratch(uint64_t n, uint64_t vocab, uint64_t dim) { return 2 * 8 * vocab * dim + 8; }
+uint64_t mpcx_ring_embed_grad_scratch(uint64_t n, uint64_t vocab, uint64_t dim) { return 8 * GradLayout(n, vocab, dim).words; }
 int mpcx_ring_embed_grad(mpcx_ctx *ctx, const int64_t *G0, const int64_t *G1, const int64_t *ids, uint64_t n, uint64_t vocab,
                          uint64_t dim, int64_t scale, int shift, int accumulate, void *scratch, int64_t *dT0, int64_t *dT1) {
     MPCX_REQUIRE(lm_fits(vocab, dim) && lm_fits(n, dim), "mpcx_ring_embed_grad: sizes too large");
@@ -627,18 +925,8 @@ int mpcx_ring_embed_grad(mpcx_ctx *ctx, const int64_t *G0, const int64_t *G1, co
     if (vocab == 0 || dim == 0) return 0;
     MPCX_REQUIRE(dT0 && scratch && (n == 0 || (ids && G0)), "mpcx_ring_embed_grad: NULL pointer");
     MPCX_REQUIRE(ctx, "mpcx_ring_embed_grad: the context is NULL");
-    u64 *s0 = (u64 *)scratch, *s1 = s0 + vocab * dim;
-    MPCX_TRY(lm_ew(ctx, vocab * dim, [=] __device__(u64 i) { s0[i] = 0, s1[i] = 0; }));
-    MPCX_TRY(lm_ew(ctx, n * dim, [=] __device__(u64 i) {
-        const u64 t = i / dim, j = i % dim, v = (u64)ids[t];
-        if (v >= vocab) return;
-        lm_atomic_add(s0 + v * dim + j, (u64)G0[i]);
-        if (G1) lm_atomic_add(s1 + v * dim + j, (u64)G1[i]);
-    }));
-    return lm_ew(ctx, vocab * dim, [=] __device__(u64 i) {
-        dT0[i] = (i64)((accumulate ? (u64)dT0[i] : 0) + (u64)((i64)(s0[i] * (u64)scale) >> shift));
-        if (dT1) dT1[i] = (i64)((accumulate ? (u64)dT1[i] : 0) + s1[i] * (u64)scale);
-    });
+    const GradArgs A{(const u64 *)G0, (const u64 *)G1, ids, n, vocab, dim, (u64)scale, shift, accumulate, (u64 *)dT0, (u64 *)dT1};
+    return dT1 ? embed_grad_run<true>(ctx, A, scratch) : embed_grad_run<false>(ctx, A, scratch);
 }
 
 // the next tensors of a call, from tensor `i` on, as one launch's table; advances i and out
