@@ -13,12 +13,19 @@ bool lm_fits(u64 a, u64 b) { return a == 0 || b <= (1ull << 60) / a; }
 typedef u64 u64x2 __attribute__((ext_vector_type(2)));
 typedef u64x2 u64x2u __attribute__((aligned(8)));
 __device__ inline u64x2 ld2(const u64 *p) { return *(const u64x2u *)p; }
-__device__ inline void st2(u64 *p, u64x2 v) { *(u64x2u *)p = v; }
+// STREAM: the hint that the words are not read again soon, for outputs larger than the last-level cache (OUT_STREAM)
+template <bool STREAM = false> __device__ inline void st2(u64 *p, u64x2 v) {
+    if (STREAM)
+        __builtin_nontemporal_store(v, (u64x2u *)p);
+    else
+        *(u64x2u *)p = v;
+}
+constexpr u64 OUT_STREAM = 256ull << 20; // bytes
 
 // ---- lookup.  A row is copied by 2^lg lanes (8 .. 256) of a workgroup, 16 bytes of each share per lane and step; the
 // four steps of a lane are all requested before the first is used.
 constexpr u32 EMB_STEPS = 4;
-template <bool TWO>
+template <bool TWO, bool STREAM>
 __global__ __launch_bounds__(256) void embed_kernel(const u64 *__restrict__ T0, const u64 *__restrict__ T1, u64 vocab, u64 dim,
                                                     const i64 *__restrict__ ids, u64 n, u64 scale, int shift,
                                                     u64 *__restrict__ E0, u64 *__restrict__ E1, u32 lg) {
@@ -52,8 +59,8 @@ __global__ __launch_bounds__(256) void embed_kernel(const u64 *__restrict__ T0, 
                 x.x = (u64)((i64)(a[u].x * scale) >> shift), x.y = (u64)((i64)(a[u].y * scale) >> shift);
             }
             if (c + 1 < dim) {
-                st2(E0 + t * dim + c, x);
-                if (TWO) st2(E1 + t * dim + c, y);
+                st2<STREAM>(E0 + t * dim + c, x);
+                if (TWO) st2<STREAM>(E1 + t * dim + c, y);
             } else {
                 E0[t * dim + c] = x.x;
                 if (TWO) E1[t * dim + c] = y.x;
@@ -68,8 +75,8 @@ inline u32 lanes_log2(u64 dim) { // lanes for a row: enough for its 16-byte piec
 }
 
 // ---- gradient of the lookup.  Rows of G whose tokens are equal are added; a wavefront (or 2^lg lanes of it) owns a slice
-// of a row of the table, GRAD_STEPS 16-byte pieces of each share per lane.
-constexpr u32 GRAD_STEPS = 4;
+// of a row of the table, NS 16-byte pieces of each share per lane, and adds NT tokens at a time: NS NT loads of each share
+// are under way together.
 struct GradArgs {
     const u64 *G0, *G1;
     const i64 *ids;
@@ -77,11 +84,11 @@ struct GradArgs {
     int shift, accumulate;
     u64 *D0, *D1;
 };
-template <bool TWO> struct RowAcc {
-    u64x2 a[GRAD_STEPS], b[TWO ? GRAD_STEPS : 1];
+template <bool TWO, u32 NS> struct RowAcc {
+    u64x2 a[NS], b[TWO ? NS : 1];
     __device__ RowAcc() {
 #pragma unroll
-        for (u32 u = 0; u < GRAD_STEPS; u++) {
+        for (u32 u = 0; u < NS; u++) {
             a[u] = 0;
             if (TWO) b[u] = 0;
         }
@@ -89,7 +96,7 @@ template <bool TWO> struct RowAcc {
     // adds columns c0 + u cs (two words each) of one row of each share
     __device__ void add(const u64 *r0, const u64 *r1, u64 c0, u64 cs, u64 dim) {
 #pragma unroll
-        for (u32 u = 0; u < GRAD_STEPS; u++) {
+        for (u32 u = 0; u < NS; u++) {
             const u64 c = c0 + u * cs;
             if (c + 1 < dim) {
                 a[u] += ld2(r0 + c);
@@ -100,78 +107,87 @@ template <bool TWO> struct RowAcc {
             }
         }
     }
-    // adds the rows of tokens list[i], i = i0, i0 + step, .. below i1, two at a time
-    template <class L> __device__ void add_tokens(const GradArgs &A, const L *list, u32 i0, u32 i1, u32 step, u64 c0, u64 cs) {
+    // adds the rows row(i) of p0 / p1, i = i0, i0 + step, .. below i1, NT at a time
+    template <u32 NT, class F>
+    __device__ void add_rows(F row, const u64 *p0, const u64 *p1, u32 i0, u32 i1, u32 step, u64 c0, u64 cs, u64 dim) {
         u32 i = i0;
-        for (; i + step < i1; i += 2 * step) {
-            const u64 t = (u64)list[i] * A.dim, s = (u64)list[i + step] * A.dim;
-            RowAcc o; // its loads go out together with this one's
-            o.add(A.G0 + s, TWO ? A.G1 + s : nullptr, c0, cs, A.dim);
-            add(A.G0 + t, TWO ? A.G1 + t : nullptr, c0, cs, A.dim);
-            join(o);
-        }
-        if (i < i1) {
-            const u64 t = (u64)list[i] * A.dim;
-            add(A.G0 + t, TWO ? A.G1 + t : nullptr, c0, cs, A.dim);
-        }
-    }
-    __device__ void join(const RowAcc &o) {
+        for (; NT > 1 && i + (NT - 1) * step < i1; i += NT * step) {
+            u64 at[NT];
+            u64x2 x[NT * NS], y[TWO ? NT * NS : 1];
 #pragma unroll
-        for (u32 u = 0; u < GRAD_STEPS; u++) {
-            a[u] += o.a[u];
-            if (TWO) b[u] += o.b[u];
+            for (u32 q = 0; q < NT; q++) at[q] = row(i + q * step);
+#pragma unroll
+            for (u32 u = 0; u < NS; u++) {
+                const u64 c = c0 + u * cs;
+#pragma unroll
+                for (u32 q = 0; q < NT; q++) {
+                    x[u * NT + q] = 0;
+                    if (TWO) y[u * NT + q] = 0;
+                    if (c + 1 < dim) {
+                        x[u * NT + q] = ld2(p0 + at[q] + c);
+                        if (TWO) y[u * NT + q] = ld2(p1 + at[q] + c);
+                    } else if (c < dim) {
+                        x[u * NT + q].x = p0[at[q] + c];
+                        if (TWO) y[u * NT + q].x = p1[at[q] + c];
+                    }
+                }
+            }
+#pragma unroll
+            for (u32 u = 0; u < NS; u++)
+#pragma unroll
+                for (u32 q = 0; q < NT; q++) {
+                    a[u] += x[u * NT + q];
+                    if (TWO) b[u] += y[u * NT + q];
+                }
+        }
+        for (; i < i1; i += step) {
+            const u64 at = row(i);
+            add(p0 + at, TWO ? p1 + at : nullptr, c0, cs, dim);
         }
     }
-    __device__ static void put(u64 *p, u64x2 v, bool pair, int accumulate) {
+    template <bool STREAM> __device__ static void put(u64 *p, u64x2 v, bool pair, int accumulate) {
         if (pair) {
             if (accumulate) v += ld2(p);
-            st2(p, v);
+            st2<STREAM>(p, v);
         } else {
             *p = accumulate ? *p + v.x : v.x;
         }
     }
-    __device__ void write(const GradArgs &A, u64 row, u64 c0, u64 cs) {
+    template <bool STREAM> __device__ void write(const GradArgs &A, u64 row, u64 c0, u64 cs) {
 #pragma unroll
-        for (u32 u = 0; u < GRAD_STEPS; u++) {
+        for (u32 u = 0; u < NS; u++) {
             const u64 c = c0 + u * cs;
             if (c >= A.dim) continue;
             u64x2 x = a[u] * A.scale;
             if (!TWO) x.x = (u64)((i64)x.x >> A.shift), x.y = (u64)((i64)x.y >> A.shift);
-            put(A.D0 + row * A.dim + c, x, c + 1 < A.dim, A.accumulate);
-            if (TWO) put(A.D1 + row * A.dim + c, b[u] * A.scale, c + 1 < A.dim, A.accumulate);
+            put<STREAM>(A.D0 + row * A.dim + c, x, c + 1 < A.dim, A.accumulate);
+            if (TWO) put<STREAM>(A.D1 + row * A.dim + c, b[u] * A.scale, c + 1 < A.dim, A.accumulate);
         }
     }
 };
-// the sums of four wavefronts in the first one; all threads call it
-template <bool TWO> __device__ inline void join_waves(RowAcc<TWO> &acc, u64x2 *lds) {
-    constexpr u32 P = TWO ? 2 * GRAD_STEPS : GRAD_STEPS;
+// the sums of four wavefronts in the first one (one 16-byte piece of each share per lane); all threads call it
+template <bool TWO> __device__ inline void join_waves(RowAcc<TWO, 1> &acc, u64x2 *lds) {
     const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
     if (wave) {
-#pragma unroll
-        for (u32 u = 0; u < GRAD_STEPS; u++) {
-            lds[((wave - 1) * P + u) * 64 + lane] = acc.a[u];
-            if (TWO) lds[((wave - 1) * P + GRAD_STEPS + u) * 64 + lane] = acc.b[u];
-        }
+        lds[(wave - 1) * 64 + lane] = acc.a[0];
+        if (TWO) lds[(wave + 2) * 64 + lane] = acc.b[0];
     }
     __syncthreads();
-    if (wave == 0) {
-        for (u32 w = 0; w < 3; w++)
-#pragma unroll
-            for (u32 u = 0; u < GRAD_STEPS; u++) {
-                acc.a[u] += lds[(w * P + u) * 64 + lane];
-                if (TWO) acc.b[u] += lds[(w * P + GRAD_STEPS + u) * 64 + lane];
-            }
-    }
+    if (wave == 0)
+        for (u32 w = 0; w < 3; w++) {
+            acc.a[0] += lds[w * 64 + lane];
+            if (TWO) acc.b[0] += lds[(w + 3) * 64 + lane];
+        }
 }
 
-// Few tokens: one launch.  A workgroup owns GRAD_ROWS rows of the table: it looks through all ids, sorts its own tokens by
-// row in LDS, and adds them -- a row of few tokens by one wavefront, a row of many by all four.
+// Few tokens: one launch.  A workgroup owns GRAD_ROWS rows of the table, 128 columns of them: it looks through all ids,
+// sorts its own tokens by row in LDS, and adds them -- a row of few tokens by one wavefront, a row of many by all four.
 constexpr u32 GRAD_ROWS = 8, GRAD_SMALL_N = 4096, GRAD_ALONE = 8;
 template <bool TWO> __global__ __launch_bounds__(256) void embed_grad_small_kernel(GradArgs A) {
     __shared__ u16 list[GRAD_SMALL_N];
     __shared__ u32 cnt[GRAD_ROWS], off[GRAD_ROWS + 1];
-    __shared__ u64x2 lds[3 * (TWO ? 2 : 1) * GRAD_STEPS * 64];
+    __shared__ u64x2 lds[3 * (TWO ? 2 : 1) * 64];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = (u32)A.n;
     const u64 v0 = (u64)blockIdx.x * GRAD_ROWS;
     const u32 rows = (u32)(A.vocab - v0 < GRAD_ROWS ? A.vocab - v0 : GRAD_ROWS);
@@ -198,27 +214,28 @@ template <bool TWO> __global__ __launch_bounds__(256) void embed_grad_small_kern
             if (r < rows) list[atomicAdd(&cnt[r], 1u)] = (u16)t;
         }
     __syncthreads();
-    const u64 c0 = (u64)blockIdx.y * (128 * GRAD_STEPS) + 2 * lane;
+    const u64 c0 = (u64)blockIdx.y * 128 + 2 * lane;
+    auto row = [&](u32 i) { return (u64)list[i] * A.dim; };
     for (u32 r = wave; r < rows; r += 4) {
         const u32 k = off[r + 1] - off[r];
         if (k > GRAD_ALONE || (k == 0 && A.accumulate)) continue;
-        RowAcc<TWO> acc;
-        acc.add_tokens(A, list, off[r], off[r + 1], 1, c0, 128);
-        acc.write(A, v0 + r, c0, 128);
+        RowAcc<TWO, 1> acc;
+        acc.template add_rows<4>(row, A.G0, A.G1, off[r], off[r + 1], 1, c0, 0, A.dim);
+        acc.template write<false>(A, v0 + r, c0, 0);
     }
     for (u32 r = 0; r < rows; r++) {
         if (off[r + 1] - off[r] <= GRAD_ALONE) continue;
-        RowAcc<TWO> acc;
-        acc.add_tokens(A, list, off[r] + wave, off[r + 1], 4, c0, 128);
+        RowAcc<TWO, 1> acc;
+        acc.template add_rows<8>(row, A.G0, A.G1, off[r] + wave, off[r + 1], 4, c0, 0, A.dim);
         join_waves<TWO>(acc, lds);
-        if (wave == 0) acc.write(A, v0 + r, c0, 128);
+        if (wave == 0) acc.template write<false>(A, v0 + r, c0, 0);
     }
 }
 
 // Many tokens: the tokens are put in the order of their rows first (a counting sort, in which the rows' places are taken
 // as they come: sums mod 2^64 do not depend on it), then every row is added by one group of lanes.  A row of more than
 // GRAD_CHUNK tokens is cut into at most GRAD_MAX_CHUNKS chunks, whose sums go through scratch memory.
-constexpr u32 GRAD_CHUNK = 32, GRAD_MAX_CHUNKS = 256;
+constexpr u32 GRAD_TOGETHER = 4, GRAD_CHUNK = 32, GRAD_MAX_CHUNKS = 256;
 struct GradChunk {
     u32 first, count; // in the ordered tokens
 };
@@ -235,11 +252,39 @@ struct GradWork {
 __global__ __launch_bounds__(256) void grad_clear_kernel(u32 *p, u64 n) {
     for (u64 i = (u64)blockIdx.x * 256 + threadIdx.x; i < n; i += (u64)gridDim.x * 256) p[i] = 0;
 }
+// count[v] = tokens of row v, rank[t] = place of token t among those of its row.  A workgroup first counts its own
+// tokens in a hash table in LDS, then adds each row's number to memory once: the frequent tokens of a text would
+// otherwise queue up at one address (65536 tokens, one in sixteen the same: 48 us).
+constexpr u32 GRAD_TOKENS = 1024, GRAD_SLOTS = 2048; // per workgroup of 256: tokens, slots of its table
 __global__ __launch_bounds__(256) void grad_count_kernel(const i64 *__restrict__ ids, u32 n, u64 vocab, GradWork W) {
-    const u32 t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= n) return;
-    const u64 v = (u64)ids[t];
-    if (v < vocab) W.rank[t] = atomicAdd(&W.count[v], 1u);
+    __shared__ u32 key[GRAD_SLOTS], num[GRAD_SLOTS];
+    const u32 tid = threadIdx.x;
+    for (u32 i = tid; i < GRAD_SLOTS; i += 256) key[i] = ~0u, num[i] = 0;
+    __syncthreads();
+    u32 slot[GRAD_TOKENS / 256], rank[GRAD_TOKENS / 256];
+#pragma unroll
+    for (u32 q = 0; q < GRAD_TOKENS / 256; q++) {
+        const u32 t = blockIdx.x * GRAD_TOKENS + 256 * q + tid;
+        const u64 v = t < n ? (u64)ids[t] : vocab;
+        slot[q] = ~0u;
+        if (v < vocab) {
+            u32 h = (u32)v * 2654435761u >> 21; // the table has a free slot for every token
+            for (;;) {
+                const u32 k = atomicCAS(&key[h], ~0u, (u32)v);
+                if (k == ~0u || k == (u32)v) break;
+                h = (h + 1) & (GRAD_SLOTS - 1);
+            }
+            slot[q] = h;
+            rank[q] = atomicAdd(&num[h], 1u);
+        }
+    }
+    __syncthreads();
+    for (u32 i = tid; i < GRAD_SLOTS; i += 256)
+        if (num[i]) num[i] = atomicAdd(&W.count[key[i]], num[i]);
+    __syncthreads();
+#pragma unroll
+    for (u32 q = 0; q < GRAD_TOKENS / 256; q++)
+        if (slot[q] != ~0u) W.rank[blockIdx.x * GRAD_TOKENS + 256 * q + tid] = num[slot[q]] + rank[q];
 }
 __global__ __launch_bounds__(256) void grad_place_kernel(u32 vocab, GradWork W) {
     __shared__ u32 ws[4], at;
@@ -261,13 +306,18 @@ __global__ __launch_bounds__(256) void grad_place_kernel(u32 vocab, GradWork W) 
     u32 first = at + s - c;
     for (u32 w = 0; w < wave; w++) first += ws[w];
     if (v < vocab) W.start[v] = first;
+    u32 size = 0, k = 0, slot = 0;
     if (c > GRAD_CHUNK) {
-        u32 size = (c + GRAD_MAX_CHUNKS - 1) / GRAD_MAX_CHUNKS;
+        size = (c + GRAD_MAX_CHUNKS - 1) / GRAD_MAX_CHUNKS;
         if (size < GRAD_CHUNK) size = GRAD_CHUNK;
-        const u32 k = (c + size - 1) / size;
-        const u32 slot = atomicAdd(&W.cursor[1], k);
+        k = (c + size - 1) / size;
+        slot = atomicAdd(&W.cursor[1], k);
         W.heavy[atomicAdd(&W.cursor[2], 1u)] = GradHeavy{v, slot, k, 0};
-        for (u32 i = 0; i < k; i++) W.chunks[slot + i] = GradChunk{first + i * size, c - i * size < size ? c - i * size : size};
+    }
+    for (u64 heavy = __ballot(k != 0); heavy; heavy &= heavy - 1) { // a row's chunks are written by the whole wavefront
+        const int src = __builtin_ctzll(heavy);
+        const u32 hk = __shfl(k, src), hs = __shfl(size, src), hf = __shfl(first, src), hc = __shfl(c, src), hb = __shfl(slot, src);
+        for (u32 i = lane; i < hk; i += 64) W.chunks[hb + i] = GradChunk{hf + i * hs, hc - i * hs < hs ? hc - i * hs : hs};
     }
 }
 __global__ __launch_bounds__(256) void grad_order_kernel(const i64 *__restrict__ ids, u32 n, u64 vocab, GradWork W) {
@@ -276,57 +326,49 @@ __global__ __launch_bounds__(256) void grad_order_kernel(const i64 *__restrict__
     const u64 v = (u64)ids[t];
     if (v < vocab) W.order[W.start[v] + W.rank[t]] = t;
 }
-// The first `heavy_blocks` workgroups add the chunks of the heavy rows into scratch memory, the others one row of the
-// table per 2^lg lanes.
-template <bool TWO> __global__ __launch_bounds__(256) void grad_rows_kernel(GradArgs A, GradWork W, u32 heavy_blocks, u32 lg, u32 slices) {
-    const u32 tid = threadIdx.x;
+// The first `heavy_blocks` workgroups add the chunks of the heavy rows into scratch memory, 128 columns per wavefront; the
+// others one row of the table, 128 columns or less, per 2^lg lanes.
+template <bool TWO, bool STREAM>
+__global__ __launch_bounds__(256) void grad_rows_kernel(GradArgs A, GradWork W, u32 heavy_blocks, u32 lg, u32 slices) {
+    RowAcc<TWO, 1> acc;
     if (blockIdx.x < heavy_blocks) {
-        const u32 lane = tid & 63;
         const u64 items = (u64)W.cursor[1] * slices;
-        for (u64 it = (u64)blockIdx.x * 4 + (tid >> 6); it < items; it += (u64)heavy_blocks * 4) {
-            const u32 k = (u32)(it / slices), slice = (u32)(it % slices);
+        for (u64 it = (u64)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += (u64)heavy_blocks * 4) {
+            const u64 k = it / slices, c0 = (it % slices) * 128 + 2 * (threadIdx.x & 63);
             const GradChunk ch = W.chunks[k];
-            const u64 cs = 2ull << lg, c0 = (u64)slice * cs * GRAD_STEPS + 2 * lane;
-            if (lane >> lg) continue;
-            RowAcc<TWO> acc;
-            acc.add_tokens(A, W.order + ch.first, 0, ch.count, 1, c0, cs);
-            u64 *p = W.partial + (u64)k * 2 * A.dim;
-#pragma unroll
-            for (u32 u = 0; u < GRAD_STEPS; u++) {
-                const u64 c = c0 + u * cs;
-                if (c >= A.dim) continue;
-                RowAcc<TWO>::put(p + c, acc.a[u], c + 1 < A.dim, 0);
-                if (TWO) RowAcc<TWO>::put(p + A.dim + c, acc.b[u], c + 1 < A.dim, 0);
-            }
+            const u32 *list = W.order + ch.first;
+            acc = RowAcc<TWO, 1>();
+            acc.template add_rows<GRAD_TOGETHER>([&](u32 i) { return (u64)list[i] * A.dim; }, A.G0, A.G1, 0, ch.count, 1, c0, 0, A.dim);
+            if (c0 >= A.dim) continue;
+            u64 *p = W.partial + k * 2 * A.dim + c0;
+            acc.template put<false>(p, acc.a[0], c0 + 1 < A.dim, 0);
+            if (TWO) acc.template put<false>(p + A.dim, acc.b[0], c0 + 1 < A.dim, 0);
         }
         return;
     }
-    const u64 item = (((u64)(blockIdx.x - heavy_blocks) * 256 + tid) >> lg);
+    const u64 item = ((u64)(blockIdx.x - heavy_blocks) * 256 + threadIdx.x) >> lg;
     const u64 v = item / slices;
     if (v >= A.vocab) return;
     const u32 c = W.count[v];
     if (c > GRAD_CHUNK || (c == 0 && A.accumulate)) return;
-    const u32 lane = tid & ((1u << lg) - 1);
-    const u64 cs = 2ull << lg, c0 = (item % slices) * cs * GRAD_STEPS + 2 * lane;
-    RowAcc<TWO> acc;
-    if (c) acc.add_tokens(A, W.order + W.start[v], 0, c, 1, c0, cs);
-    acc.write(A, v, c0, cs);
+    const u64 c0 = (item % slices) * 128 + 2 * (threadIdx.x & ((1u << lg) - 1));
+    const u32 *list = W.order + (c ? W.start[v] : 0);
+    acc.template add_rows<GRAD_TOGETHER>([&](u32 i) { return (u64)list[i] * A.dim; }, A.G0, A.G1, 0, c, 1, c0, 0, A.dim);
+    acc.template write<STREAM>(A, v, c0, 0);
 }
-template <bool TWO> __global__ __launch_bounds__(256) void grad_heavy_kernel(GradArgs A, GradWork W, u32 lg, u32 slices) {
-    __shared__ u64x2 lds[3 * (TWO ? 2 : 1) * GRAD_STEPS * 64];
+// a heavy row's 128 columns: its chunks' sums, shared out to the four wavefronts of a workgroup
+template <bool TWO> __global__ __launch_bounds__(256) void grad_heavy_kernel(GradArgs A, GradWork W) {
+    __shared__ u64x2 lds[3 * (TWO ? 2 : 1) * 64];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const u64 items = (u64)W.cursor[2] * slices;
-    const u64 cs = 2ull << lg;
+    const u64 slices = (A.dim + 127) / 128, items = (u64)W.cursor[2] * slices;
     for (u64 it = blockIdx.x; it < items; it += gridDim.x) {
         const GradHeavy h = W.heavy[it / slices];
-        const u64 c0 = (lane >> lg) ? A.dim : (it % slices) * cs * GRAD_STEPS + 2 * lane; // idle lanes own no column
-        RowAcc<TWO> acc;
-        for (u32 k = wave; k < h.count; k += 4) {
-            const u64 *p = W.partial + (u64)(h.first + k) * 2 * A.dim;
-            acc.add(p, p + A.dim, c0, cs, A.dim);
-        }
+        const u64 c0 = (it % slices) * 128 + 2 * lane;
+        const u64 *p = W.partial + (u64)h.first * 2 * A.dim;
+        RowAcc<TWO, 1> acc;
+        acc.template add_rows<8>([&](u32 i) { return (u64)i * 2 * A.dim; }, p, p + A.dim, wave, h.count, 4, c0, 0, A.dim);
         join_waves<TWO>(acc, lds);
-        if (wave == 0) acc.write(A, h.row, c0, cs);
+        if (wave == 0) acc.template write<false>(A, h.row, c0, 0);
     }
 }
 
@@ -575,6 +617,7 @@ __device__ inline void top_first(WaveTop &t, u32 top, const i64 (&x)[N], const u
     const i64 v = lane < count ? buf[lane].v : INT64_MIN;
     const u32 i = lane < count ? buf[lane].i : TOP_NONE;
     u32 rank = 0;
+#pragma unroll 8
     for (u32 k = 0; k < count; k++) rank += top_better(buf[k].v, buf[k].i, v, i);
     prg_wave_sync();
     if (lane < count) buf[rank] = TopEntry{v, i, 0};
@@ -592,6 +635,7 @@ template <u32 W> __device__ inline void top_merge(const TopEntry *lists, TopEntr
     if (tid < n) {
         const TopEntry e = lists[tid];
         u32 rank = 0;
+#pragma unroll 8
         for (u32 k = 0; k < n; k++) rank += top_better(lists[k].v, lists[k].i, e.v, e.i);
         if (rank < top && e.i != TOP_NONE) out[rank] = e;
     }
@@ -790,33 +834,90 @@ template <int SH> __global__ __launch_bounds__(256) void logprobs_join_kernel(Lo
     logprobs_finish(in, A, row, s, merged, tid, 256);
 }
 
-// The gradient: one workgroup per row
-template <int SH>
-__global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, u64 vocab, float unit, const i64 *__restrict__ ids,
-                                                            u64 per_row, const float *__restrict__ d_logp,
-                                                            const float *__restrict__ d_entropy,
-                                                            const i64 *__restrict__ row_max, const float *__restrict__ log_sum,
-                                                            const float *__restrict__ entropy, float *__restrict__ grad,
-                                                            i64 *__restrict__ grad_words, float words) {
-    const u64 row = blockIdx.x, base = row * vocab;
-    const i64 m = row_max[row];
-    const float ls = log_sum[row];
-    const float h = d_entropy ? d_entropy[row] : 0.0f, H = d_entropy ? entropy[row] : 0.0f;
+// The gradient.  A workgroup takes `chunk` words of a row, 16 bytes of each share per load and GRAD_PAIRS of them together;
+// the words of the given ids are written again at the end with their own terms added, so that the pass itself knows no
+// ids and every word is rounded once.
+#ifndef LM_GP
+#define LM_GP 4
+#endif
+#ifndef LM_GNT
+#define LM_GNT 1
+#endif
+constexpr u32 GRAD_PAIRS = LM_GP;
+struct LogprobGradArgs {
+    u64 vocab, chunk;
+    u32 splits;
+    float unit, words; // 2^-frac, 2^grad_frac
+    const i64 *ids;
+    u64 per_row;
+    const float *d_logp, *d_entropy;
+    const i64 *row_max;
+    const float *log_sum, *entropy;
+    float *grad;
+    i64 *grad_words;
+};
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef f32x2 f32x2u __attribute__((aligned(4)));
+template <int SH, bool STREAM> __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, LogprobGradArgs A) {
+    __shared__ float ws[4];
+    const u32 tid = threadIdx.x;
+    const u64 row = blockIdx.x / A.splits, split = blockIdx.x % A.splits, base = row * A.vocab;
+    const u64 j0 = split * A.chunk, j1 = j0 + A.chunk < A.vocab ? j0 + A.chunk : A.vocab;
+    const i64 m = A.row_max[row];
+    const float ls = A.log_sum[row], h = A.d_entropy ? A.d_entropy[row] : 0.0f, H = A.d_entropy ? A.entropy[row] : 0.0f;
+    const i64 *ids = A.ids + row * A.per_row;
+    const float *dl = A.d_logp + row * A.per_row;
     float w = 0;
-    for (u64 t = 0; t < per_row; t++) {
-        const i64 id = ids[row * per_row + t];
-        if (id >= 0 && (u64)id < vocab) w += d_logp[row * per_row + t];
+    for (u64 t = tid; t < A.per_row; t += 256)
+        if ((u64)ids[t] < A.vocab) w += dl[t];
+    if (A.per_row > 1) {
+        for (u32 d = 32; d; d >>= 1) w += __shfl_xor(w, (int)d);
+        if ((tid & 63) == 0) ws[tid >> 6] = w;
+        __syncthreads();
+        w = ws[0] + ws[1] + ws[2] + ws[3];
+    } else if (A.per_row) {
+        w = (u64)ids[0] < A.vocab ? dl[0] : 0.0f;
     }
-    for (u64 j = threadIdx.x; j < vocab; j += 256) {
-        const float lp = -((float)((u64)m - (u64)in.at(base + j)) * unit + ls);
-        const float p = expf(lp);
-        float g = 0;
-        for (u64 t = 0; t < per_row; t++)
-            if (ids[row * per_row + t] == (i64)j) g += d_logp[row * per_row + t];
-        g -= p * w;
-        if (d_entropy) g -= h * p * (lp + H);
-        if (grad) grad[base + j] = g;
-        if (grad_words) grad_words[base + j] = nearest_word(g * words);
+    // - p w - h p (ln p + H)
+    auto part = [&](u64 x) {
+        const float lp = -(word_dist(m, (i64)x) * A.unit + ls), p = expf(lp);
+        return -p * (w + h * (lp + H));
+    };
+    for (u64 tile = j0; tile < j1; tile += 512 * GRAD_PAIRS) {
+        if (tile + 512 * GRAD_PAIRS <= j1) {
+            u64x2 x[GRAD_PAIRS];
+#pragma unroll
+            for (u32 k = 0; k < GRAD_PAIRS; k++) x[k] = in.at2(base + tile + 512 * k + 2 * tid);
+#pragma unroll
+            for (u32 k = 0; k < GRAD_PAIRS; k++) {
+                const u64 at = base + tile + 512 * k + 2 * tid;
+                const f32x2 g = {part(x[k].x), part(x[k].y)};
+                if (A.grad) {
+                    if (STREAM) __builtin_nontemporal_store(g, (f32x2u *)(A.grad + at));
+                    else *(f32x2u *)(A.grad + at) = g;
+                }
+                if (A.grad_words)
+                    st2<STREAM>((u64 *)A.grad_words + at, u64x2{(u64)nearest_word(g.x * A.words), (u64)nearest_word(g.y * A.words)});
+            }
+        } else {
+            for (u64 j = tile + tid; j < j1; j += 256) {
+                const float g = part((u64)in.at(base + j));
+                if (A.grad) A.grad[base + j] = g;
+                if (A.grad_words) A.grad_words[base + j] = nearest_word(g * A.words);
+            }
+        }
+    }
+    if (A.per_row == 0) return;
+    __syncthreads(); // the stores above are done: a word of an id is written by another lane now
+    for (u64 t = tid; t < A.per_row; t += 256) {
+        const u64 id = (u64)ids[t];
+        if (id < j0 || id >= j1) continue;
+        float g = 0; // equal ids write the same value
+        for (u64 k = 0; k < A.per_row; k++)
+            if ((u64)ids[k] == id) g += dl[k];
+        g += part((u64)in.at(base + id));
+        if (A.grad) A.grad[base + id] = g;
+        if (A.grad_words) A.grad_words[base + id] = nearest_word(g * A.words);
     }
 }
 
@@ -858,7 +959,7 @@ struct GradLayout {
 };
 template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *scratch) {
     if (A.n <= GRAD_SMALL_N && A.n * A.vocab <= GRAD_SMALL_SCAN) {
-        const u64 slices = ceil_div(A.dim, 128 * GRAD_STEPS);
+        const u64 slices = ceil_div(A.dim, 128);
         MPCX_REQUIRE(slices < 65536, "mpcx_ring_embed_grad: rows of %llu words", (unsigned long long)A.dim);
         hipLaunchKernelGGL(embed_grad_small_kernel<TWO>, dim3((u32)ceil_div(A.vocab, GRAD_ROWS), (u32)slices), dim3(256), 0,
                            ctx->stream, A);
@@ -869,18 +970,20 @@ template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *s
     u64 *w = (u64 *)scratch;
     const GradWork W{(u32 *)(w + L.cursor), (u32 *)(w + L.count), (u32 *)(w + L.start), (u32 *)(w + L.rank), (u32 *)(w + L.order),
                      (GradChunk *)(w + L.chunks), (GradHeavy *)(w + L.heavy), w + L.partial};
+    const u32 n = (u32)A.n, vb = (u32)ceil_div(A.vocab, 256);
     u32 lg = 3; // lanes of a row: up to a wavefront
-    while (lg < 6 && (2ull * GRAD_STEPS << lg) < A.dim) lg++;
-    const u64 slices = ceil_div(A.dim, 2ull * GRAD_STEPS << lg), heavy_blocks = 512;
+    while (lg < 6 && (2ull << lg) < A.dim) lg++;
+    const u64 slices = ceil_div(A.dim, 128), heavy_blocks = n > GRAD_CHUNK ? 512 : 0; // otherwise no row is heavy
     const u64 blocks = ceil_div(A.vocab * slices, 256u >> lg) + heavy_blocks;
     MPCX_REQUIRE(blocks < (1ull << 31), "mpcx_ring_embed_grad: table too large for one launch");
-    const u32 n = (u32)A.n, tb = (u32)ceil_div(A.n, 256), vb = (u32)ceil_div(A.vocab, 256);
     hipLaunchKernelGGL(grad_clear_kernel, dim3(vb), dim3(256), 0, ctx->stream, W.cursor, 4 + A.vocab);
-    if (n) hipLaunchKernelGGL(grad_count_kernel, dim3(tb), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
+    if (n) hipLaunchKernelGGL(grad_count_kernel, dim3((u32)ceil_div(n, GRAD_TOKENS)), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
     hipLaunchKernelGGL(grad_place_kernel, dim3(vb), dim3(256), 0, ctx->stream, (u32)A.vocab, W);
-    if (n) hipLaunchKernelGGL(grad_order_kernel, dim3(tb), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
-    hipLaunchKernelGGL(grad_rows_kernel<TWO>, dim3((u32)blocks), dim3(256), 0, ctx->stream, A, W, (u32)heavy_blocks, lg, (u32)slices);
-    if (n > GRAD_CHUNK) hipLaunchKernelGGL(grad_heavy_kernel<TWO>, dim3(512), dim3(256), 0, ctx->stream, A, W, lg, (u32)slices);
+    if (n) hipLaunchKernelGGL(grad_order_kernel, dim3((u32)ceil_div(n, 256)), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
+    const bool stream = A.vocab * A.dim * (TWO ? 16 : 8) > OUT_STREAM;
+    hipLaunchKernelGGL((stream ? grad_rows_kernel<TWO, true> : grad_rows_kernel<TWO, false>), dim3((u32)blocks), dim3(256), 0,
+                       ctx->stream, A, W, (u32)heavy_blocks, lg, (u32)slices);
+    if (heavy_blocks) hipLaunchKernelGGL(grad_heavy_kernel<TWO>, dim3(2048), dim3(256), 0, ctx->stream, A, W);
     MPCX_LAUNCH_CHECK();
     return 0;
 }
@@ -904,12 +1007,11 @@ int mpcx_ring_embed(mpcx_ctx *ctx, const int64_t *T0, const int64_t *T1, uint64_
     u64 blocks = ceil_div(n, 256u >> lg);
     if (blocks > MPCX_MAX_GRID) blocks = MPCX_MAX_GRID;
     const dim3 grid((u32)blocks, (u32)slices), block(256);
-    if (T1)
-        hipLaunchKernelGGL(embed_kernel<true>, grid, block, 0, ctx->stream, (const u64 *)T0, (const u64 *)T1, vocab, dim, ids, n,
-                           (u64)scale, shift, (u64 *)E0, (u64 *)E1, lg);
-    else
-        hipLaunchKernelGGL(embed_kernel<false>, grid, block, 0, ctx->stream, (const u64 *)T0, (const u64 *)nullptr, vocab, dim, ids,
-                           n, (u64)scale, shift, (u64 *)E0, (u64 *)nullptr, lg);
+    const bool stream = n * dim * (T1 ? 16 : 8) > OUT_STREAM;
+    const auto kernel = T1 ? (stream ? embed_kernel<true, true> : embed_kernel<true, false>)
+                           : (stream ? embed_kernel<false, true> : embed_kernel<false, false>);
+    hipLaunchKernelGGL(kernel, grid, block, 0, ctx->stream, (const u64 *)T0, (const u64 *)T1, vocab, dim, ids, n, (u64)scale, shift,
+                       (u64 *)E0, (u64 *)E1, lg);
     MPCX_LAUNCH_CHECK();
     return 0;
 }
@@ -1066,15 +1168,21 @@ int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b,
     MPCX_REQUIRE(a && row_max && log_sum && (grad || grad_words) && (per_row == 0 || (ids && d_logp)) && (!d_entropy || entropy),
                  "mpcx_reveal_logprobs_grad: NULL pointer");
     MPCX_REQUIRE(ctx, "mpcx_reveal_logprobs_grad: the context is NULL");
-    auto run = [&](auto in) -> int {
-        hipLaunchKernelGGL(logprobs_grad_kernel, dim3((u32)rows), dim3(256), 0, ctx->stream, in, vocab, ldexpf(1.0f, -frac), ids,
-                           per_row, d_logp, d_entropy, row_max, log_sum, entropy, grad, grad_words, ldexpf(1.0f, grad_frac));
+    LogprobGradArgs A{};
+    A.vocab = vocab, A.chunk = logprob_chunk(rows, vocab), A.splits = (u32)ceil_div(vocab, A.chunk);
+    A.unit = ldexpf(1.0f, -frac), A.words = ldexpf(1.0f, grad_words ? grad_frac : 0);
+    A.ids = ids, A.per_row = per_row, A.d_logp = d_logp, A.d_entropy = d_entropy;
+    A.row_max = row_max, A.log_sum = log_sum, A.entropy = entropy, A.grad = grad, A.grad_words = grad_words;
+    const bool stream = LM_GNT && rows * vocab * ((grad ? 4 : 0) + (grad_words ? 8 : 0)) > OUT_STREAM;
+    auto run = [&](auto kernel, auto in) -> int {
+        hipLaunchKernelGGL(kernel, dim3((u32)(rows * A.splits)), dim3(256), 0, ctx->stream, in, A);
         MPCX_LAUNCH_CHECK();
         return 0;
     };
-    return c ? run(LogitIn<3>{(const u64 *)a, (const u64 *)b, (const u64 *)c})
-         : b ? run(LogitIn<2>{(const u64 *)a, (const u64 *)b, nullptr})
-             : run(LogitIn<1>{(const u64 *)a, nullptr, nullptr});
+    const u64 *pa = (const u64 *)a, *pb = (const u64 *)b, *pc = (const u64 *)c;
+    if (c) return run(stream ? logprobs_grad_kernel<3, true> : logprobs_grad_kernel<3, false>, LogitIn<3>{pa, pb, pc});
+    if (b) return run(stream ? logprobs_grad_kernel<2, true> : logprobs_grad_kernel<2, false>, LogitIn<2>{pa, pb, nullptr});
+    return run(stream ? logprobs_grad_kernel<1, true> : logprobs_grad_kernel<1, false>, LogitIn<1>{pa, nullptr, nullptr});
 }
 
 } // extern "C"

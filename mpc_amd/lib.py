@@ -103,7 +103,7 @@ def _word(x, keep):
     if isinstance(x, DeviceArray):
         return x.ptr
     if isinstance(x, (list, tuple)):  # a host array: of device addresses (arrays, tensors) or of counts
-        arr = (ctypes.c_uint64 * max(len(x), 1))(*[_word(e, keep) for e in x])
+        arr = (ctypes.c_uint64 * max(len(x), 1))(*[e if type(e) is int else _word(e, keep) for e in x])
         keep.append(arr)
         return ctypes.addressof(arr)
     raise TypeError(f"cannot pass {t} to the C ABI")
