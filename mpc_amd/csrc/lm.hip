@@ -13,14 +13,15 @@ bool lm_fits(u64 a, u64 b) { return a == 0 || b <= (1ull << 60) / a; }
 typedef u64 u64x2 __attribute__((ext_vector_type(2)));
 typedef u64x2 u64x2u __attribute__((aligned(8)));
 __device__ inline u64x2 ld2(const u64 *p) { return *(const u64x2u *)p; }
-// STREAM: the hint that the words are not read again soon, for outputs larger than the last-level cache (OUT_STREAM)
+// STREAM: the hint that the words are not read again soon, for calls that move more than the last-level cache holds
+// (lookup of 16384 x 4096 words of two shares 301 -> 283 us, gradient of log probabilities of 2048 x 32768 387 -> 379)
 template <bool STREAM = false> __device__ inline void st2(u64 *p, u64x2 v) {
     if (STREAM)
         __builtin_nontemporal_store(v, (u64x2u *)p);
     else
         *(u64x2u *)p = v;
 }
-constexpr u64 OUT_STREAM = 256ull << 20; // bytes
+constexpr u64 STREAM_BYTES = 256ull << 20;
 
 // ---- lookup.  A row is copied by 2^lg lanes (8 .. 256) of a workgroup, 16 bytes of each share per lane and step; the
 // four steps of a lane are all requested before the first is used.
@@ -572,55 +573,90 @@ struct WaveTop {
             mask &= __ballot(top_better(x, idx, tv, ti));
         }
     }
-};
-// The first tile of a wavefront: N candidates per lane at once.  A distance D is found by bisection such that at least
-// `top` lanes hold something within D of the maximum; what lies within D (rarely more than a few above `top`) is
-// gathered in LDS and sorted by counting, for each, how many are better.  Where more than 64 lie within D (many equal
-// words), or lanes are few, the candidates are inserted one by one.
-template <u32 N>
-__device__ inline void top_first(WaveTop &t, u32 top, const i64 (&x)[N], const u32 (&idx)[N], const bool (&valid)[N], i64 lane_max,
-                                 bool lane_any, TopEntry *buf) {
-    const u32 lane = threadIdx.x & 63;
-    const i64 m = wave_max(lane_any ? lane_max : INT64_MIN);
-    const float near = lane_any ? word_dist(m, lane_max) : INFINITY;
-    float lo = 0, hi = near;
-    if ((u32)__popcll(__ballot(lane_any)) < top) {
-        hi = INFINITY;
-    } else {
-        if (!lane_any) hi = 0;
-        for (u32 d = 32; d; d >>= 1) hi = fmaxf(hi, __shfl_xor(hi, (int)d));
-        for (u32 r = 0; r < 12; r++) {
-            const float mid = 0.5f * (lo + hi);
-            if ((u32)__popcll(__ballot(near <= mid)) >= top)
-                hi = mid;
-            else
-                lo = mid;
+    // N candidates per lane: every lane's best one that is left, until none beats the border
+    template <u32 N> __device__ void insert_all(u32 top, const i64 (&x)[N], const u32 (&idx)[N], const bool (&valid)[N]) {
+        u32 left = 0;
+#pragma unroll
+        for (u32 k = 0; k < N; k++) left |= (u32)valid[k] << k;
+        for (;;) {
+            i64 bv = INT64_MIN;
+            u32 bi = TOP_NONE, bk = 0;
+#pragma unroll
+            for (u32 k = 0; k < N; k++)
+                if ((left >> k & 1) && top_better(x[k], idx[k], bv, bi)) bv = x[k], bi = idx[k], bk = k;
+            if (!__ballot(top_better(bv, bi, tv, ti))) return;
+            left &= ~(1u << bk);
+            insert(top, bi != TOP_NONE, bv, bi);
         }
     }
+};
+// A distance such that at least `top` of the K values of 64 lanes lie within it, and hardly more than TOP_SLACK others
+// (values below 0 are not there; infinity when there are not enough): a bisection that counts with ballots.  `guess` is
+// tried first -- sixteen in the exponent, so that rows whose masked words lie far away do not take the range.
+constexpr u32 TOP_SLACK = 8;
+template <u32 K> __device__ inline float top_border(const float (&near)[K], u32 top, float guess) {
+    auto within = [&](float d) {
+        u32 n = 0;
+#pragma unroll
+        for (u32 k = 0; k < K; k++) n += (u32)__popcll(__ballot(near[k] >= 0 && near[k] <= d));
+        return n;
+    };
+    float lo = 0, hi = guess;
+    if (within(guess) < top) {
+        if (within(INFINITY) < top) return INFINITY;
+        lo = guess, hi = 0;
+#pragma unroll
+        for (u32 k = 0; k < K; k++) hi = fmaxf(hi, near[k]);
+        for (u32 d = 32; d; d >>= 1) hi = fmaxf(hi, __shfl_xor(hi, (int)d));
+    }
+    for (u32 r = 0; r < 16; r++) {
+        const float mid = 0.5f * (lo + hi);
+        const u32 n = within(mid);
+        if (n >= top) hi = mid;
+        else lo = mid;
+        if (n >= top && n <= top + TOP_SLACK) break;
+    }
+    return hi;
+}
+// The first tile of a wavefront: N candidates per lane at once.  With the border distance of the lanes' N / 2 pair maxima
+// (`all`: there are no more than 64 candidates, and none), what lies within it (rarely more than a few above `top`) is gathered in `buf`.  Returns its number, or 0 where more
+// than 64 lie within it (many equal words): then the candidates have been inserted one by one.
+template <u32 N>
+__device__ inline u32 top_first(WaveTop &t, u32 top, const i64 (&x)[N], const u32 (&idx)[N], const bool (&valid)[N], i64 lane_max,
+                                float guess, bool all, TopEntry *buf) {
+    const u32 lane = threadIdx.x & 63;
+    const i64 m = wave_max(lane_max);
+    float near[N / 2];
+#pragma unroll
+    for (u32 k = 0; k < N / 2; k++) near[k] = valid[2 * k] ? word_dist(m, valid[2 * k + 1] && x[2 * k + 1] > x[2 * k] ? x[2 * k + 1] : x[2 * k]) : -1.0f;
+    const float border = all ? INFINITY : top_border<N / 2>(near, top, guess);
     u32 count = 0;
     u32 slot[N];
 #pragma unroll
     for (u32 k = 0; k < N; k++) {
-        const u64 b = __ballot(valid[k] && word_dist(m, x[k]) <= hi);
+        const u64 b = __ballot(valid[k] && word_dist(m, x[k]) <= border);
         slot[k] = ((b >> lane) & 1) ? count + (u32)__popcll(b & ((1ull << lane) - 1)) : TOP_NONE;
         count += (u32)__popcll(b);
     }
     if (count > 64) {
-#pragma unroll
-        for (u32 k = 0; k < N; k++) t.insert(top, valid[k], x[k], idx[k]);
-        return;
+        t.insert_all(top, x, idx, valid);
+        return 0;
     }
 #pragma unroll
     for (u32 k = 0; k < N; k++)
         if (slot[k] != TOP_NONE) buf[slot[k]] = TopEntry{x[k], idx[k], 0};
     prg_wave_sync();
-    const i64 v = lane < count ? buf[lane].v : INT64_MIN;
-    const u32 i = lane < count ? buf[lane].i : TOP_NONE;
+    return count;
+}
+// the `count` entries of buf, sorted by counting the better ones of each, become the wavefront's list
+__device__ inline void top_sort(WaveTop &t, u32 top, u32 count, TopEntry *buf) {
+    const u32 lane = threadIdx.x & 63;
+    const TopEntry e = lane < count ? buf[lane] : TopEntry{INT64_MIN, TOP_NONE, 0};
     u32 rank = 0;
 #pragma unroll 8
-    for (u32 k = 0; k < count; k++) rank += top_better(buf[k].v, buf[k].i, v, i);
+    for (u32 k = 0; k < count; k++) rank += top_better(buf[k].v, buf[k].i, e.v, e.i);
     prg_wave_sync();
-    if (lane < count) buf[rank] = TopEntry{v, i, 0};
+    if (lane < count) buf[rank] = e;
     prg_wave_sync();
     if (lane < count && lane < top) t.v = buf[lane].v, t.i = buf[lane].i;
     prg_wave_sync();
@@ -650,15 +686,23 @@ struct RowSums {
         const float d = word_dist(to, m) * unit2, f = exp2_fast(-d);
         T = (T + d * S) * f, S *= f, m = to;
     }
+    template <class P> __device__ void join(const P &part, float unit2) {
+        RowSums o;
+        o.m = part.m, o.S = part.S, o.T = part.T;
+        if (o.m > m) move_to(o.m, unit2);
+        else o.move_to(m, unit2);
+        S += o.S, T += o.T;
+    }
     __device__ void wave_join(float unit2) {
         move_to(wave_max(m), unit2);
         for (u32 d = 32; d; d >>= 1) S += __shfl_xor(S, (int)d), T += __shfl_xor(T, (int)d);
     }
 };
-struct RowPart {
+struct RowPart { // of one wavefront; S = 0: it has read no words
     i64 m;
     float S, T;
 };
+constexpr u32 LIST = 32; // entries of a part's list, in any order; those that are not there have the index TOP_NONE
 
 struct LogprobArgs {
     u64 rows, vocab;
@@ -673,12 +717,14 @@ struct LogprobArgs {
     float *top_logp;
     i64 *row_max;
     float *log_sum;
-    RowPart *parts;  // splits > 1: rows x splits, then
-    TopEntry *lists; // rows x splits x top
+    RowPart *parts;  // splits > 1: rows x splits x 4 wavefronts, then
+    TopEntry *lists; // LIST entries for each
 };
-// a row's outputs, by `n` threads (thread `t` of them); list: the row's sorted entries
+// a row's outputs, by `n` threads (thread `t` of them); list: the row's sorted entries; at_first: the word of the thread's
+// first id, where that has been read (first_id inside the vocabulary)
 template <int SH>
-__device__ inline void logprobs_finish(const LogitIn<SH> &in, const LogprobArgs &A, u64 row, RowSums s, const TopEntry *list, u32 t, u32 n) {
+__device__ inline void logprobs_finish(const LogitIn<SH> &in, const LogprobArgs &A, u64 row, RowSums s, const TopEntry *list, u32 t, u32 n,
+                                       u64 first_id = ~0ull, i64 at_first = 0) {
     const float ls = logf(s.S);
     if (t == 0) {
         if (A.entropy) A.entropy[row] = ls + s.T / s.S * 0.69314718f;
@@ -687,7 +733,8 @@ __device__ inline void logprobs_finish(const LogitIn<SH> &in, const LogprobArgs 
     }
     for (u64 k = t; k < A.per_row; k += n) {
         const u64 id = (u64)A.ids[row * A.per_row + k];
-        A.logp[row * A.per_row + k] = id < A.vocab ? -(word_dist(s.m, in.at(row * A.vocab + id)) * A.unit + ls) : 0.0f;
+        const i64 x = id >= A.vocab ? 0 : k == t && first_id == id ? at_first : in.at(row * A.vocab + id);
+        A.logp[row * A.per_row + k] = id < A.vocab ? -(word_dist(s.m, x) * A.unit + ls) : 0.0f;
     }
     if (t < A.top) {
         A.top_ids[row * A.top + t] = (i64)list[t].i;
@@ -697,19 +744,21 @@ __device__ inline void logprobs_finish(const LogitIn<SH> &in, const LogprobArgs 
 
 // W wavefronts of a workgroup of four read `chunk` words of a row, in tiles of 64 x 8 words each.  A lane keeps its own
 // maximum and sums and moves them when a tile raises its maximum; nothing is exchanged between lanes before the end but
-// the ballots that look for new entries of the top list.
-template <u32 W, int SH> __global__ __launch_bounds__(256) void logprobs_kernel(LogitIn<SH> in, LogprobArgs A) {
+// the ballots that look for new entries of the top list.  SPLIT: several workgroups read a row, and every wavefront
+// leaves its own part for logprobs_join_kernel.
+template <u32 W, bool SPLIT, int SH> __global__ __launch_bounds__(256) void logprobs_kernel(LogitIn<SH> in, LogprobArgs A) {
     constexpr u32 U = 4, N = 2 * U, TILE = 64 * N;
     __shared__ TopEntry buf[4][64];
     __shared__ TopEntry merged[32];
     __shared__ RowPart ws[4];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const u64 group = W == 1 ? (u64)blockIdx.x * 4 + wave : blockIdx.x;
-    const u64 row = group / A.splits, split = group % A.splits;
+    const u64 row = SPLIT ? group / A.splits : group, split = SPLIT ? group % A.splits : 0;
     if (W == 1 && row >= A.rows) return; // a wavefront of its own: no barrier follows
     const u64 base = row * A.vocab, j0 = split * A.chunk, j1 = j0 + A.chunk < A.vocab ? j0 + A.chunk : A.vocab;
     RowSums s;
     WaveTop top;
+    u32 count = 0; // entries in buf that are not in `top` yet
     bool first = true;
     for (u64 tile = j0 + (W == 1 ? 0 : wave) * TILE; tile < j1; tile += W * TILE) {
         i64 x[N];
@@ -730,11 +779,9 @@ template <u32 W, int SH> __global__ __launch_bounds__(256) void logprobs_kernel(
             }
         }
         i64 m = x[0];
-        bool any = valid[0];
 #pragma unroll
         for (u32 k = 0; k < N; k++) {
             m = x[k] > m ? x[k] : m;
-            any |= valid[k];
             idx[k] = (u32)(tile + 128 * (k / 2) + 2 * lane + (k & 1));
         }
         if (m > s.m) s.move_to(m, A.unit2);
@@ -745,15 +792,27 @@ template <u32 W, int SH> __global__ __launch_bounds__(256) void logprobs_kernel(
         }
         if (A.top) {
             if (first) {
-                top_first<N>(top, A.top, x, idx, valid, m, any, buf[wave]);
+                count = top_first<N>(top, A.top, x, idx, valid, m, 16.0f / A.unit, j1 - tile <= 64, buf[wave]);
                 first = false;
-            } else if (__ballot(m >= top.tv)) {
-#pragma unroll
-                for (u32 k = 0; k < N; k++) top.insert(A.top, valid[k], x[k], idx[k]);
+            } else {
+                if (count) top_sort(top, A.top, count, buf[wave]), count = 0;
+                if (__ballot(m >= top.tv)) top.insert_all(A.top, x, idx, valid);
             }
         }
     }
     s.wave_join(A.unit2);
+    if (SPLIT) {
+        const u64 part = group * 4 + wave;
+        if (lane == 0) A.parts[part] = RowPart{s.m, s.S, s.T};
+        if (A.top) {
+            if (count > LIST) top_sort(top, A.top, count, buf[wave]), count = 0;
+            TopEntry e{lane < A.top ? top.v : INT64_MIN, lane < A.top ? top.i : TOP_NONE, 0};
+            if (count) e = lane < count ? buf[wave][lane] : TopEntry{INT64_MIN, TOP_NONE, 0};
+            if (lane < LIST) A.lists[part * LIST + lane] = e;
+        }
+        return;
+    }
+    if (count) top_sort(top, A.top, count, buf[wave]);
     if (W == 1) {
         if (lane < A.top) buf[wave][lane] = TopEntry{top.v, top.i, 0};
         prg_wave_sync();
@@ -764,86 +823,97 @@ template <u32 W, int SH> __global__ __launch_bounds__(256) void logprobs_kernel(
     __syncthreads(); // every wavefront has left its own part of buf
     TopEntry *lists = &buf[0][0];
     if (lane < A.top) lists[wave * A.top + lane] = TopEntry{top.v, top.i, 0};
-    for (u32 w = 0; w < 4; w++) {
-        RowSums o;
-        o.m = ws[w].m, o.S = ws[w].S, o.T = ws[w].T;
-        if (w == 0) {
-            s = o;
-            continue;
-        }
-        if (o.m > s.m) s.move_to(o.m, A.unit2);
-        else o.move_to(s.m, A.unit2);
-        s.S += o.S, s.T += o.T;
-    }
+    s = RowSums();
+    for (u32 w = 0; w < 4; w++) s.join(ws[w], A.unit2);
     __syncthreads();
     if (A.top) top_merge<4>(lists, merged, A.top);
-    if (A.splits == 1) {
-        logprobs_finish(in, A, row, s, merged, tid, 256);
-    } else {
-        if (tid == 0) A.parts[group] = RowPart{s.m, s.S, s.T};
-        if (tid < A.top) A.lists[group * A.top + tid] = merged[tid];
-    }
+    logprobs_finish(in, A, row, s, merged, tid, 256);
 }
-// joins the parts of a row: one workgroup per row
-template <int SH> __global__ __launch_bounds__(256) void logprobs_join_kernel(LogitIn<SH> in, LogprobArgs A) {
-    constexpr u32 N = 8;
-    __shared__ TopEntry buf[4][64];
-    __shared__ TopEntry merged[32];
-    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// Joins the parts of a row: one workgroup per row.  What counts is the time of one such call, so parts and lists are asked
+// for together and every wavefront forms the maximum and the border (from the lanes' maxima over four interleaved sets of
+// parts each) for itself; its entries within the border go to LDS, and after the one barrier the first wavefront sorts
+// them.
+template <int SH> __global__ __launch_bounds__(1024) void logprobs_join_kernel(LogitIn<SH> in, LogprobArgs A) {
+    constexpr u32 K = 4, E = 8;
+    __shared__ TopEntry buf[64];
+    __shared__ u32 count;
+    const u32 tid = threadIdx.x, lane = tid & 63;
     const u64 row = blockIdx.x;
-    const RowPart *parts = A.parts + row * A.splits;
-    RowSums s;
-    for (u32 k = lane; k < A.splits; k += 64) { // every wavefront for itself
-        RowSums o;
-        o.m = parts[k].m, o.S = parts[k].S, o.T = parts[k].T;
-        if (o.m > s.m) s.move_to(o.m, A.unit2);
-        else o.move_to(s.m, A.unit2);
-        s.S += o.S, s.T += o.T;
+    const u32 n = A.splits * 4, slots = A.top ? n * LIST : 0;
+    const RowPart *parts = A.parts + row * n;
+    const TopEntry *lists = A.lists + row * n * LIST;
+    const u64 id = tid < A.per_row ? (u64)A.ids[row * A.per_row + tid] : A.vocab; // asked for early, used at the end
+    TopEntry e[E];
+#pragma unroll
+    for (u32 k = 0; k < E; k++) {
+        const u32 j = k * blockDim.x + tid;
+        e[k] = j < slots ? lists[j] : TopEntry{INT64_MIN, TOP_NONE, 0};
     }
+    RowSums s;
+    i64 best[K];
+#pragma unroll
+    for (u32 k = 0; k < K; k++) best[k] = INT64_MIN;
+    u32 any = 0;
+    for (u32 p0 = 0; p0 < n; p0 += 64 * K) {
+        RowPart o[K];
+#pragma unroll
+        for (u32 k = 0; k < K; k++) {
+            const u32 p = p0 + 64 * k + lane;
+            o[k] = p < n ? parts[p] : RowPart{INT64_MIN, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (u32 k = 0; k < K; k++) {
+            s.join(o[k], A.unit2);
+            if (o[k].S > 0.0f) any |= 1u << k, best[k] = o[k].m > best[k] ? o[k].m : best[k];
+        }
+    }
+    if (tid == 0) count = 0;
+    const i64 at_id = id < A.vocab ? in.at(row * A.vocab + id) : 0;
     s.wave_join(A.unit2);
+    float border = 0;
     if (A.top) {
-        const TopEntry *lists = A.lists + row * A.splits * A.top;
-        const u32 n = A.splits * A.top;
-        WaveTop top;
-        bool first = true;
-        for (u32 tile = wave * 64 * N; tile < n; tile += 4 * 64 * N) {
-            i64 x[N], m = INT64_MIN;
-            u32 idx[N];
-            bool valid[N], any = false;
+        float near[K];
 #pragma unroll
-            for (u32 k = 0; k < N; k++) {
-                const u32 j = tile + 64 * k + lane;
-                const TopEntry e = j < n ? lists[j] : TopEntry{INT64_MIN, TOP_NONE, 0};
-                x[k] = e.v, idx[k] = e.i, valid[k] = e.i != TOP_NONE, any |= valid[k];
-                m = e.v > m ? e.v : m;
-            }
-            if (first) {
-                top_first<N>(top, A.top, x, idx, valid, m, any, buf[wave]);
-                first = false;
-            } else if (__ballot(any && m >= top.tv)) {
+        for (u32 k = 0; k < K; k++) near[k] = (any >> k & 1) ? word_dist(s.m, best[k]) : -1.0f;
+        border = top_border<K>(near, A.top, 16.0f / A.unit);
+    }
+    __syncthreads();
+    for (u32 j0 = 0; j0 < slots; j0 += E * blockDim.x) {
+        if (j0) {
 #pragma unroll
-                for (u32 k = 0; k < N; k++) top.insert(A.top, valid[k], x[k], idx[k]);
+            for (u32 k = 0; k < E; k++) {
+                const u32 j = j0 + k * blockDim.x + tid;
+                e[k] = j < slots ? lists[j] : TopEntry{INT64_MIN, TOP_NONE, 0};
             }
         }
-        __syncthreads();
-        TopEntry *all = &buf[0][0];
-        if (lane < A.top) all[wave * A.top + lane] = TopEntry{top.v, top.i, 0};
-        __syncthreads();
-        top_merge<4>(all, merged, A.top);
+#pragma unroll
+        for (u32 k = 0; k < E; k++)
+            if (e[k].i != TOP_NONE && word_dist(s.m, e[k].v) <= border) {
+                const u32 at = atomicAdd(&count, 1u);
+                if (at < 64) buf[at] = e[k];
+            }
     }
-    logprobs_finish(in, A, row, s, merged, tid, 256);
+    __syncthreads();
+    if (tid < 64 && A.top) {
+        WaveTop top;
+        if (count <= 64) {
+            top_sort(top, A.top, count, buf);
+        } else { // many equal words: all lists, one entry after the other
+            for (u32 j = lane; j - lane < slots; j += 64) {
+                const TopEntry q = j < slots ? lists[j] : TopEntry{INT64_MIN, TOP_NONE, 0};
+                top.insert(A.top, q.i != TOP_NONE, q.v, q.i);
+            }
+        }
+        if (lane < A.top) buf[lane] = TopEntry{top.v, top.i, 0};
+        prg_wave_sync();
+    }
+    logprobs_finish(in, A, row, s, buf, tid, blockDim.x, id, at_id);
 }
 
 // The gradient.  A workgroup takes `chunk` words of a row, 16 bytes of each share per load and GRAD_PAIRS of them together;
 // the words of the given ids are written again at the end with their own terms added, so that the pass itself knows no
 // ids and every word is rounded once.
-#ifndef LM_GP
-#define LM_GP 4
-#endif
-#ifndef LM_GNT
-#define LM_GNT 1
-#endif
-constexpr u32 GRAD_PAIRS = LM_GP;
+constexpr u32 GRAD_PAIRS = 8;
 struct LogprobGradArgs {
     u64 vocab, chunk;
     u32 splits;
@@ -883,29 +953,30 @@ template <int SH, bool STREAM> __global__ __launch_bounds__(256) void logprobs_g
         const float lp = -(word_dist(m, (i64)x) * A.unit + ls), p = expf(lp);
         return -p * (w + h * (lp + H));
     };
-    for (u64 tile = j0; tile < j1; tile += 512 * GRAD_PAIRS) {
-        if (tile + 512 * GRAD_PAIRS <= j1) {
-            u64x2 x[GRAD_PAIRS];
-#pragma unroll
-            for (u32 k = 0; k < GRAD_PAIRS; k++) x[k] = in.at2(base + tile + 512 * k + 2 * tid);
-#pragma unroll
-            for (u32 k = 0; k < GRAD_PAIRS; k++) {
-                const u64 at = base + tile + 512 * k + 2 * tid;
-                const f32x2 g = {part(x[k].x), part(x[k].y)};
-                if (A.grad) {
-                    if (STREAM) __builtin_nontemporal_store(g, (f32x2u *)(A.grad + at));
-                    else *(f32x2u *)(A.grad + at) = g;
-                }
-                if (A.grad_words)
-                    st2<STREAM>((u64 *)A.grad_words + at, u64x2{(u64)nearest_word(g.x * A.words), (u64)nearest_word(g.y * A.words)});
-            }
-        } else {
-            for (u64 j = tile + tid; j < j1; j += 256) {
-                const float g = part((u64)in.at(base + j));
-                if (A.grad) A.grad[base + j] = g;
-                if (A.grad_words) A.grad_words[base + j] = nearest_word(g * A.words);
-            }
+    auto put1 = [&](u64 at, float g) {
+        if (A.grad) A.grad[at] = g;
+        if (A.grad_words) A.grad_words[at] = nearest_word(g * A.words);
+    };
+    auto put2 = [&](u64 at, u64x2 x) {
+        const f32x2 g = {part(x.x), part(x.y)};
+        if (A.grad) {
+            if (STREAM) __builtin_nontemporal_store(g, (f32x2u *)(A.grad + at));
+            else *(f32x2u *)(A.grad + at) = g;
         }
+        if (A.grad_words) st2<STREAM>((u64 *)A.grad_words + at, u64x2{(u64)nearest_word(g.x * A.words), (u64)nearest_word(g.y * A.words)});
+    };
+    u64 tile = j0;
+    for (; tile + 512 * GRAD_PAIRS <= j1; tile += 512 * GRAD_PAIRS) {
+        const u64 at = base + tile + 2 * tid;
+        u64x2 x[GRAD_PAIRS];
+#pragma unroll
+        for (u32 k = 0; k < GRAD_PAIRS; k++) x[k] = in.at2(at + 512 * k);
+#pragma unroll
+        for (u32 k = 0; k < GRAD_PAIRS; k++) put2(at + 512 * k, x[k]);
+    }
+    for (u64 j = tile + 2 * tid; j < j1; j += 512) {
+        if (j + 1 < j1) put2(base + j, in.at2(base + j));
+        else put1(base + j, part((u64)in.at(base + j)));
     }
     if (A.per_row == 0) return;
     __syncthreads(); // the stores above are done: a word of an id is written by another lane now
@@ -916,8 +987,7 @@ template <int SH, bool STREAM> __global__ __launch_bounds__(256) void logprobs_g
         for (u64 k = 0; k < A.per_row; k++)
             if ((u64)ids[k] == id) g += dl[k];
         g += part((u64)in.at(base + id));
-        if (A.grad) A.grad[base + id] = g;
-        if (A.grad_words) A.grad_words[base + id] = nearest_word(g * A.words);
+        put1(base + id, g);
     }
 }
 
@@ -925,13 +995,16 @@ constexpr u64 LP_GROUPS = 1024; // workgroups that fill the chip: four on each C
 constexpr u64 LP_CHUNK = 2048;  // words: one tile for each of four wavefronts
 constexpr u64 LP_WAVE_ROW = 1024; // rows up to this length are read by one wavefront each
 template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, const LogprobArgs &A) {
-    if (A.splits == 1 && A.vocab <= LP_WAVE_ROW)
-        hipLaunchKernelGGL((logprobs_kernel<1, SH>), dim3((u32)ceil_div(A.rows, 4)), dim3(256), 0, ctx->stream, in, A);
+    if (A.splits > 1)
+        hipLaunchKernelGGL((logprobs_kernel<4, true, SH>), dim3((u32)(A.rows * A.splits)), dim3(256), 0, ctx->stream, in, A);
+    else if (A.vocab <= LP_WAVE_ROW)
+        hipLaunchKernelGGL((logprobs_kernel<1, false, SH>), dim3((u32)ceil_div(A.rows, 4)), dim3(256), 0, ctx->stream, in, A);
     else
-        hipLaunchKernelGGL((logprobs_kernel<4, SH>), dim3((u32)(A.rows * A.splits)), dim3(256), 0, ctx->stream, in, A);
+        hipLaunchKernelGGL((logprobs_kernel<4, false, SH>), dim3((u32)A.rows), dim3(256), 0, ctx->stream, in, A);
     MPCX_LAUNCH_CHECK();
     if (A.splits > 1) {
-        hipLaunchKernelGGL(logprobs_join_kernel<SH>, dim3((u32)A.rows), dim3(256), 0, ctx->stream, in, A);
+        const u64 threads = A.top ? ceil_div((u64)A.splits * 4 * LIST / 8, 64) * 64 : 64; // eight entries each
+        hipLaunchKernelGGL(logprobs_join_kernel<SH>, dim3((u32)A.rows), dim3((u32)(threads < 1024 ? threads : 1024)), 0, ctx->stream, in, A);
         MPCX_LAUNCH_CHECK();
     }
     return 0;
@@ -980,7 +1053,7 @@ template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *s
     if (n) hipLaunchKernelGGL(grad_count_kernel, dim3((u32)ceil_div(n, GRAD_TOKENS)), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
     hipLaunchKernelGGL(grad_place_kernel, dim3(vb), dim3(256), 0, ctx->stream, (u32)A.vocab, W);
     if (n) hipLaunchKernelGGL(grad_order_kernel, dim3((u32)ceil_div(n, 256)), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
-    const bool stream = A.vocab * A.dim * (TWO ? 16 : 8) > OUT_STREAM;
+    const bool stream = (A.n + A.vocab) * A.dim * (TWO ? 16 : 8) > STREAM_BYTES;
     hipLaunchKernelGGL((stream ? grad_rows_kernel<TWO, true> : grad_rows_kernel<TWO, false>), dim3((u32)blocks), dim3(256), 0,
                        ctx->stream, A, W, (u32)heavy_blocks, lg, (u32)slices);
     if (heavy_blocks) hipLaunchKernelGGL(grad_heavy_kernel<TWO>, dim3(2048), dim3(256), 0, ctx->stream, A, W);
@@ -1007,7 +1080,7 @@ int mpcx_ring_embed(mpcx_ctx *ctx, const int64_t *T0, const int64_t *T1, uint64_
     u64 blocks = ceil_div(n, 256u >> lg);
     if (blocks > MPCX_MAX_GRID) blocks = MPCX_MAX_GRID;
     const dim3 grid((u32)blocks, (u32)slices), block(256);
-    const bool stream = n * dim * (T1 ? 16 : 8) > OUT_STREAM;
+    const bool stream = n * dim * (T1 ? 32 : 16) > STREAM_BYTES;
     const auto kernel = T1 ? (stream ? embed_kernel<true, true> : embed_kernel<true, false>)
                            : (stream ? embed_kernel<false, true> : embed_kernel<false, false>);
     hipLaunchKernelGGL(kernel, grid, block, 0, ctx->stream, (const u64 *)T0, (const u64 *)T1, vocab, dim, ids, n, (u64)scale, shift,
@@ -1130,7 +1203,7 @@ static u64 logprob_chunk(u64 rows, u64 vocab) {
 }
 uint64_t mpcx_reveal_logprobs_scratch(uint64_t rows, uint64_t vocab, uint64_t top) {
     const u64 splits = vocab ? ceil_div(vocab, logprob_chunk(rows, vocab)) : 1;
-    return splits > 1 ? rows * splits * (sizeof(RowPart) + top * sizeof(TopEntry)) : 16;
+    return splits > 1 ? rows * splits * 4 * (sizeof(RowPart) + (top ? LIST * sizeof(TopEntry) : 0)) : 16;
 }
 int mpcx_reveal_logprobs(mpcx_ctx *ctx, const int64_t *a, const int64_t *b, const int64_t *c, uint64_t rows, uint64_t vocab,
                          int frac, const int64_t *ids, uint64_t per_row, uint64_t top, void *scratch, float *logp,
@@ -1149,7 +1222,7 @@ int mpcx_reveal_logprobs(mpcx_ctx *ctx, const int64_t *a, const int64_t *b, cons
     A.unit = ldexpf(1.0f, -frac), A.unit2 = ldexpf(1.44269504f, -frac);
     A.ids = ids, A.per_row = per_row, A.logp = logp, A.entropy = entropy, A.top_ids = top_ids, A.top_logp = top_logp;
     A.row_max = row_max, A.log_sum = log_sum;
-    A.parts = (RowPart *)scratch, A.lists = (TopEntry *)(A.parts + rows * A.splits);
+    A.parts = (RowPart *)scratch, A.lists = (TopEntry *)(A.parts + rows * A.splits * 4);
     return c ? logprobs_run<3>(ctx, {(const u64 *)a, (const u64 *)b, (const u64 *)c}, A)
          : b ? logprobs_run<2>(ctx, {(const u64 *)a, (const u64 *)b, nullptr}, A)
              : logprobs_run<1>(ctx, {(const u64 *)a, nullptr, nullptr}, A);
@@ -1173,7 +1246,7 @@ int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b,
     A.unit = ldexpf(1.0f, -frac), A.words = ldexpf(1.0f, grad_words ? grad_frac : 0);
     A.ids = ids, A.per_row = per_row, A.d_logp = d_logp, A.d_entropy = d_entropy;
     A.row_max = row_max, A.log_sum = log_sum, A.entropy = entropy, A.grad = grad, A.grad_words = grad_words;
-    const bool stream = LM_GNT && rows * vocab * ((grad ? 4 : 0) + (grad_words ? 8 : 0)) > OUT_STREAM;
+    const bool stream = rows * vocab * ((c ? 24 : b ? 16 : 8) + (grad ? 4 : 0) + (grad_words ? 8 : 0)) > STREAM_BYTES;
     auto run = [&](auto kernel, auto in) -> int {
         hipLaunchKernelGGL(kernel, dim3((u32)(rows * A.splits)), dim3(256), 0, ctx->stream, in, A);
         MPCX_LAUNCH_CHECK();
