@@ -540,53 +540,69 @@ __device__ inline i64 wave_max(i64 v) {
     return v;
 }
 
-// The likeliest `top` <= 32 entries a wavefront has seen, best first: entry l in lane l, in the order value descending,
-// index ascending (all entries differ).  (tv, ti) is the last of them, the border that a new one has to beat.
+// The likeliest `top` <= 32 entries that a wavefront has seen, in the order value descending, index ascending (all entries
+// differ): up to 64 candidates in LDS in any order, and a border (tv, ti) that a new one has to beat.  When the 64 places
+// are full the candidates are sorted -- every one counts the better ones, from LDS -- and the first `top` stay; a sort
+// costs what a handful of one-by-one insertions would, and most tiles bring no candidate at all.
 struct TopEntry {
     i64 v;
     u32 i, pad;
 };
-__device__ inline bool top_better(i64 av, u32 ai, i64 bv, u32 bi) { return av > bv || (av == bv && ai < bi); }
 constexpr u32 TOP_NONE = ~0u; // the index of an entry that is not there (with the lowest value: behind all others)
+__device__ inline bool top_better(i64 av, u32 ai, i64 bv, u32 bi) { return av > bv || (av == bv && ai < bi); }
 struct WaveTop {
-    i64 v = INT64_MIN, tv = INT64_MIN;
-    u32 i = TOP_NONE, ti = TOP_NONE;
-    __device__ void border(u32 top) {
-        tv = lane_word(v, top - 1);
-        ti = (u32)__builtin_amdgcn_readlane((int)i, (int)top - 1);
-    }
-    // one candidate per lane; those that beat the border go in one after the other
-    __device__ void insert(u32 top, bool valid, i64 x, u32 idx) {
+    TopEntry *buf; // 64 entries
+    u32 top, count = 0;
+    i64 tv = INT64_MIN;
+    u32 ti = TOP_NONE;
+    __device__ WaveTop(TopEntry *b, u32 t) : buf(b), top(t) {}
+    __device__ void sort() {
         const u32 lane = threadIdx.x & 63;
-        u64 mask = __ballot(valid && top_better(x, idx, tv, ti));
-        while (mask) {
-            const u32 src = (u32)__builtin_ctzll(mask);
-            const i64 cv = lane_word(x, src);
-            const u32 ci = (u32)__builtin_amdgcn_readlane((int)idx, (int)src);
-            const u32 pos = (u32)__popcll(__ballot(top_better(v, i, cv, ci)));
-            const i64 uv = (i64)__shfl_up((long long)v, 1);
-            const u32 ui = (u32)__shfl_up((int)i, 1);
-            if (lane > pos) v = uv, i = ui;
-            if (lane == pos) v = cv, i = ci;
-            border(top);
-            mask &= mask - 1;
-            mask &= __ballot(top_better(x, idx, tv, ti));
-        }
+        const TopEntry e = lane < count ? buf[lane] : TopEntry{INT64_MIN, TOP_NONE, 0};
+        u32 rank = 0;
+#pragma unroll 8
+        for (u32 k = 0; k < count; k++) rank += top_better(buf[k].v, buf[k].i, e.v, e.i);
+        prg_wave_sync();
+        if (lane < count) buf[rank] = e;
+        prg_wave_sync();
+        if (count < top) return;
+        count = top;
+        tv = lane_word(buf[top - 1].v, 0), ti = (u32)__builtin_amdgcn_readfirstlane((int)buf[top - 1].i);
     }
-    // N candidates per lane: every lane's best one that is left, until none beats the border
-    template <u32 N> __device__ void insert_all(u32 top, const i64 (&x)[N], const u32 (&idx)[N], const bool (&valid)[N]) {
-        u32 left = 0;
+    // at most one candidate per lane, and room for them
+    __device__ void append(bool in, i64 x, u32 idx) {
+        const u64 b = __ballot(in);
+        if (in) buf[count + (u32)__popcll(b & ((1ull << (threadIdx.x & 63)) - 1))] = TopEntry{x, idx, 0};
+        count += (u32)__popcll(b);
+        prg_wave_sync();
+    }
+    // N candidates per lane
+    template <u32 N> __device__ void add(const i64 (&x)[N], const u32 (&idx)[N], const bool (&valid)[N]) {
+        const u32 lane = threadIdx.x & 63;
+        u32 left = 0, n = 0;
 #pragma unroll
-        for (u32 k = 0; k < N; k++) left |= (u32)valid[k] << k;
-        for (;;) {
-            i64 bv = INT64_MIN;
-            u32 bi = TOP_NONE, bk = 0;
+        for (u32 k = 0; k < N; k++) {
+            const bool in = valid[k] && top_better(x[k], idx[k], tv, ti);
+            left |= (u32)in << k;
+            n += (u32)__popcll(__ballot(in));
+        }
+#pragma unroll 1
+        while (n) {
+            if (count + n > 64) sort();
+            n = 0;
 #pragma unroll
-            for (u32 k = 0; k < N; k++)
-                if ((left >> k & 1) && top_better(x[k], idx[k], bv, bi)) bv = x[k], bi = idx[k], bk = k;
-            if (!__ballot(top_better(bv, bi, tv, ti))) return;
-            left &= ~(1u << bk);
-            insert(top, bi != TOP_NONE, bv, bi);
+            for (u32 k = 0; k < N; k++) {
+                const bool in = (left >> k & 1) && top_better(x[k], idx[k], tv, ti);
+                const u64 b = __ballot(in);
+                const u32 at = count + (u32)__popcll(b & ((1ull << lane) - 1)), c = (u32)__popcll(b), room = 64 - count;
+                if (in && at < 64) {
+                    buf[at] = TopEntry{x[k], idx[k], 0};
+                    left &= ~(1u << k);
+                }
+                count += c < room ? c : room;
+                n += c < room ? 0 : c - room;
+            }
+            prg_wave_sync();
         }
     }
 };
@@ -618,49 +634,33 @@ template <u32 K> __device__ inline float top_border(const float (&near)[K], u32 
     }
     return hi;
 }
-// The first tile of a wavefront: N candidates per lane at once.  With the border distance of the lanes' N / 2 pair maxima
-// (`all`: there are no more than 64 candidates, and none), what lies within it (rarely more than a few above `top`) is gathered in `buf`.  Returns its number, or 0 where more
-// than 64 lie within it (many equal words): then the candidates have been inserted one by one.
+// The first tile of a wavefront: only what lies within the border distance of the lanes' N / 2 pair maxima is a candidate
+// (rarely more than a few above `top`).
 template <u32 N>
-__device__ inline u32 top_first(WaveTop &t, u32 top, const i64 (&x)[N], const u32 (&idx)[N], const bool (&valid)[N], i64 lane_max,
-                                float guess, bool all, TopEntry *buf) {
-    const u32 lane = threadIdx.x & 63;
+__device__ inline void top_first(WaveTop &t, const i64 (&x)[N], const u32 (&idx)[N], const bool (&valid)[N], i64 lane_max, float guess) {
     const i64 m = wave_max(lane_max);
     float near[N / 2];
 #pragma unroll
     for (u32 k = 0; k < N / 2; k++) near[k] = valid[2 * k] ? word_dist(m, valid[2 * k + 1] && x[2 * k + 1] > x[2 * k] ? x[2 * k + 1] : x[2 * k]) : -1.0f;
-    const float border = all ? INFINITY : top_border<N / 2>(near, top, guess);
-    u32 count = 0;
-    u32 slot[N];
+    const float border = top_border<N / 2>(near, t.top, guess);
+    bool in[N];
+    u32 at[N], n = 0;
 #pragma unroll
     for (u32 k = 0; k < N; k++) {
-        const u64 b = __ballot(valid[k] && word_dist(m, x[k]) <= border);
-        slot[k] = ((b >> lane) & 1) ? count + (u32)__popcll(b & ((1ull << lane) - 1)) : TOP_NONE;
-        count += (u32)__popcll(b);
+        in[k] = valid[k] && word_dist(m, x[k]) <= border;
+        const u64 b = __ballot(in[k]);
+        at[k] = n + (u32)__popcll(b & ((1ull << (threadIdx.x & 63)) - 1));
+        n += (u32)__popcll(b);
     }
-    if (count > 64) {
-        t.insert_all(top, x, idx, valid);
-        return 0;
+    if (n > 64) { // many equal words
+        t.add(x, idx, in);
+        return;
     }
 #pragma unroll
     for (u32 k = 0; k < N; k++)
-        if (slot[k] != TOP_NONE) buf[slot[k]] = TopEntry{x[k], idx[k], 0};
+        if (in[k]) t.buf[at[k]] = TopEntry{x[k], idx[k], 0};
+    t.count = n;
     prg_wave_sync();
-    return count;
-}
-// the `count` entries of buf, sorted by counting the better ones of each, become the wavefront's list
-__device__ inline void top_sort(WaveTop &t, u32 top, u32 count, TopEntry *buf) {
-    const u32 lane = threadIdx.x & 63;
-    const TopEntry e = lane < count ? buf[lane] : TopEntry{INT64_MIN, TOP_NONE, 0};
-    u32 rank = 0;
-#pragma unroll 8
-    for (u32 k = 0; k < count; k++) rank += top_better(buf[k].v, buf[k].i, e.v, e.i);
-    prg_wave_sync();
-    if (lane < count) buf[rank] = e;
-    prg_wave_sync();
-    if (lane < count && lane < top) t.v = buf[lane].v, t.i = buf[lane].i;
-    prg_wave_sync();
-    t.border(top);
 }
 // The lists of the W wavefronts of a workgroup (in `lists`, `top` entries each) -> out[0 .. top): every entry counts the
 // better ones.  Entries that are not there stay behind the rest.  All threads call it; ends with a barrier.
@@ -757,8 +757,7 @@ template <u32 W, bool SPLIT, int SH> __global__ __launch_bounds__(256) void logp
     if (W == 1 && row >= A.rows) return; // a wavefront of its own: no barrier follows
     const u64 base = row * A.vocab, j0 = split * A.chunk, j1 = j0 + A.chunk < A.vocab ? j0 + A.chunk : A.vocab;
     RowSums s;
-    WaveTop top;
-    u32 count = 0; // entries in buf that are not in `top` yet
+    WaveTop top(buf[wave], A.top);
     bool first = true;
     for (u64 tile = j0 + (W == 1 ? 0 : wave) * TILE; tile < j1; tile += W * TILE) {
         i64 x[N];
@@ -791,50 +790,59 @@ template <u32 W, bool SPLIT, int SH> __global__ __launch_bounds__(256) void logp
             s.S += e, s.T = fmaf(d, e, s.T);
         }
         if (A.top) {
-            if (first) {
-                count = top_first<N>(top, A.top, x, idx, valid, m, 16.0f / A.unit, j1 - tile <= 64, buf[wave]);
-                first = false;
-            } else {
-                if (count) top_sort(top, A.top, count, buf[wave]), count = 0;
-                if (__ballot(m >= top.tv)) top.insert_all(A.top, x, idx, valid);
+            if (first && j1 - tile > 64) {
+                top_first<N>(top, x, idx, valid, m, 16.0f / A.unit);
+            } else if (__ballot(m >= top.tv)) {
+                if (top.count > A.top) top.sort(); // for a border that is up to date
+                // the border's entry has a lower index than this tile's words, so equal words do not beat it; and a lane
+                // hardly ever has two that do
+                u32 over = 0;
+#pragma unroll
+                for (u32 k = 0; k < N; k++) over |= (u32)(valid[k] && x[k] > top.tv) << k;
+                const u64 lanes = __ballot(over);
+                if (__ballot(over & (over - 1)) || top.count + (u32)__popcll(lanes) > 64 || top.ti == TOP_NONE) {
+                    top.add(x, idx, valid);
+                } else if (lanes) {
+                    const u32 k = (u32)__builtin_ctz(over | 256);
+                    top.append(over, m, (u32)tile + 128 * (k / 2) + 2 * lane + (k & 1));
+                }
             }
+            first = false;
         }
     }
     s.wave_join(A.unit2);
+    if (A.top && (!SPLIT || top.count > LIST)) top.sort();
     if (SPLIT) {
         const u64 part = group * 4 + wave;
         if (lane == 0) A.parts[part] = RowPart{s.m, s.S, s.T};
         if (A.top) {
-            if (count > LIST) top_sort(top, A.top, count, buf[wave]), count = 0;
-            TopEntry e{lane < A.top ? top.v : INT64_MIN, lane < A.top ? top.i : TOP_NONE, 0};
-            if (count) e = lane < count ? buf[wave][lane] : TopEntry{INT64_MIN, TOP_NONE, 0};
-            if (lane < LIST) A.lists[part * LIST + lane] = e;
+            if (lane < LIST) A.lists[part * LIST + lane] = lane < top.count ? top.buf[lane] : TopEntry{INT64_MIN, TOP_NONE, 0};
         }
         return;
     }
-    if (count) top_sort(top, A.top, count, buf[wave]);
     if (W == 1) {
-        if (lane < A.top) buf[wave][lane] = TopEntry{top.v, top.i, 0};
-        prg_wave_sync();
         logprobs_finish(in, A, row, s, buf[wave], lane, 64);
         return;
     }
     if (lane == 0) ws[wave] = RowPart{s.m, s.S, s.T};
+    const TopEntry mine = lane < top.count ? top.buf[lane] : TopEntry{INT64_MIN, TOP_NONE, 0};
     __syncthreads(); // every wavefront has left its own part of buf
     TopEntry *lists = &buf[0][0];
-    if (lane < A.top) lists[wave * A.top + lane] = TopEntry{top.v, top.i, 0};
+    if (lane < A.top) lists[wave * A.top + lane] = mine;
     s = RowSums();
     for (u32 w = 0; w < 4; w++) s.join(ws[w], A.unit2);
     __syncthreads();
     if (A.top) top_merge<4>(lists, merged, A.top);
     logprobs_finish(in, A, row, s, merged, tid, 256);
 }
+constexpr u32 JOIN_THREADS = 512; // 256 / 512 / 1024: 9.4 / 8.2 / 8.1 us for one row of 131072 with 20 alternatives
 // Joins the parts of a row: one workgroup per row.  What counts is the time of one such call, so parts and lists are asked
 // for together and every wavefront forms the maximum and the border (from the lanes' maxima over four interleaved sets of
 // parts each) for itself; its entries within the border go to LDS, and after the one barrier the first wavefront sorts
 // them.
-template <int SH> __global__ __launch_bounds__(1024) void logprobs_join_kernel(LogitIn<SH> in, LogprobArgs A) {
-    constexpr u32 K = 4, E = 8;
+template <int SH> __global__ __launch_bounds__(JOIN_THREADS) void logprobs_join_kernel(LogitIn<SH> in, LogprobArgs A) {
+    constexpr u32 JOIN_THREADS = 512; // 256 / 512 / 1024: 9.4 / 8.2 / 8.1 us for one row of 131072 with 20 alternatives
+    constexpr u32 K = 4, THREADS = JOIN_THREADS, E = 8192 / THREADS;
     __shared__ TopEntry buf[64];
     __shared__ u32 count;
     const u32 tid = threadIdx.x, lane = tid & 63;
@@ -846,7 +854,7 @@ template <int SH> __global__ __launch_bounds__(1024) void logprobs_join_kernel(L
     TopEntry e[E];
 #pragma unroll
     for (u32 k = 0; k < E; k++) {
-        const u32 j = k * blockDim.x + tid;
+        const u32 j = k * THREADS + tid;
         e[k] = j < slots ? lists[j] : TopEntry{INT64_MIN, TOP_NONE, 0};
     }
     RowSums s;
@@ -878,11 +886,11 @@ template <int SH> __global__ __launch_bounds__(1024) void logprobs_join_kernel(L
         border = top_border<K>(near, A.top, 16.0f / A.unit);
     }
     __syncthreads();
-    for (u32 j0 = 0; j0 < slots; j0 += E * blockDim.x) {
+    for (u32 j0 = 0; j0 < slots; j0 += E * THREADS) {
         if (j0) {
 #pragma unroll
             for (u32 k = 0; k < E; k++) {
-                const u32 j = j0 + k * blockDim.x + tid;
+                const u32 j = j0 + k * THREADS + tid;
                 e[k] = j < slots ? lists[j] : TopEntry{INT64_MIN, TOP_NONE, 0};
             }
         }
@@ -895,19 +903,21 @@ template <int SH> __global__ __launch_bounds__(1024) void logprobs_join_kernel(L
     }
     __syncthreads();
     if (tid < 64 && A.top) {
-        WaveTop top;
+        WaveTop top(buf, A.top);
         if (count <= 64) {
-            top_sort(top, A.top, count, buf);
-        } else { // many equal words: all lists, one entry after the other
+            top.count = count;
+        } else { // many equal words: all lists, one after the other
             for (u32 j = lane; j - lane < slots; j += 64) {
                 const TopEntry q = j < slots ? lists[j] : TopEntry{INT64_MIN, TOP_NONE, 0};
-                top.insert(A.top, q.i != TOP_NONE, q.v, q.i);
+                const i64 x[1] = {q.v};
+                const u32 idx[1] = {q.i};
+                const bool valid[1] = {q.i != TOP_NONE};
+                top.add(x, idx, valid);
             }
         }
-        if (lane < A.top) buf[lane] = TopEntry{top.v, top.i, 0};
-        prg_wave_sync();
+        top.sort();
     }
-    logprobs_finish(in, A, row, s, buf, tid, blockDim.x, id, at_id);
+    logprobs_finish(in, A, row, s, buf, tid, THREADS, id, at_id);
 }
 
 // The gradient.  A workgroup takes `chunk` words of a row, 16 bytes of each share per load and GRAD_PAIRS of them together;
@@ -1003,8 +1013,7 @@ template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, const LogprobA
         hipLaunchKernelGGL((logprobs_kernel<4, false, SH>), dim3((u32)A.rows), dim3(256), 0, ctx->stream, in, A);
     MPCX_LAUNCH_CHECK();
     if (A.splits > 1) {
-        const u64 threads = A.top ? ceil_div((u64)A.splits * 4 * LIST / 8, 64) * 64 : 64; // eight entries each
-        hipLaunchKernelGGL(logprobs_join_kernel<SH>, dim3((u32)A.rows), dim3((u32)(threads < 1024 ? threads : 1024)), 0, ctx->stream, in, A);
+        hipLaunchKernelGGL(logprobs_join_kernel<SH>, dim3((u32)A.rows), dim3(JOIN_THREADS), 0, ctx->stream, in, A);
         MPCX_LAUNCH_CHECK();
     }
     return 0;
