@@ -166,19 +166,19 @@ template <bool TWO, u32 NS> struct RowAcc {
         }
     }
 };
-// the sums of four wavefronts in the first one (one 16-byte piece of each share per lane); all threads call it
-template <bool TWO> __device__ inline void join_waves(RowAcc<TWO, 1> &acc, u64x2 *lds) {
+// the sums of WAVES wavefronts in the first one (one 16-byte piece of each share per lane); all threads call it
+template <bool TWO, u32 WAVES> __device__ inline void join_waves(RowAcc<TWO, 1> &acc, u64x2 *lds) {
     const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
     if (wave) {
         lds[(wave - 1) * 64 + lane] = acc.a[0];
-        if (TWO) lds[(wave + 2) * 64 + lane] = acc.b[0];
+        if (TWO) lds[(WAVES - 1 + wave - 1) * 64 + lane] = acc.b[0];
     }
     __syncthreads();
     if (wave == 0)
-        for (u32 w = 0; w < 3; w++) {
+        for (u32 w = 0; w < WAVES - 1; w++) {
             acc.a[0] += lds[w * 64 + lane];
-            if (TWO) acc.b[0] += lds[(w + 3) * 64 + lane];
+            if (TWO) acc.b[0] += lds[(WAVES - 1 + w) * 64 + lane];
         }
 }
 
@@ -228,28 +228,90 @@ template <bool TWO> __global__ __launch_bounds__(256) void embed_grad_small_kern
         if (off[r + 1] - off[r] <= GRAD_ALONE) continue;
         RowAcc<TWO, 1> acc;
         acc.template add_rows<8>(row, A.G0, A.G1, off[r] + wave, off[r + 1], 4, c0, 0, A.dim);
-        join_waves<TWO>(acc, lds);
+        join_waves<TWO, 4>(acc, lds);
         if (wave == 0) acc.template write<false>(A, v0 + r, c0, 0);
     }
 }
 
-// Many tokens: the tokens are put in the order of their rows first (a counting sort, in which the rows' places are taken
-// as they come: sums mod 2^64 do not depend on it), then every row is added by one group of lanes.  A row of more than
-// GRAD_CHUNK tokens is cut into at most GRAD_MAX_CHUNKS chunks, whose sums go through scratch memory.
-constexpr u32 GRAD_TOGETHER = 4, GRAD_CHUNK = 32, GRAD_MAX_CHUNKS = 256;
-struct GradChunk {
-    u32 first, count; // in the ordered tokens
-};
-struct GradHeavy {
-    u32 row, first, count, pad; // its chunks
-};
+// Many tokens: the tokens are put in the order of their rows first (a counting sort; the order inside a row is as it
+// comes, sums mod 2^64 do not depend on it), then every row is added by one group of lanes.  A heavy row, of more than
+// GRAD_CHUNK tokens, is added chunk by chunk: chunk k is the places [GRAD_CHUNK k, GRAD_CHUNK (k + 1)) of the order, which
+// no heavy row lies inside of, so that it meets two at most; their sums go through scratch memory, and the workgroups of
+// the chunk that a heavy row begins in add them up.
+constexpr u32 GRAD_TOGETHER = 4, GRAD_CHUNK = 32;
 struct GradWork {
-    u32 *cursor; // [0] ordered tokens given out, [1] chunks, [2] heavy rows
+    u32 *total; // places of the order: tokens inside the vocabulary
     u32 *count, *start, *rank, *order;
-    GradChunk *chunks;
-    GradHeavy *heavy;
-    u64 *partial; // per chunk: dim words of each share
+    u32 *ends;    // the rows of the first and the last place of each full chunk
+    u64 *partial; // two sums of each chunk: dim words of each share
+    __device__ void place(u32 at, u32 t, u32 v) const {
+        order[at] = t;
+        const u32 p = at % GRAD_CHUNK;
+        if (p == 0) ends[2 * (at / GRAD_CHUNK)] = v;
+        if (p == GRAD_CHUNK - 1) ends[2 * (at / GRAD_CHUNK) + 1] = v;
+    }
 };
+// chunk k: its places, and the rows of the first and the last one
+struct GradChunk {
+    u32 p0, p1, va, vb;
+    __device__ GradChunk(const GradWork &W, const i64 *ids, u32 total, u32 k) {
+        p0 = k * GRAD_CHUNK, p1 = total - p0 < GRAD_CHUNK ? total : p0 + GRAD_CHUNK;
+        va = W.ends[2 * k];
+        vb = p1 - p0 == GRAD_CHUNK ? W.ends[2 * k + 1] : (u32)ids[W.order[p1 - 1]];
+    }
+};
+// The whole sort in one launch: a workgroup owns `rows` rows of the table and looks through all ids twice, counting its
+// tokens in LDS (and those of the rows before, which gives its first place), then placing them.  65536 tokens: 10 us;
+// a histogram in memory takes four launches and 30 us, and less from about GRAD_SCAN_N tokens on.
+constexpr u32 GRAD_SCAN_ROWS = 4096, GRAD_SCAN_THREADS = 1024;
+__global__ __launch_bounds__(1024) void grad_scan_kernel(const i64 *__restrict__ ids, u32 n, u64 vocab, u32 rows, GradWork W) {
+    __shared__ u32 cnt[GRAD_SCAN_ROWS], ws[16], wb[16];
+    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const u64 v0 = (u64)blockIdx.x * rows;
+    const u32 own = (u32)(vocab - v0 < rows ? vocab - v0 : rows);
+    for (u32 r = tid; r < GRAD_SCAN_ROWS; r += GRAD_SCAN_THREADS) cnt[r] = 0;
+    __syncthreads();
+    u32 below = 0;
+#pragma unroll 4
+    for (u32 t = tid; t < n; t += GRAD_SCAN_THREADS) {
+        const u64 v = (u64)ids[t];
+        below += v < v0;
+        if (v - v0 < own) atomicAdd(&cnt[v - v0], 1u);
+    }
+    __syncthreads();
+    u32 c[4], s = 0; // four rows of a thread
+#pragma unroll
+    for (u32 k = 0; k < 4; k++) c[k] = cnt[4 * tid + k], s += c[k];
+    u32 sum = s;
+    for (u32 d = 1; d < 64; d <<= 1) {
+        const u32 o = (u32)__shfl_up((int)sum, d);
+        if (lane >= d) sum += o;
+    }
+    for (u32 d = 32; d; d >>= 1) below += (u32)__shfl_xor((int)below, d);
+    if (lane == 63) ws[wave] = sum;
+    if (lane == 0) wb[wave] = below;
+    __syncthreads();
+    u32 at = sum - s, mine = 0;
+    for (u32 w = 0; w < 16; w++) {
+        at += wb[w] + (w < wave ? ws[w] : 0);
+        mine += ws[w];
+    }
+    if (tid == GRAD_SCAN_THREADS - 1 && v0 + own == vocab) *W.total = at + s;
+#pragma unroll
+    for (u32 k = 0; k < 4; k++) {
+        const u32 r = 4 * tid + k;
+        if (r < own) W.count[v0 + r] = c[k], W.start[v0 + r] = at;
+        cnt[r] = at;
+        at += c[k];
+    }
+    __syncthreads();
+    if (mine)
+#pragma unroll 4
+        for (u32 t = tid; t < n; t += GRAD_SCAN_THREADS) {
+            const u64 r = (u64)ids[t] - v0;
+            if (r < own) W.place(atomicAdd(&cnt[r], 1u), t, (u32)(v0 + r));
+        }
+}
 __global__ __launch_bounds__(256) void grad_clear_kernel(u32 *p, u64 n) {
     for (u64 i = (u64)blockIdx.x * 256 + threadIdx.x; i < n; i += (u64)gridDim.x * 256) p[i] = 0;
 }
@@ -287,6 +349,7 @@ __global__ __launch_bounds__(256) void grad_count_kernel(const i64 *__restrict__
     for (u32 q = 0; q < GRAD_TOKENS / 256; q++)
         if (slot[q] != ~0u) W.rank[blockIdx.x * GRAD_TOKENS + 256 * q + tid] = num[slot[q]] + rank[q];
 }
+// the rows' first places, in the order in which the workgroups come
 __global__ __launch_bounds__(256) void grad_place_kernel(u32 vocab, GradWork W) {
     __shared__ u32 ws[4], at;
     const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -300,50 +363,42 @@ __global__ __launch_bounds__(256) void grad_place_kernel(u32 vocab, GradWork W) 
     if (lane == 63) ws[wave] = s;
     __syncthreads();
     if (tid == 0) {
-        const u32 total = ws[0] + ws[1] + ws[2] + ws[3];
-        at = total ? atomicAdd(&W.cursor[0], total) : 0;
+        const u32 sum = ws[0] + ws[1] + ws[2] + ws[3];
+        at = sum ? atomicAdd(W.total, sum) : 0;
     }
     __syncthreads();
     u32 first = at + s - c;
     for (u32 w = 0; w < wave; w++) first += ws[w];
     if (v < vocab) W.start[v] = first;
-    u32 size = 0, k = 0, slot = 0;
-    if (c > GRAD_CHUNK) {
-        size = (c + GRAD_MAX_CHUNKS - 1) / GRAD_MAX_CHUNKS;
-        if (size < GRAD_CHUNK) size = GRAD_CHUNK;
-        k = (c + size - 1) / size;
-        slot = atomicAdd(&W.cursor[1], k);
-        W.heavy[atomicAdd(&W.cursor[2], 1u)] = GradHeavy{v, slot, k, 0};
-    }
-    for (u64 heavy = __ballot(k != 0); heavy; heavy &= heavy - 1) { // a row's chunks are written by the whole wavefront
-        const int src = __builtin_ctzll(heavy);
-        const u32 hk = __shfl(k, src), hs = __shfl(size, src), hf = __shfl(first, src), hc = __shfl(c, src), hb = __shfl(slot, src);
-        for (u32 i = lane; i < hk; i += 64) W.chunks[hb + i] = GradChunk{hf + i * hs, hc - i * hs < hs ? hc - i * hs : hs};
-    }
 }
 __global__ __launch_bounds__(256) void grad_order_kernel(const i64 *__restrict__ ids, u32 n, u64 vocab, GradWork W) {
     const u32 t = blockIdx.x * 256 + threadIdx.x;
     if (t >= n) return;
     const u64 v = (u64)ids[t];
-    if (v < vocab) W.order[W.start[v] + W.rank[t]] = t;
+    if (v < vocab) W.place(W.start[v] + W.rank[t], t, (u32)v);
 }
-// The first `heavy_blocks` workgroups add the chunks of the heavy rows into scratch memory, 128 columns per wavefront; the
-// others one row of the table, 128 columns or less, per 2^lg lanes.
+// The first `heavy_blocks` workgroups add the chunks' parts of heavy rows into scratch memory, 128 columns per wavefront;
+// the others one row of the table, 128 columns or less, per 2^lg lanes.
 template <bool TWO, bool STREAM>
 __global__ __launch_bounds__(256) void grad_rows_kernel(GradArgs A, GradWork W, u32 heavy_blocks, u32 lg, u32 slices) {
     RowAcc<TWO, 1> acc;
     if (blockIdx.x < heavy_blocks) {
-        const u64 items = (u64)W.cursor[1] * slices;
+        const u32 total = *W.total;
+        const u64 items = (u64)((total + GRAD_CHUNK - 1) / GRAD_CHUNK) * slices;
         for (u64 it = (u64)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += (u64)heavy_blocks * 4) {
             const u64 k = it / slices, c0 = (it % slices) * 128 + 2 * (threadIdx.x & 63);
-            const GradChunk ch = W.chunks[k];
-            const u32 *list = W.order + ch.first;
-            acc = RowAcc<TWO, 1>();
-            acc.template add_rows<GRAD_TOGETHER>([&](u32 i) { return (u64)list[i] * A.dim; }, A.G0, A.G1, 0, ch.count, 1, c0, 0, A.dim);
-            if (c0 >= A.dim) continue;
-            u64 *p = W.partial + k * 2 * A.dim + c0;
-            acc.template put<false>(p, acc.a[0], c0 + 1 < A.dim, 0);
-            if (TWO) acc.template put<false>(p + A.dim, acc.b[0], c0 + 1 < A.dim, 0);
+            const GradChunk ch(W, A.ids, total, (u32)k);
+            for (u32 side = 0; side < (ch.va == ch.vb ? 1u : 2u); side++) {
+                const u32 v = side ? ch.vb : ch.va, c = W.count[v], first = W.start[v];
+                if (c <= GRAD_CHUNK) continue;
+                const u32 i0 = first > ch.p0 ? first : ch.p0, i1 = first + c < ch.p1 ? first + c : ch.p1;
+                acc = RowAcc<TWO, 1>();
+                acc.template add_rows<GRAD_TOGETHER>([&](u32 i) { return (u64)W.order[i] * A.dim; }, A.G0, A.G1, i0, i1, 1, c0, 0, A.dim);
+                if (c0 >= A.dim) continue;
+                u64 *p = W.partial + (2 * k + side) * 2 * A.dim + c0;
+                acc.template put<false>(p, acc.a[0], c0 + 1 < A.dim, 0);
+                if (TWO) acc.template put<false>(p + A.dim, acc.b[0], c0 + 1 < A.dim, 0);
+            }
         }
         return;
     }
@@ -357,19 +412,40 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(GradArgs A, GradWork W, 
     acc.template add_rows<GRAD_TOGETHER>([&](u32 i) { return (u64)list[i] * A.dim; }, A.G0, A.G1, 0, c, 1, c0, 0, A.dim);
     acc.template write<STREAM>(A, v, c0, 0);
 }
-// a heavy row's 128 columns: its chunks' sums, shared out to the four wavefronts of a workgroup
-template <bool TWO> __global__ __launch_bounds__(256) void grad_heavy_kernel(GradArgs A, GradWork W) {
-    __shared__ u64x2 lds[3 * (TWO ? 2 : 1) * 64];
-    const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const u64 slices = (A.dim + 127) / 128, items = (u64)W.cursor[2] * slices;
-    for (u64 it = blockIdx.x; it < items; it += gridDim.x) {
-        const GradHeavy h = W.heavy[it / slices];
-        const u64 c0 = (it % slices) * 128 + 2 * lane;
-        const u64 *p = W.partial + (u64)h.first * 2 * A.dim;
+// 128 columns of the heavy rows that begin in eight chunks (one at most does in each): a wavefront looks at one chunk and
+// adds the sums of its row when they are few; those of a longer row are shared out to all wavefronts.
+constexpr u32 HEAVY_WAVES = 8, HEAVY_ALONE = 8;
+template <bool TWO> __global__ __launch_bounds__(64 * HEAVY_WAVES) void grad_heavy_kernel(GradArgs A, GradWork W, u32 slices) {
+    __shared__ u64x2 lds[(HEAVY_WAVES - 1) * (TWO ? 2 : 1) * 64];
+    __shared__ u32 begin[HEAVY_WAVES], chunks[HEAVY_WAVES], rows[HEAVY_WAVES]; // the sum of the first chunk, how many, the row
+    const u32 total = *W.total, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const u32 k = blockIdx.x / slices * HEAVY_WAVES + wave;
+    const u64 c0 = (u64)(blockIdx.x % slices) * 128 + 2 * lane;
+    u32 n = 0, b = 0, v = 0;
+    if ((u64)k * GRAD_CHUNK < total) {
+        const GradChunk ch(W, A.ids, total, k);
+        const u32 c = W.count[ch.vb], first = W.start[ch.vb];
+        if (c > GRAD_CHUNK && first >= ch.p0) n = (first + c - 1) / GRAD_CHUNK - k + 1;
+        b = 2 * k + (ch.va != ch.vb), v = ch.vb;
+    }
+    // the first chunk's sum is the one of its last row, every other chunk's that of its first row
+    auto add = [&](RowAcc<TWO, 1> &acc, u32 b, u32 i0, u32 n, u32 step) {
+        acc.template add_rows<8>([&](u32 i) { return (u64)(i ? (b & ~1u) + 2 * i : b) * 2 * A.dim; }, W.partial, W.partial + A.dim, i0,
+                                 n, step, c0, 0, A.dim);
+    };
+    if (lane == 0) begin[wave] = b, rows[wave] = v, chunks[wave] = n > HEAVY_ALONE ? n : 0;
+    if (n && n <= HEAVY_ALONE) {
         RowAcc<TWO, 1> acc;
-        acc.template add_rows<8>([&](u32 i) { return (u64)i * 2 * A.dim; }, p, p + A.dim, wave, h.count, 4, c0, 0, A.dim);
-        join_waves<TWO>(acc, lds);
-        if (wave == 0) acc.template write<false>(A, h.row, c0, 0);
+        add(acc, b, 0, n, 1);
+        acc.template write<false>(A, v, c0, 0);
+    }
+    __syncthreads();
+    for (u32 q = 0; q < HEAVY_WAVES; q++) {
+        if (chunks[q] == 0) continue;
+        RowAcc<TWO, 1> acc;
+        add(acc, begin[q], wave, chunks[q], HEAVY_WAVES);
+        join_waves<TWO, HEAVY_WAVES>(acc, lds);
+        if (wave == 0) acc.template write<false>(A, rows[q], c0, 0);
     }
 }
 
@@ -1019,30 +1095,38 @@ template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, const LogprobA
     return 0;
 }
 
-constexpr u64 GRAD_SMALL_SCAN = 1 << 24;
+// Ids that the one-launch form reads, up to which it is taken: n ids for each of its workgroups
+#ifndef LM_SS
+#define LM_SS (1 << 22)
+#endif
+#ifndef LM_HB
+#define LM_HB 1024
+#endif
+#ifndef LM_SN
+#define LM_SN (1 << 15)
+#endif
+constexpr u64 GRAD_SMALL_SCAN = LM_SS, GRAD_SCAN_N = LM_SN;
 // scratch memory of the many-token form, in 8-byte words from its start
 struct GradLayout {
-    u64 cursor, count, start, rank, order, chunks, heavy, partial, words;
-    GradLayout(u64 n, u64 vocab, u64 dim) {
-        // a heavy row has more than GRAD_CHUNK tokens, and its chunks hold GRAD_CHUNK tokens or more, all but the last one
-        const u64 max_heavy = n / (GRAD_CHUNK + 1), max_chunks = n / GRAD_CHUNK + max_heavy;
+    u64 total, count, start, rank, order, ends, partial, words, rows, n;
+    bool scan() const { return n <= GRAD_SCAN_N && rows <= GRAD_SCAN_ROWS; } // sorted by one launch, `rows` rows a workgroup
+    GradLayout(u64 n_, u64 vocab, u64 dim) : rows(ceil_div(vocab, 256) < GRAD_ROWS ? GRAD_ROWS : ceil_div(vocab, 256)), n(n_) {
         u64 at = 0;
         auto take = [&](u64 &where, u64 bytes) { where = at, at += ceil_div(bytes, 16) * 2; };
-        take(cursor, 16);
-        take(count, 4 * vocab); // right behind the cursors: cleared together
+        take(total, 16);
+        take(count, 4 * vocab); // right behind the total: cleared together
         take(start, 4 * vocab);
-        take(rank, 4 * n);
+        take(rank, scan() ? 0 : 4 * n);
         take(order, 4 * n);
-        take(chunks, max_chunks * sizeof(GradChunk));
-        take(heavy, max_heavy * sizeof(GradHeavy));
-        take(partial, max_chunks * 2 * dim * 8);
+        take(ends, n / GRAD_CHUNK * 8 + 8);
+        take(partial, n > GRAD_CHUNK ? ceil_div(n, GRAD_CHUNK) * 4 * dim * 8 : 0);
         words = at;
     }
 };
 template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *scratch) {
-    if (A.n <= GRAD_SMALL_N && A.n * A.vocab <= GRAD_SMALL_SCAN) {
-        const u64 slices = ceil_div(A.dim, 128);
-        MPCX_REQUIRE(slices < 65536, "mpcx_ring_embed_grad: rows of %llu words", (unsigned long long)A.dim);
+    const u64 slices = ceil_div(A.dim, 128);
+    const u64 small_blocks = ceil_div(A.vocab, GRAD_ROWS) * slices;
+    if (A.n <= GRAD_SMALL_N && A.n * small_blocks <= GRAD_SMALL_SCAN && slices < 65536) {
         hipLaunchKernelGGL(embed_grad_small_kernel<TWO>, dim3((u32)ceil_div(A.vocab, GRAD_ROWS), (u32)slices), dim3(256), 0,
                            ctx->stream, A);
         MPCX_LAUNCH_CHECK();
@@ -1050,22 +1134,29 @@ template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *s
     }
     const GradLayout L(A.n, A.vocab, A.dim);
     u64 *w = (u64 *)scratch;
-    const GradWork W{(u32 *)(w + L.cursor), (u32 *)(w + L.count), (u32 *)(w + L.start), (u32 *)(w + L.rank), (u32 *)(w + L.order),
-                     (GradChunk *)(w + L.chunks), (GradHeavy *)(w + L.heavy), w + L.partial};
-    const u32 n = (u32)A.n, vb = (u32)ceil_div(A.vocab, 256);
+    const GradWork W{(u32 *)(w + L.total), (u32 *)(w + L.count), (u32 *)(w + L.start), (u32 *)(w + L.rank), (u32 *)(w + L.order),
+                     (u32 *)(w + L.ends), w + L.partial};
+    const u32 n = (u32)A.n;
     u32 lg = 3; // lanes of a row: up to a wavefront
     while (lg < 6 && (2ull << lg) < A.dim) lg++;
-    const u64 slices = ceil_div(A.dim, 128), heavy_blocks = n > GRAD_CHUNK ? 512 : 0; // otherwise no row is heavy
-    const u64 blocks = ceil_div(A.vocab * slices, 256u >> lg) + heavy_blocks;
-    MPCX_REQUIRE(blocks < (1ull << 31), "mpcx_ring_embed_grad: table too large for one launch");
-    hipLaunchKernelGGL(grad_clear_kernel, dim3(vb), dim3(256), 0, ctx->stream, W.cursor, 4 + A.vocab);
-    if (n) hipLaunchKernelGGL(grad_count_kernel, dim3((u32)ceil_div(n, GRAD_TOKENS)), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
-    hipLaunchKernelGGL(grad_place_kernel, dim3(vb), dim3(256), 0, ctx->stream, (u32)A.vocab, W);
-    if (n) hipLaunchKernelGGL(grad_order_kernel, dim3((u32)ceil_div(n, 256)), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
+    const u64 heavy_blocks = n <= GRAD_CHUNK ? 0 : A.n > A.vocab ? LM_HB : 512; // otherwise no row is heavy
+    const u64 blocks = ceil_div(A.vocab * slices, 256u >> lg) + heavy_blocks, chunks = ceil_div(n, GRAD_CHUNK);
+    MPCX_REQUIRE(blocks < (1ull << 31) && chunks * slices < (1ull << 31), "mpcx_ring_embed_grad: sizes too large for one launch");
+    if (L.scan()) {
+        hipLaunchKernelGGL(grad_scan_kernel, dim3((u32)ceil_div(A.vocab, L.rows)), dim3(GRAD_SCAN_THREADS), 0, ctx->stream, A.ids, n,
+                           A.vocab, (u32)L.rows, W);
+    } else {
+        const u32 vb = (u32)ceil_div(A.vocab, 256);
+        hipLaunchKernelGGL(grad_clear_kernel, dim3(vb), dim3(256), 0, ctx->stream, W.total, 4 + A.vocab);
+        if (n) hipLaunchKernelGGL(grad_count_kernel, dim3((u32)ceil_div(n, GRAD_TOKENS)), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
+        hipLaunchKernelGGL(grad_place_kernel, dim3(vb), dim3(256), 0, ctx->stream, (u32)A.vocab, W);
+        if (n) hipLaunchKernelGGL(grad_order_kernel, dim3((u32)ceil_div(n, 256)), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
+    }
     const bool stream = (A.n + A.vocab) * A.dim * (TWO ? 16 : 8) > STREAM_BYTES;
     hipLaunchKernelGGL((stream ? grad_rows_kernel<TWO, true> : grad_rows_kernel<TWO, false>), dim3((u32)blocks), dim3(256), 0,
                        ctx->stream, A, W, (u32)heavy_blocks, lg, (u32)slices);
-    if (heavy_blocks) hipLaunchKernelGGL(grad_heavy_kernel<TWO>, dim3(2048), dim3(256), 0, ctx->stream, A, W);
+    if (heavy_blocks)
+        hipLaunchKernelGGL(grad_heavy_kernel<TWO>, dim3((u32)(ceil_div(chunks, HEAVY_WAVES) * slices)), dim3(64 * HEAVY_WAVES), 0, ctx->stream, A, W, (u32)slices);
     MPCX_LAUNCH_CHECK();
     return 0;
 }

@@ -81,6 +81,24 @@ def test_embed_grad(gpu, vocab, dim, n, kind, shares):
             assert np.array_equal(g, ref.embed_grad(G[k], ids, vocab, dim, scale, shift)), (scale, shift, k)
 
 
+@pytest.mark.parametrize("vocab,dim,n,kind", [(300, 130, 5000, "zipf"), (300, 130, 5000, "one"), (9000, 40, 140001, "zipf"),
+                                              (3, 200, 140001, "zipf"), (1100000, 2, 70, "zipf"), (1100000, 2, 5000, "one"),
+                                              (33, 1030, 4100, "cycle"), (33, 257, 33 * 32, "cycle"), (33, 257, 33 * 33, "cycle"),
+                                              (700, 129, 40000, "cycle"), (20, 5, 6000, "none"), (5000, 300, 4097, "zipf")])
+@pytest.mark.parametrize("shares", [1, 2])
+def test_embed_grad_of_many_tokens(gpu, vocab, dim, n, kind, shares):
+    """Rows of 32, 33, .. tokens at every place of the order, texts of one token, vocabularies and lengths of every form."""
+    rng = np.random.default_rng(n + vocab)
+    ids = np.arange(n, dtype=np.int64) % vocab if kind == "cycle" else tokens(rng, n, vocab, kind)
+    G = [rnd(rng, n, dim) for _ in range(shares)]
+    got = gpu.ring_embed_grad(G[0].ravel(), G[1].ravel() if shares == 2 else None, ids, vocab, dim, -7, 0)
+    ok = (ids >= 0) & (ids < vocab)
+    for k, g in enumerate([got] if shares == 1 else got):
+        want = np.zeros((vocab, dim), np.uint64)
+        np.add.at(want, ids[ok], ref.words(G[k])[ok])
+        assert np.array_equal(ref.words(g).reshape(vocab, dim), want * np.uint64(2 ** 64 - 7)), k
+
+
 @pytest.mark.parametrize("shares", [1, 2])
 @pytest.mark.parametrize("vocab,dim,n", [(300, 130, 2000), (5, 1, 4000), (9000, 33, 40), (20, 8, 0)])
 def test_embed_grad_accumulates(gpu, shares, vocab, dim, n):
