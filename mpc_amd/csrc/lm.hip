@@ -184,7 +184,11 @@ template <bool TWO, u32 WAVES> __device__ inline void join_waves(RowAcc<TWO, 1> 
 
 // Few tokens: one launch.  A workgroup owns GRAD_ROWS rows of the table, 128 columns of them: it looks through all ids,
 // sorts its own tokens by row in LDS, and adds them -- a row of few tokens by one wavefront, a row of many by all four.
-constexpr u32 GRAD_ROWS = 8, GRAD_SMALL_N = 4096, GRAD_ALONE = 8;
+// Taken up to GRAD_SMALL_N tokens (1000 rows of 256: 2048 tokens 14 us against 18 of the other form, 4096: 29 against 22) and
+// up to GRAD_SMALL_SCAN ids read by all workgroups together (8000 rows of 512: 1024 tokens 21 us against 27, 2000: 30
+// against 30).
+constexpr u32 GRAD_ROWS = 8, GRAD_SMALL_N = 2048, GRAD_ALONE = 8;
+constexpr u64 GRAD_SMALL_SCAN = 1 << 23;
 template <bool TWO> __global__ __launch_bounds__(256) void embed_grad_small_kernel(GradArgs A) {
     __shared__ u16 list[GRAD_SMALL_N];
     __shared__ u32 cnt[GRAD_ROWS], off[GRAD_ROWS + 1];
@@ -261,9 +265,11 @@ struct GradChunk {
     }
 };
 // The whole sort in one launch: a workgroup owns `rows` rows of the table and looks through all ids twice, counting its
-// tokens in LDS (and those of the rows before, which gives its first place), then placing them.  65536 tokens: 10 us;
-// a histogram in memory takes four launches and 30 us, and less from about GRAD_SCAN_N tokens on.
+// tokens in LDS (and those of the rows before, which gives its first place), then placing them.  Up to GRAD_SCAN_N tokens:
+// with 1000 rows of 256, 32768 tokens take 55 us in all against 74 with the histogram in memory below (four launches),
+// 65536 take 76 against 71.
 constexpr u32 GRAD_SCAN_ROWS = 4096, GRAD_SCAN_THREADS = 1024;
+constexpr u64 GRAD_SCAN_N = 32768;
 __global__ __launch_bounds__(1024) void grad_scan_kernel(const i64 *__restrict__ ids, u32 n, u64 vocab, u32 rows, GradWork W) {
     __shared__ u32 cnt[GRAD_SCAN_ROWS], ws[16], wb[16];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -1095,17 +1101,6 @@ template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, const LogprobA
     return 0;
 }
 
-// Ids that the one-launch form reads, up to which it is taken: n ids for each of its workgroups
-#ifndef LM_SS
-#define LM_SS (1 << 22)
-#endif
-#ifndef LM_HB
-#define LM_HB 1024
-#endif
-#ifndef LM_SN
-#define LM_SN (1 << 15)
-#endif
-constexpr u64 GRAD_SMALL_SCAN = LM_SS, GRAD_SCAN_N = LM_SN;
 // scratch memory of the many-token form, in 8-byte words from its start
 struct GradLayout {
     u64 total, count, start, rank, order, ends, partial, words, rows, n;
@@ -1139,7 +1134,7 @@ template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *s
     const u32 n = (u32)A.n;
     u32 lg = 3; // lanes of a row: up to a wavefront
     while (lg < 6 && (2ull << lg) < A.dim) lg++;
-    const u64 heavy_blocks = n <= GRAD_CHUNK ? 0 : A.n > A.vocab ? LM_HB : 512; // otherwise no row is heavy
+    const u64 heavy_blocks = n <= GRAD_CHUNK ? 0 : A.n > A.vocab ? 1024 : 512; // otherwise no row is heavy
     const u64 blocks = ceil_div(A.vocab * slices, 256u >> lg) + heavy_blocks, chunks = ceil_div(n, GRAD_CHUNK);
     MPCX_REQUIRE(blocks < (1ull << 31) && chunks * slices < (1ull << 31), "mpcx_ring_embed_grad: sizes too large for one launch");
     if (L.scan()) {
