@@ -108,7 +108,7 @@ template <bool TWO, u32 NS> struct RowAcc {
             }
         }
     }
-    // adds the rows row(i) of p0 / p1, i = i0, i0 + step, .. below i1, NT at a time
+    // adds the rows row(i) of p0 / p1, i = i0, i0 + step, .. below i1, NT at a time, what is left NT / 2 at a time and so on
     template <u32 NT, class F>
     __device__ void add_rows(F row, const u64 *p0, const u64 *p1, u32 i0, u32 i1, u32 step, u64 c0, u64 cs, u64 dim) {
         u32 i = i0;
@@ -141,6 +141,7 @@ template <bool TWO, u32 NS> struct RowAcc {
                     if (TWO) b[u] += y[u * NT + q];
                 }
         }
+        if (NT > 1) return add_rows<(NT > 1 ? NT / 2 : 1)>(row, p0, p1, i, i1, step, c0, cs, dim);
         for (; i < i1; i += step) {
             const u64 at = row(i);
             add(p0 + at, TWO ? p1 + at : nullptr, c0, cs, dim);
@@ -191,33 +192,35 @@ constexpr u32 GRAD_ROWS = 8, GRAD_SMALL_N = 2048, GRAD_ALONE = 8;
 constexpr u64 GRAD_SMALL_SCAN = 1 << 23;
 template <bool TWO> __global__ __launch_bounds__(256) void embed_grad_small_kernel(GradArgs A) {
     __shared__ u16 list[GRAD_SMALL_N];
-    __shared__ u32 cnt[GRAD_ROWS], off[GRAD_ROWS + 1];
+    __shared__ u32 cnt[GRAD_ROWS + 1], off[GRAD_ROWS + 1];
     __shared__ u64x2 lds[3 * (TWO ? 2 : 1) * 64];
     const u32 tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = (u32)A.n;
     const u64 v0 = (u64)blockIdx.x * GRAD_ROWS;
     const u32 rows = (u32)(A.vocab - v0 < GRAD_ROWS ? A.vocab - v0 : GRAD_ROWS);
-    if (tid < GRAD_ROWS) cnt[tid] = 0;
-    __syncthreads();
-    for (u32 t = tid; t < n; t += 256) {
-        const u64 r = (u64)A.ids[t] - v0;
-        if (r < rows) atomicAdd(&cnt[r], 1u);
+    constexpr u32 PER = GRAD_SMALL_N / 256;
+    u32 mine[PER]; // rows of this workgroup that the thread's tokens belong to
+#pragma unroll
+    for (u32 q = 0; q < PER; q++) {
+        const u32 t = 256 * q + tid;
+        const u64 r = t < n ? (u64)A.ids[t] - v0 : GRAD_ROWS;
+        mine[q] = r < rows ? (u32)r : GRAD_ROWS;
     }
+    if (tid <= GRAD_ROWS) cnt[tid] = 0;
     __syncthreads();
-    if (tid == 0) {
+#pragma unroll
+    for (u32 q = 0; q < PER; q++)
+        if (mine[q] < GRAD_ROWS) mine[q] |= atomicAdd(&cnt[mine[q]], 1u) << 8; // its place among the row's
+    __syncthreads();
+    if (tid <= GRAD_ROWS) {
         u32 s = 0;
-        for (u32 r = 0; r < GRAD_ROWS; r++) {
-            off[r] = s;
-            s += cnt[r];
-            cnt[r] = off[r];
-        }
-        off[GRAD_ROWS] = s;
+#pragma unroll
+        for (u32 r = 0; r < GRAD_ROWS; r++) s += r < tid ? cnt[r] : 0;
+        off[tid] = s;
     }
     __syncthreads();
-    if (off[GRAD_ROWS])
-        for (u32 t = tid; t < n; t += 256) {
-            const u64 r = (u64)A.ids[t] - v0;
-            if (r < rows) list[atomicAdd(&cnt[r], 1u)] = (u16)t;
-        }
+#pragma unroll
+    for (u32 q = 0; q < PER; q++)
+        if (mine[q] != GRAD_ROWS) list[off[mine[q] & 255] + (mine[q] >> 8)] = (u16)(256 * q + tid);
     __syncthreads();
     const u64 c0 = (u64)blockIdx.y * 128 + 2 * lane;
     auto row = [&](u32 i) { return (u64)list[i] * A.dim; };

@@ -1,5 +1,6 @@
 """ctypes binding of libmpcx.so (the C ABI in include/mpcx.h).  Device memory is either owned by a
 :class:`DeviceArray` (mpcx_malloc) or borrowed from a torch tensor via its ``data_ptr()``."""
+import array
 import ctypes
 import os
 
@@ -103,9 +104,13 @@ def _word(x, keep):
     if isinstance(x, DeviceArray):
         return x.ptr
     if isinstance(x, (list, tuple)):  # a host array: of device addresses (arrays, tensors) or of counts
-        arr = (ctypes.c_uint64 * max(len(x), 1))(*[e if type(e) is int else _word(e, keep) for e in x])
-        keep.append(arr)
-        return ctypes.addressof(arr)
+        try:
+            words = [e.data_ptr() for e in x]
+        except AttributeError:
+            words = [(e if type(e) is int else _word(e, keep)) & 0xFFFFFFFFFFFFFFFF for e in x]
+        host = array.array("Q", words or [0])
+        keep.append(host)
+        return host.buffer_info()[0]
     raise TypeError(f"cannot pass {t} to the C ABI")
 
 
