@@ -845,3 +845,123 @@ void ABY3Engine::relu(const VecPair &Xj, VecPair &Rj) {
     for (size_t i = 0; i < (size_t)rd.size(); i++) assert(rd[i] == (xd[i] < 0 ? 0 : xd[i]));
 #endif
 }
+
+// ---- language models on shares
+namespace {
+// a matrix's words on the device in row-major order, and back
+struct RowMajor {
+    Dev<int64_t> d;
+    size_t rows, cols;
+    RowMajor(mpcx_ctx *ctx, size_t r, size_t c) : d(ctx, r * c), rows(r), cols(c) {}
+    RowMajor(mpcx_ctx *ctx, const MatrixXl &m) : RowMajor(ctx, m.rows(), m.cols()) {
+        if (!d.n) return;
+        Dev<int64_t> col(ctx, m.data(), d.n);
+        GPU_OK(ctx, mpcx_relayout(ctx, col, d, rows, cols, 1, 0));
+    }
+    void down(MatrixXl &m) {
+        m.resize(rows, cols);
+        if (!d.n) return;
+        Dev<int64_t> col(d.ctx, d.n);
+        GPU_OK(d.ctx, mpcx_relayout(d.ctx, d, col, rows, cols, 0, 1));
+        col.down(m.data(), d.n);
+    }
+};
+} // namespace
+
+void ABY3Engine::embed(const MatPair &table, const vector<int64_t> &ids, int64_t scale, MatPair &rows) {
+    const size_t vocab = table[0].rows(), dim = table[0].cols(), n = ids.size();
+    assert((size_t)table[1].rows() == vocab && (size_t)table[1].cols() == dim);
+    RowMajor t0(gpu, table[0]), t1(gpu, table[1]), e0(gpu, n, dim), e1(gpu, n, dim);
+    Dev<int64_t> id(gpu, ids.data(), n);
+    GPU_OK(gpu, mpcx_ring_embed(gpu, t0.d, t1.d, vocab, dim, id, n, scale, 0, e0.d, e1.d));
+    e0.down(rows[0]);
+    e1.down(rows[1]);
+}
+
+void ABY3Engine::embed_grad(const MatPair &rows_grad, const vector<int64_t> &ids, size_t vocab, int64_t scale, MatPair &table_grad) {
+    const size_t n = ids.size(), dim = rows_grad[0].cols();
+    assert((size_t)rows_grad[0].rows() == n && (size_t)rows_grad[1].rows() == n && (size_t)rows_grad[1].cols() == dim);
+    RowMajor g0(gpu, rows_grad[0]), g1(gpu, rows_grad[1]), t0(gpu, vocab, dim), t1(gpu, vocab, dim);
+    Dev<int64_t> id(gpu, ids.data(), n);
+    Dev<uint8_t> scratch(gpu, mpcx_ring_embed_grad_scratch(n, vocab, dim));
+    GPU_OK(gpu, mpcx_ring_embed_grad(gpu, g0.d, g1.d, id, n, vocab, dim, scale, 0, 0, scratch.p, t0.d, t1.d));
+    t0.down(table_grad[0]);
+    t1.down(table_grad[1]);
+}
+
+void ABY3Engine::clip_norm(const vector<VecPair> &X, uint64_t max_norm, size_t number, vector<VecPair> &Y, int64_t *factor) {
+    const Peers pe(party_id);
+    vector<std::unique_ptr<Dev<int64_t>>> own;
+    vector<const int64_t *> x0, x1;
+    vector<uint64_t> lens;
+    size_t total = 0;
+    for (const VecPair &t : X) {
+        const size_t n = t[0].size();
+        assert((size_t)t[1].size() == n);
+        for (int k = 0; k < 2; k++) {
+            own.emplace_back(new Dev<int64_t>(gpu, t[k].data(), n));
+            (k ? x1 : x0).push_back(own.back()->p);
+        }
+        lens.push_back(n);
+        total += n;
+    }
+    // round 1: the squared norm is opened
+    Dev<int64_t> zp(gpu, 1), z0(gpu, 1), zn(gpu, 1), coef(gpu, 1), y(gpu, total);
+    Dev<uint8_t> scratch(gpu, mpcx_aby3_sqnorm_scratch(X.size()));
+    GPU_OK(gpu, mpcx_aby3_sqnorm_local(gpu, x0.data(), x1.data(), lens.data(), X.size(), prgs[pe.next].init_seed, prgs[pe.next].pops,
+                                       prgs[pe.prev].init_seed, prgs[pe.prev].pops, scratch.p, z0));
+    prgs[pe.next].advance(gpu, 1);
+    prgs[pe.prev].advance(gpu, 1);
+    z0.to_string(message_send[pe.next]);
+    message_send[pe.prev] = message_send[pe.next];
+    messenger->send_and_recv(message_send, message_recv);
+    MSG_CHECK(message_recv[pe.prev].size() == sizeof(int64_t) && message_recv[pe.next].size() == sizeof(int64_t));
+    upload_string(zp, message_recv[pe.prev]);
+    upload_string(zn, message_recv[pe.next]);
+    // round 2: trunc's, of the scaled tensors
+    const size_t k = party_id == 1 ? 2 : 1; // parties 1 and 2 draw from the stream they share
+    GPU_OK(gpu, mpcx_aby3_clip_local(gpu, (int)party_id, x0.data(), x1.data(), lens.data(), X.size(), zp, z0, zn, max_norm,
+                                     (int)number, prgs[k].init_seed, prgs[k].pops, y, coef));
+    if (party_id != 0) prgs[k].advance(gpu, total);
+    message_send[pe.next].clear();
+    y.to_string(message_send[pe.prev]);
+    messenger->send_and_recv(message_send, message_recv);
+    MSG_CHECK(message_recv[pe.next].size() == total * sizeof(int64_t));
+    Y.resize(X.size());
+    size_t at = 0;
+    for (size_t i = 0; i < lens.size(); i++) {
+        const size_t bytes = lens[i] * sizeof(int64_t);
+        for (int q = 0; q < 2; q++) {
+            Y[i][q].resize(lens[i]);
+            copy_bytes(Y[i][q].data(), (q ? message_recv[pe.next] : message_send[pe.prev]).data() + at, bytes);
+        }
+        at += bytes;
+    }
+    if (factor) coef.down(factor, 1);
+}
+
+void ABY3Engine::reveal_logprobs(const MatPair &logits, size_t number, const vector<int64_t> &ids, size_t top, LogProbs &out) {
+    const size_t rows = logits[0].rows(), cols = logits[0].cols(), n = rows * cols;
+    assert((size_t)logits[1].rows() == rows && (size_t)logits[1].cols() == cols && ids.size() == rows);
+    const Peers pe(party_id);
+    message_send[pe.prev].clear();
+    matrix2string(logits[0], message_send[pe.next]);
+    messenger->send_and_recv(message_send, message_recv);
+    MSG_CHECK(message_recv[pe.prev].size() == n * sizeof(int64_t));
+    Dev<int64_t> a(gpu, n), b(gpu, n), id(gpu, ids.data(), rows), top_ids(gpu, rows * top);
+    upload_string(a, message_recv[pe.prev]);
+    upload_string(b, message_send[pe.next]);
+    RowMajor c(gpu, logits[1]);
+    Dev<float> logp(gpu, rows), entropy(gpu, rows), top_logp(gpu, rows * top);
+    Dev<uint8_t> scratch(gpu, mpcx_reveal_logprobs_scratch(rows, cols, top));
+    GPU_OK(gpu, mpcx_reveal_logprobs(gpu, a, b, c.d, rows, cols, (int)number, id, 1, top, scratch.p, logp, entropy, top_ids, top_logp,
+                                     nullptr, nullptr));
+    auto take = [](auto &dev, auto &v) {
+        v.resize(dev.n);
+        if (dev.n) dev.down(v.data(), dev.n);
+    };
+    take(logp, out.logp);
+    take(entropy, out.entropy);
+    take(top_logp, out.top_logp);
+    take(top_ids, out.top_ids);
+}

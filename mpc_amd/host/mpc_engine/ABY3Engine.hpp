@@ -84,6 +84,23 @@ class ABY3Engine {
     // nine rounds, messages and generator words as the three calls, but G, P, the carry tree and the sign bits stay
     // on the device between the rounds (only messages cross to the host).  Bit-identical to the composition.
     void relu(const VecPair &X, VecPair &R);
+    // Language models on shares (weights shared, text public; include/mpcx.h describes the arithmetic).
+    // rows = scale * table[ids] (ids.size() x table.cols(); a zero row for an id outside the table); no round.
+    void embed(const MatPair &table, const vector<int64_t> &ids, int64_t scale, MatPair &rows);
+    // The gradient of that lookup: table_grad (vocab x rows.cols()) = scale * the sums of the rows of equal ids; no round.
+    void embed_grad(const MatPair &rows_grad, const vector<int64_t> &ids, size_t vocab, int64_t scale, MatPair &table_grad);
+    // Y = X clipped to the global norm max_norm of all tensors together (max_norm and X with `number` fractional bits): two
+    // rounds, the opened squared norm (one word to each of the others) and trunc's.  One word popped from each pair stream,
+    // then trunc's words.  factor receives the public factor (`number` fractional bits).  X and Y may be the same.
+    void clip_norm(const vector<VecPair> &X, uint64_t max_norm, size_t number, vector<VecPair> &Y, int64_t *factor = nullptr);
+    // Opens logits (the round of reveal_matrix) with `number` fractional bits and returns, on every party, what a caller
+    // reads of each row: the log probability of ids[row] (0 for an id outside the columns), the entropy, and the `top`
+    // likeliest columns with their log probabilities (rows x top, best first, ties by the lower column).
+    struct LogProbs {
+        vector<float> logp, entropy, top_logp;
+        vector<int64_t> top_ids;
+    };
+    void reveal_logprobs(const MatPair &logits, size_t number, const vector<int64_t> &ids, size_t top, LogProbs &out);
     // Keeps a device copy of a share pair (e.g. a weight matrix that many products use) until unpin: matrix_mul finds
     // an operand by the address of its pair and skips the upload.  Explicit on purpose: the caller promises not to
     // change or destroy a pinned pair.  The destructor releases what is still pinned.  With MPCX_DEVICES every GPU of

@@ -3,6 +3,7 @@
 // (test/test_ABY3.cpp, test/test_securenn.cpp: reveal(op(share(x))) == op(x)), and share checksums are
 // printed as "KAT <name> <party> <hex>" lines so that a harness can compare them with known answers.
 // Exit code 0 = every check passed.
+#include <math.h>
 #include <stdio.h>
 #include <stdlib.h>
 #include <atomic>
@@ -550,6 +551,76 @@ static void empty_inputs_party(InProcHub *hub, size_t p) {
     }
 }
 
+// language models on shares: lookup, its gradient, clipping and opened log probabilities against plain loops
+static void aby3_language_party(InProcHub *hub, size_t p) {
+    InProcMessenger msgr(hub, p);
+    ABY3Engine e(&msgr, p);
+    PRgenerator g(77, 0);
+    const size_t vocab = 37, dim = 19, rows = 23;
+    MatrixXl T(vocab, dim), E, D;
+    for (size_t i = 0; i < vocab; i++)
+        for (size_t j = 0; j < dim; j++) T(i, j) = g.pop_int64();
+    vector<int64_t> ids(rows);
+    for (size_t i = 0; i < rows; i++) ids[i] = (int64_t)((uint64_t)g.pop_int64() % (vocab / 3));
+    ids[4] = -1, ids[5] = (int64_t)vocab, ids[6] = ids[7];
+    array<MatrixXl, 2> Tj, Ej, Dj;
+    e.share_matrix(T, Tj);
+    e.embed(Tj, ids, -5, Ej);
+    e.reveal_matrix(Ej, E);
+    for (size_t i = 0; i < rows; i++)
+        for (size_t j = 0; j < dim; j++) CHECK(E(i, j) == (ids[i] >= 0 && ids[i] < (int64_t)vocab ? (int64_t)((uint64_t)T(ids[i], j) * (uint64_t)-5) : 0));
+    e.embed_grad(Ej, ids, vocab, 3, Dj);
+    e.reveal_matrix(Dj, D);
+    for (size_t v = 0; v < vocab; v++)
+        for (size_t j = 0; j < dim; j++) {
+            uint64_t s = 0;
+            for (size_t i = 0; i < rows; i++)
+                if (ids[i] == (int64_t)v) s += (uint64_t)E(i, j);
+            CHECK((uint64_t)D(v, j) == 3 * s);
+        }
+    // tensors of norm 5 (3, 4 and zeros, 16 fractional bits), clipped to 1; then to 10, which leaves them
+    vector<array<VecI64, 2>> Xs(3), Ys;
+    vector<VecI64> plain;
+    for (size_t n : {(size_t)5, (size_t)0, (size_t)300}) {
+        VecI64 v(n);
+        for (size_t i = 0; i < n; i++) v[i] = 0;
+        plain.push_back(v);
+    }
+    plain[0][1] = 3 << 16, plain[2][299] = -(4 << 16);
+    for (size_t i = 0; i < 3; i++) e.share(plain[i], Xs[i]);
+    for (int64_t bound : {1, 10}) {
+        int64_t factor = -1;
+        e.clip_norm(Xs, (uint64_t)bound << 16, 16, Ys, &factor);
+        CHECK(factor == (bound == 1 ? (1 << 16) / 5 : 1 << 16));
+        for (size_t i = 0; i < 3; i++) {
+            VecI64 y;
+            e.reveal(Ys[i], y);
+            CHECK(y.size() == plain[i].size());
+            for (size_t k = 0; k < (size_t)y.size(); k++) CHECK(llabs(y[k] - ((plain[i][k] * factor) >> 16)) <= 2);
+        }
+    }
+    Ys = Xs; // in place
+    e.clip_norm(Ys, 1 << 16, 16, Ys);
+    VecI64 y;
+    e.reveal(Ys[0], y);
+    CHECK(llabs(y[1] - ((plain[0][1] * ((1 << 16) / 5)) >> 16)) <= 2);
+    // logits: a row with a clear winner, an even row, ties
+    MatrixXl L(3, 6);
+    for (size_t i = 0; i < 3; i++)
+        for (size_t j = 0; j < 6; j++) L(i, j) = i == 2 ? (int64_t)(j & 1) << 16 : 0;
+    L(0, 4) = 50 << 16;
+    array<MatrixXl, 2> Lj;
+    e.share_matrix(L, Lj);
+    ABY3Engine::LogProbs out;
+    e.reveal_logprobs(Lj, 16, {4, 2, 6}, 3, out);
+    CHECK(out.logp.size() == 3 && out.top_ids.size() == 9 && out.top_logp.size() == 9 && out.entropy.size() == 3);
+    CHECK(fabsf(out.logp[0]) < 1e-6f && fabsf(out.logp[1] + logf(6)) < 1e-6f && out.logp[2] == 0);
+    CHECK(fabsf(out.entropy[0]) < 1e-6f && fabsf(out.entropy[1] - logf(6)) < 1e-5f);
+    CHECK(out.top_ids[0] == 4 && out.top_ids[1] == 0 && out.top_ids[2] == 1);
+    for (size_t k = 0; k < 3; k++) CHECK(out.top_ids[3 + k] == (int64_t)k && out.top_ids[6 + k] == (int64_t)(2 * k + 1));
+    CHECK(fabsf(out.top_logp[6] + logf(3 + 3 * expf(-1))) < 1e-6f);
+}
+
 template <class F> static void run3(F party) {
     InProcHub hub;
     std::thread t0(party, &hub, 0), t1(party, &hub, 1), t2(party, &hub, 2);
@@ -590,6 +661,7 @@ int main() {
     run3(aby3_additions_party);
     run3(snn_additions_party);
     run3(empty_inputs_party);
+    run3(aby3_language_party);
     if (failures.load()) {
         printf("host_selftest: %d check(s) FAILED\n", failures.load());
         return 1;
