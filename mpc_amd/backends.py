@@ -15,6 +15,13 @@ def _c(a, dt):
     return np.ascontiguousarray(a, dtype=dt)
 
 
+def _sized(what, n, *arrays):
+    """Refuses arrays whose lengths do not fit the shapes they are passed with (None: not there)."""
+    for a in arrays:
+        if a is not None and a.size != n:
+            raise ValueError(f"{what}: an array of {a.size} elements where the shapes ask for {n}")
+
+
 class GpuBackend:
     """Same surface as OracleBackend, executed by libmpcx.so on cuda:0 (no fallback of any kind)."""
     name = "gpu"
@@ -359,24 +366,36 @@ class GpuBackend:
 
     def ring_embed(self, T0, T1, vocab, dim, ids, scale=1, shift=0):
         n = ids.size
+        _sized("ring_embed", vocab * dim, T0, T1)
         outs = [("out", np.int64, n * dim)] * (1 if T1 is None else 2)
         return self._go("ring_embed", _c(T0, np.int64), _c(T1, np.int64), vocab, dim, _c(ids, np.int64), n, scale, shift, *outs,
                         *([None] if T1 is None else []))
 
     def ring_embed_grad(self, G0, G1, ids, vocab, dim, scale=1, shift=0):
         n = ids.size
+        _sized("ring_embed_grad", n * dim, G0, G1)
         outs = [("out", np.int64, vocab * dim)] * (1 if G1 is None else 2)
         return self._go("ring_embed_grad", _c(G0, np.int64), _c(G1, np.int64), _c(ids, np.int64), n, vocab, dim, scale, shift, 0,
                         self._scratch("ring_embed_grad", n, vocab, dim), *outs, *([None] if G1 is None else []))
 
+    @staticmethod
+    def _same_lengths(what, X0s, X1s):
+        if len(X0s) != len(X1s):
+            raise ValueError(f"{what}: {len(X0s)} first shares and {len(X1s)} second ones")
+        for a, b in zip(X0s, X1s):
+            _sized(what, a.size, b)
+
     def aby3_sqnorm_local(self, X0s, X1s, seed_next, pop_next, seed_prev, pop_prev):
         """X0s, X1s: lists of the tensors' shares."""
+        self._same_lengths("aby3_sqnorm_local", X0s, X1s)
         X0s, X1s = [_c(x, np.int64) for x in X0s], [_c(x, np.int64) for x in X1s]
         return self._go("aby3_sqnorm_local", X0s, X1s, [x.size for x in X0s], len(X0s), seed_next, pop_next, seed_prev, pop_prev,
                         self._scratch("aby3_sqnorm", len(X0s)), ("out", np.int64, 1))
 
     def aby3_clip_local(self, party, X0s, X1s, z_prev, z0, z1, max_norm, number, seed12, pop12):
         """Returns the message (the tensors one after the other) and the factor."""
+        self._same_lengths("aby3_clip_local", X0s, X1s)
+        _sized("aby3_clip_local", 1, z_prev, z0, z1)
         lens = [x.size for x in X0s]
         X0s, X1s = [_c(x, np.int64) for x in X0s], [_c(x, np.int64) for x in X1s]
         return self._go("aby3_clip_local", party, X0s, X1s, lens, len(lens), _c(z_prev, np.int64), _c(z0, np.int64),
@@ -385,6 +404,8 @@ class GpuBackend:
     def reveal_logprobs(self, a, b, c, rows, vocab, frac, ids, top=0):
         """Returns logp, entropy, top_ids, top_logp, row_max, log_sum (flat)."""
         per_row = ids.size // rows if rows else 0
+        _sized("reveal_logprobs", rows * vocab, a, b, c)
+        _sized("reveal_logprobs", rows * per_row, ids)
         return self._go("reveal_logprobs", _c(a, np.int64), _c(b, np.int64), _c(c, np.int64), rows, vocab, frac, _c(ids, np.int64),
                         per_row, top, self._scratch("reveal_logprobs", rows, vocab, top), ("out", np.float32, rows * per_row),
                         ("out", np.float32, rows), ("out", np.int64, rows * top), ("out", np.float32, rows * top),
@@ -393,6 +414,9 @@ class GpuBackend:
     def reveal_logprobs_grad(self, a, b, c, rows, vocab, frac, ids, d_logp, d_entropy, row_max, log_sum, entropy, grad_frac):
         """Returns the gradient as floats and as ring words with grad_frac fractional bits (flat)."""
         per_row = ids.size // rows if rows else 0
+        _sized("reveal_logprobs_grad", rows * vocab, a, b, c)
+        _sized("reveal_logprobs_grad", rows * per_row, ids, d_logp)
+        _sized("reveal_logprobs_grad", rows, d_entropy, row_max, log_sum, entropy)
         return self._go("reveal_logprobs_grad", _c(a, np.int64), _c(b, np.int64), _c(c, np.int64), rows, vocab, frac,
                         _c(ids, np.int64), per_row, _c(d_logp, np.float32), _c(d_entropy, np.float32), _c(row_max, np.int64),
                         _c(log_sum, np.float32), _c(entropy, np.float32), ("out", np.float32, rows * vocab),

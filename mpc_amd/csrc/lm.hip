@@ -6,8 +6,15 @@
 
 namespace {
 
-// a product of sizes that stays below 2^60 words (every byte count then fits 64 bits)
-bool lm_fits(u64 a, u64 b) { return a == 0 || b <= (1ull << 60) / a; }
+// a product of sizes that stays below 2^56 words (every byte count then fits 64 bits)
+bool lm_fits(u64 a, u64 b) { return a == 0 || b <= (1ull << 56) / a; }
+// Workgroups of one launch (a grid holds fewer than 2^32 threads); what is left over is reached by striding, or by
+// another launch.
+constexpr u64 LM_MAX_BLOCKS = 1ull << 22;
+u64 lm_blocks(u64 n) {
+    const u64 cap = LM_MAX_BLOCKS < MPCX_MAX_GRID ? LM_MAX_BLOCKS : MPCX_MAX_GRID;
+    return n < cap ? n : cap;
+}
 
 // two neighbouring words by one 16-byte access; share arrays are 8-byte aligned only, which the hardware takes
 typedef u64 u64x2 __attribute__((ext_vector_type(2)));
@@ -411,50 +418,57 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(GradArgs A, GradWork W, 
         }
         return;
     }
-    const u64 item = ((u64)(blockIdx.x - heavy_blocks) * 256 + threadIdx.x) >> lg;
-    const u64 v = item / slices;
-    if (v >= A.vocab) return;
-    const u32 c = W.count[v];
-    if (c > GRAD_CHUNK || (c == 0 && A.accumulate)) return;
-    const u64 c0 = (item % slices) * 128 + 2 * (threadIdx.x & ((1u << lg) - 1));
-    const u32 *list = W.order + (c ? W.start[v] : 0);
-    acc.template add_rows<GRAD_TOGETHER>([&](u32 i) { return (u64)list[i] * A.dim; }, A.G0, A.G1, 0, c, 1, c0, 0, A.dim);
-    acc.template write<STREAM>(A, v, c0, 0);
+    const u64 step = (u64)(gridDim.x - heavy_blocks) * 256 >> lg;
+    for (u64 item = ((u64)(blockIdx.x - heavy_blocks) * 256 + threadIdx.x) >> lg;; item += step) {
+        const u64 v = item / slices;
+        if (v >= A.vocab) return;
+        const u32 c = W.count[v];
+        if (c > GRAD_CHUNK || (c == 0 && A.accumulate)) continue;
+        const u64 c0 = (item % slices) * 128 + 2 * (threadIdx.x & ((1u << lg) - 1));
+        const u32 *list = W.order + (c ? W.start[v] : 0);
+        acc = RowAcc<TWO, 1>();
+        acc.template add_rows<GRAD_TOGETHER>([&](u32 i) { return (u64)list[i] * A.dim; }, A.G0, A.G1, 0, c, 1, c0, 0, A.dim);
+        acc.template write<STREAM>(A, v, c0, 0);
+    }
 }
 // 128 columns of the heavy rows that begin in eight chunks (one at most does in each): a wavefront looks at one chunk and
 // adds the sums of its row when they are few; those of a longer row are shared out to all wavefronts.
 constexpr u32 HEAVY_WAVES = 8, HEAVY_ALONE = 8;
-template <bool TWO> __global__ __launch_bounds__(64 * HEAVY_WAVES) void grad_heavy_kernel(GradArgs A, GradWork W, u32 slices) {
+template <bool TWO>
+__global__ __launch_bounds__(64 * HEAVY_WAVES) void grad_heavy_kernel(GradArgs A, GradWork W, u32 slices, u64 items) {
     __shared__ u64x2 lds[(HEAVY_WAVES - 1) * (TWO ? 2 : 1) * 64];
     __shared__ u32 begin[HEAVY_WAVES], chunks[HEAVY_WAVES], rows[HEAVY_WAVES]; // the sum of the first chunk, how many, the row
     const u32 total = *W.total, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const u32 k = blockIdx.x / slices * HEAVY_WAVES + wave;
-    const u64 c0 = (u64)(blockIdx.x % slices) * 128 + 2 * lane;
-    u32 n = 0, b = 0, v = 0;
-    if ((u64)k * GRAD_CHUNK < total) {
-        const GradChunk ch(W, A.ids, total, k);
-        const u32 c = W.count[ch.vb], first = W.start[ch.vb];
-        if (c > GRAD_CHUNK && first >= ch.p0) n = (first + c - 1) / GRAD_CHUNK - k + 1;
-        b = 2 * k + (ch.va != ch.vb), v = ch.vb;
-    }
-    // the first chunk's sum is the one of its last row, every other chunk's that of its first row
-    auto add = [&](RowAcc<TWO, 1> &acc, u32 b, u32 i0, u32 n, u32 step) {
-        acc.template add_rows<8>([&](u32 i) { return (u64)(i ? (b & ~1u) + 2 * i : b) * 2 * A.dim; }, W.partial, W.partial + A.dim, i0,
-                                 n, step, c0, 0, A.dim);
-    };
-    if (lane == 0) begin[wave] = b, rows[wave] = v, chunks[wave] = n > HEAVY_ALONE ? n : 0;
-    if (n && n <= HEAVY_ALONE) {
-        RowAcc<TWO, 1> acc;
-        add(acc, b, 0, n, 1);
-        acc.template write<false>(A, v, c0, 0);
-    }
-    __syncthreads();
-    for (u32 q = 0; q < HEAVY_WAVES; q++) {
-        if (chunks[q] == 0) continue;
-        RowAcc<TWO, 1> acc;
-        add(acc, begin[q], wave, chunks[q], HEAVY_WAVES);
-        join_waves<TWO, HEAVY_WAVES>(acc, lds);
-        if (wave == 0) acc.template write<false>(A, rows[q], c0, 0);
+    for (u64 it = blockIdx.x; it < items; it += gridDim.x) { // items = slices for every HEAVY_WAVES chunks
+        const u32 k = (u32)(it / slices) * HEAVY_WAVES + wave;
+        const u64 c0 = (it % slices) * 128 + 2 * lane;
+        u32 n = 0, b = 0, v = 0;
+        if ((u64)k * GRAD_CHUNK < total) {
+            const GradChunk ch(W, A.ids, total, k);
+            const u32 c = W.count[ch.vb], first = W.start[ch.vb];
+            if (c > GRAD_CHUNK && first >= ch.p0) n = (first + c - 1) / GRAD_CHUNK - k + 1;
+            b = 2 * k + (ch.va != ch.vb), v = ch.vb;
+        }
+        // the first chunk's sum is the one of its last row, every other chunk's that of its first row
+        auto add = [&](RowAcc<TWO, 1> &acc, u32 b, u32 i0, u32 n, u32 step) {
+            acc.template add_rows<8>([&](u32 i) { return (u64)(i ? (b & ~1u) + 2 * i : b) * 2 * A.dim; }, W.partial,
+                                     W.partial + A.dim, i0, n, step, c0, 0, A.dim);
+        };
+        __syncthreads(); // the lists of the item before have been read
+        if (lane == 0) begin[wave] = b, rows[wave] = v, chunks[wave] = n > HEAVY_ALONE ? n : 0;
+        if (n && n <= HEAVY_ALONE) {
+            RowAcc<TWO, 1> acc;
+            add(acc, b, 0, n, 1);
+            acc.template write<false>(A, v, c0, 0);
+        }
+        __syncthreads();
+        for (u32 q = 0; q < HEAVY_WAVES; q++) {
+            if (chunks[q] == 0) continue;
+            RowAcc<TWO, 1> acc;
+            add(acc, begin[q], wave, chunks[q], HEAVY_WAVES);
+            join_waves<TWO, HEAVY_WAVES>(acc, lds);
+            if (wave == 0) acc.template write<false>(A, rows[q], c0, 0);
+        }
     }
 }
 
@@ -593,6 +607,7 @@ __global__ void clip_factor_kernel(ClipArgs A, i64 *coef) { *coef = (i64)A.facto
 // words, exact before their one conversion to a float.
 template <int SH> struct LogitIn {
     const u64 *a, *b, *c;
+    void skip(u64 n) { a += n, b = b ? b + n : b, c = c ? c + n : c; }
     __device__ i64 at(u64 i) const {
         u64 x = a[i];
         if (SH > 1) x += b[i];
@@ -869,11 +884,13 @@ template <u32 W, bool SPLIT, int SH> __global__ __launch_bounds__(256) void logp
             idx[k] = (u32)(tile + 128 * (k / 2) + 2 * lane + (k & 1));
         }
         if (m > s.m) s.move_to(m, A.unit2);
+        float S = 0, T = 0; // of the tile: a lane's sums take one step of rounding a tile, not one a word
 #pragma unroll
         for (u32 k = 0; k < N; k++) {
             const float d = word_dist(s.m, x[k]) * A.unit2, e = valid[k] ? exp2_fast(-d) : 0.0f;
-            s.S += e, s.T = fmaf(d, e, s.T);
+            S += e, T = fmaf(d, e, T);
         }
+        s.S += S, s.T += T;
         if (A.top) {
             if (first && j1 - tile > 64) {
                 top_first<N>(top, x, idx, valid, m, 16.0f / A.unit);
@@ -926,7 +943,6 @@ constexpr u32 JOIN_THREADS = 512; // 256 / 512 / 1024: 9.4 / 8.2 / 8.1 us for on
 // parts each) for itself; its entries within the border go to LDS, and after the one barrier the first wavefront sorts
 // them.
 template <int SH> __global__ __launch_bounds__(JOIN_THREADS) void logprobs_join_kernel(LogitIn<SH> in, LogprobArgs A) {
-    constexpr u32 JOIN_THREADS = 512; // 256 / 512 / 1024: 9.4 / 8.2 / 8.1 us for one row of 131072 with 20 alternatives
     constexpr u32 K = 4, THREADS = JOIN_THREADS, E = 8192 / THREADS;
     __shared__ TopEntry buf[64];
     __shared__ u32 count;
@@ -1074,7 +1090,9 @@ template <int SH, bool STREAM> __global__ __launch_bounds__(256) void logprobs_g
         else put1(base + j, part((u64)in.at(base + j)));
     }
     if (A.per_row == 0) return;
-    __syncthreads(); // the stores above are done: a word of an id is written by another lane now
+    // a word of an id is written by another lane now: the stores above have to be done
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
     for (u64 t = tid; t < A.per_row; t += 256) {
         const u64 id = (u64)ids[t];
         if (id < j0 || id >= j1) continue;
@@ -1089,17 +1107,25 @@ template <int SH, bool STREAM> __global__ __launch_bounds__(256) void logprobs_g
 constexpr u64 LP_GROUPS = 1024; // workgroups that fill the chip: four on each CU
 constexpr u64 LP_CHUNK = 2048;  // words: one tile for each of four wavefronts
 constexpr u64 LP_WAVE_ROW = 1024; // rows up to this length are read by one wavefront each
-template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, const LogprobArgs &A) {
-    if (A.splits > 1)
-        hipLaunchKernelGGL((logprobs_kernel<4, true, SH>), dim3((u32)(A.rows * A.splits)), dim3(256), 0, ctx->stream, in, A);
-    else if (A.vocab <= LP_WAVE_ROW)
-        hipLaunchKernelGGL((logprobs_kernel<1, false, SH>), dim3((u32)ceil_div(A.rows, 4)), dim3(256), 0, ctx->stream, in, A);
-    else
-        hipLaunchKernelGGL((logprobs_kernel<4, false, SH>), dim3((u32)A.rows), dim3(256), 0, ctx->stream, in, A);
-    MPCX_LAUNCH_CHECK();
-    if (A.splits > 1) {
-        hipLaunchKernelGGL(logprobs_join_kernel<SH>, dim3((u32)A.rows), dim3(JOIN_THREADS), 0, ctx->stream, in, A);
+template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, LogprobArgs A) {
+    const u64 all = A.rows;
+    for (u64 r0 = 0; r0 < all; r0 += LM_MAX_BLOCKS) { // rows of one launch; more than one launch: nothing is split
+        A.rows = all - r0 < LM_MAX_BLOCKS ? all - r0 : LM_MAX_BLOCKS;
+        if (A.splits > 1)
+            hipLaunchKernelGGL((logprobs_kernel<4, true, SH>), dim3((u32)(A.rows * A.splits)), dim3(256), 0, ctx->stream, in, A);
+        else if (A.vocab <= LP_WAVE_ROW)
+            hipLaunchKernelGGL((logprobs_kernel<1, false, SH>), dim3((u32)ceil_div(A.rows, 4)), dim3(256), 0, ctx->stream, in, A);
+        else
+            hipLaunchKernelGGL((logprobs_kernel<4, false, SH>), dim3((u32)A.rows), dim3(256), 0, ctx->stream, in, A);
         MPCX_LAUNCH_CHECK();
+        if (A.splits > 1) {
+            hipLaunchKernelGGL(logprobs_join_kernel<SH>, dim3((u32)A.rows), dim3(JOIN_THREADS), 0, ctx->stream, in, A);
+            MPCX_LAUNCH_CHECK();
+        }
+        in.skip(A.rows * A.vocab);
+        auto skip = [&](auto *&p, u64 n) { p = p ? p + n : p; };
+        skip(A.ids, A.rows * A.per_row), skip(A.logp, A.rows * A.per_row), skip(A.entropy, A.rows), skip(A.row_max, A.rows);
+        skip(A.log_sum, A.rows), skip(A.top_ids, A.rows * A.top), skip(A.top_logp, A.rows * A.top);
     }
     return 0;
 }
@@ -1124,7 +1150,7 @@ struct GradLayout {
 template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *scratch) {
     const u64 slices = ceil_div(A.dim, 128);
     const u64 small_blocks = ceil_div(A.vocab, GRAD_ROWS) * slices;
-    if (A.n <= GRAD_SMALL_N && A.n * small_blocks <= GRAD_SMALL_SCAN && slices < 65536) {
+    if (A.n <= GRAD_SMALL_N && (A.n ? A.n : 1) * small_blocks <= GRAD_SMALL_SCAN && slices < 65536) {
         hipLaunchKernelGGL(embed_grad_small_kernel<TWO>, dim3((u32)ceil_div(A.vocab, GRAD_ROWS), (u32)slices), dim3(256), 0,
                            ctx->stream, A);
         MPCX_LAUNCH_CHECK();
@@ -1138,8 +1164,9 @@ template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *s
     u32 lg = 3; // lanes of a row: up to a wavefront
     while (lg < 6 && (2ull << lg) < A.dim) lg++;
     const u64 heavy_blocks = n <= GRAD_CHUNK ? 0 : A.n > A.vocab ? 1024 : 512; // otherwise no row is heavy
-    const u64 blocks = ceil_div(A.vocab * slices, 256u >> lg) + heavy_blocks, chunks = ceil_div(n, GRAD_CHUNK);
-    MPCX_REQUIRE(blocks < (1ull << 31) && chunks * slices < (1ull << 31), "mpcx_ring_embed_grad: sizes too large for one launch");
+    const u64 blocks = lm_blocks(ceil_div(A.vocab * slices, 256u >> lg)) + heavy_blocks;
+    const u64 heavy_items = ceil_div(ceil_div(n, GRAD_CHUNK), HEAVY_WAVES) * slices;
+    MPCX_REQUIRE(slices < (1ull << 32), "mpcx_ring_embed_grad: rows of %llu words", (unsigned long long)A.dim);
     if (L.scan()) {
         hipLaunchKernelGGL(grad_scan_kernel, dim3((u32)ceil_div(A.vocab, L.rows)), dim3(GRAD_SCAN_THREADS), 0, ctx->stream, A.ids, n,
                            A.vocab, (u32)L.rows, W);
@@ -1154,7 +1181,8 @@ template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *s
     hipLaunchKernelGGL((stream ? grad_rows_kernel<TWO, true> : grad_rows_kernel<TWO, false>), dim3((u32)blocks), dim3(256), 0,
                        ctx->stream, A, W, (u32)heavy_blocks, lg, (u32)slices);
     if (heavy_blocks)
-        hipLaunchKernelGGL(grad_heavy_kernel<TWO>, dim3((u32)(ceil_div(chunks, HEAVY_WAVES) * slices)), dim3(64 * HEAVY_WAVES), 0, ctx->stream, A, W, (u32)slices);
+        hipLaunchKernelGGL(grad_heavy_kernel<TWO>, dim3((u32)lm_blocks(heavy_items)), dim3(64 * HEAVY_WAVES), 0, ctx->stream, A, W,
+                           (u32)slices, heavy_items);
     MPCX_LAUNCH_CHECK();
     return 0;
 }
@@ -1175,9 +1203,7 @@ int mpcx_ring_embed(mpcx_ctx *ctx, const int64_t *T0, const int64_t *T1, uint64_
     const u32 lg = lanes_log2(dim);
     const u64 slices = ceil_div(dim, 2 * EMB_STEPS << lg);
     MPCX_REQUIRE(slices < 65536, "mpcx_ring_embed: rows of %llu words", (unsigned long long)dim);
-    u64 blocks = ceil_div(n, 256u >> lg);
-    if (blocks > MPCX_MAX_GRID) blocks = MPCX_MAX_GRID;
-    const dim3 grid((u32)blocks, (u32)slices), block(256);
+    const dim3 grid((u32)lm_blocks(ceil_div(n, 256u >> lg)), (u32)slices), block(256);
     const bool stream = n * dim * (T1 ? 32 : 16) > STREAM_BYTES;
     const auto kernel = T1 ? (stream ? embed_kernel<true, true> : embed_kernel<true, false>)
                            : (stream ? embed_kernel<false, true> : embed_kernel<false, false>);
@@ -1307,7 +1333,7 @@ int mpcx_reveal_logprobs(mpcx_ctx *ctx, const int64_t *a, const int64_t *b, cons
                          int frac, const int64_t *ids, uint64_t per_row, uint64_t top, void *scratch, float *logp,
                          float *entropy, int64_t *top_ids, float *top_logp, int64_t *row_max, float *log_sum) {
     MPCX_REQUIRE(vocab >= 1 && vocab < (1ull << 31), "mpcx_reveal_logprobs: vocabulary of %llu", (unsigned long long)vocab);
-    MPCX_REQUIRE(rows < (1ull << 31) && lm_fits(rows, per_row), "mpcx_reveal_logprobs: sizes too large");
+    MPCX_REQUIRE(lm_fits(rows, vocab) && lm_fits(rows, per_row), "mpcx_reveal_logprobs: sizes too large");
     MPCX_REQUIRE(frac >= 0 && frac <= 62, "mpcx_reveal_logprobs: %d fractional bits", frac);
     MPCX_REQUIRE(top <= 32 && top <= vocab, "mpcx_reveal_logprobs: %llu alternatives", (unsigned long long)top);
     MPCX_REQUIRE(b || !c, "mpcx_reveal_logprobs: the third share without the second");
@@ -1331,7 +1357,7 @@ int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b,
                               const float *d_entropy, const int64_t *row_max, const float *log_sum, const float *entropy,
                               float *grad, int64_t *grad_words, int grad_frac) {
     MPCX_REQUIRE(vocab >= 1 && vocab < (1ull << 31), "mpcx_reveal_logprobs_grad: vocabulary of %llu", (unsigned long long)vocab);
-    MPCX_REQUIRE(rows < (1ull << 31) && lm_fits(rows, per_row), "mpcx_reveal_logprobs_grad: sizes too large");
+    MPCX_REQUIRE(lm_fits(rows, vocab) && lm_fits(rows, per_row), "mpcx_reveal_logprobs_grad: sizes too large");
     MPCX_REQUIRE(frac >= 0 && frac <= 62, "mpcx_reveal_logprobs_grad: %d fractional bits", frac);
     MPCX_REQUIRE(!grad_words || (grad_frac >= 0 && grad_frac <= 62), "mpcx_reveal_logprobs_grad: %d fractional bits", grad_frac);
     MPCX_REQUIRE(b || !c, "mpcx_reveal_logprobs_grad: the third share without the second");
@@ -1346,8 +1372,15 @@ int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b,
     A.row_max = row_max, A.log_sum = log_sum, A.entropy = entropy, A.grad = grad, A.grad_words = grad_words;
     const bool stream = rows * vocab * ((c ? 24 : b ? 16 : 8) + (grad ? 4 : 0) + (grad_words ? 8 : 0)) > STREAM_BYTES;
     auto run = [&](auto kernel, auto in) -> int {
-        hipLaunchKernelGGL(kernel, dim3((u32)(rows * A.splits)), dim3(256), 0, ctx->stream, in, A);
-        MPCX_LAUNCH_CHECK();
+        for (u64 r0 = 0; r0 < rows; r0 += LM_MAX_BLOCKS) { // rows of one launch; more than one launch: nothing is split
+            const u64 now = rows - r0 < LM_MAX_BLOCKS ? rows - r0 : LM_MAX_BLOCKS;
+            hipLaunchKernelGGL(kernel, dim3((u32)(now * A.splits)), dim3(256), 0, ctx->stream, in, A);
+            MPCX_LAUNCH_CHECK();
+            in.skip(now * vocab);
+            auto skip = [&](auto *&p, u64 n) { p = p ? p + n : p; };
+            skip(A.ids, now * per_row), skip(A.d_logp, now * per_row), skip(A.d_entropy, now), skip(A.row_max, now);
+            skip(A.log_sum, now), skip(A.entropy, now), skip(A.grad, now * vocab), skip(A.grad_words, now * vocab);
+        }
         return 0;
     };
     const u64 *pa = (const u64 *)a, *pb = (const u64 *)b, *pc = (const u64 *)c;

@@ -87,7 +87,7 @@ class DeviceArray:
             pass
 
 
-def _word(x, keep):
+def _word(x, device, keep):
     """One argument of the C ABI as the 64-bit word that carries it: an address, a size, or an int (whose callee reads the
     low half).  `keep` holds what must outlive the call."""
     t = type(x)
@@ -97,7 +97,9 @@ def _word(x, keep):
         return 0
     if t is DeviceArray:
         return x.ptr
-    if hasattr(x, "data_ptr"):  # torch tensor on the device
+    if hasattr(x, "data_ptr"):  # torch tensor: kernels can take neither host memory nor another device's
+        if x.get_device() != device:
+            raise MpcxError(f"a tensor on {x.device} was passed to a context on device {device}")
         return x.data_ptr()
     if isinstance(x, (int, np.integer)):
         return int(x)
@@ -105,9 +107,9 @@ def _word(x, keep):
         return x.ptr
     if isinstance(x, (list, tuple)):  # a host array: of device addresses (arrays, tensors) or of counts
         try:
-            words = [e.data_ptr() for e in x]
+            words = [e.data_ptr() if e.get_device() == device else _word(e, device, keep) for e in x]  # tensors: the short way
         except AttributeError:
-            words = [(e if type(e) is int else _word(e, keep)) & 0xFFFFFFFFFFFFFFFF for e in x]
+            words = [(e if type(e) is int else _word(e, device, keep)) & 0xFFFFFFFFFFFFFFFF for e in x]
         host = array.array("Q", words or [0])
         keep.append(host)
         return host.buffer_info()[0]
@@ -140,7 +142,8 @@ class Context:
             raise MpcxError(f"{name}: {self.lib.mpcx_last_error(self.h).decode()}")
 
     def call(self, name, *args):
-        """Calls ``mpcx_<name>(ctx, *args)``; DeviceArrays / tensors / ints are converted."""
+        """Calls ``mpcx_<name>(ctx, *args)``; DeviceArrays, tensors on the context's device, ints and lists of these are
+        converted."""
         if not self.h:
             raise MpcxError(f"mpcx_{name}: the context is closed")
         fn = self._fns.get((name, len(args)))
@@ -149,7 +152,7 @@ class Context:
             fn.argtypes = [ctypes.c_void_p] + [ctypes.c_uint64] * len(args)
             self._fns[name, len(args)] = fn
         keep = []
-        if fn(self.h, *[_word(x, keep) for x in args]):
+        if fn(self.h, *[_word(x, self.device, keep) for x in args]):
             raise MpcxError(f"mpcx_{name}: {self.lib.mpcx_last_error(self.h).decode()}")
 
     def scratch_bytes(self, name, *sizes):

@@ -437,6 +437,60 @@ def test_logprobs_beyond_four_billion_words(resident, rows, vocab):
         torch.cuda.empty_cache()
 
 
+def test_more_rows_than_one_launch_takes(resident):
+    """Rows, table rows and tokens beyond what the grid of one launch holds."""
+    ctx, torch, dev, be, side = resident
+    i64 = lambda *s: torch.empty(*s, dtype=torch.int64, device=dev)
+    with torch.cuda.stream(side):
+        rows = (1 << 24) + 5
+        x = torch.zeros(rows, 2, dtype=torch.int64, device=dev)
+        x[-1, 1] = x[1 << 22, 1] = 1 << 16
+        ids = torch.ones(rows, dtype=torch.int64, device=dev)
+        f = lambda *s: torch.empty(*s, dtype=torch.float32, device=dev)
+        logp, ent, ls, tl, ti, m = f(rows), f(rows), f(rows), f(rows), i64(rows), i64(rows)
+        ws = torch.empty(ctx.scratch_bytes("reveal_logprobs", rows, 2, 1), dtype=torch.uint8, device=dev)
+        ctx.call("reveal_logprobs", x, None, None, rows, 2, 16, ids, 1, 1, ws, logp, ent, ti, tl, m, ls)
+        grad, w = f(rows, 2), torch.ones(rows, dtype=torch.float32, device=dev)
+        ctx.call("reveal_logprobs_grad", x, None, None, rows, 2, 16, ids, 1, w, None, m, ls, None, grad, None, 0)
+        peak = torch.tensor([1 << 22, rows - 1], device=dev)
+        assert ti.nonzero()[:, 0].tolist() == peak.tolist() and m.nonzero()[:, 0].tolist() == peak.tolist()
+        lp1 = -np.log1p(np.exp(-1.0))
+        assert (logp[peak] - lp1).abs().max().item() < 8 * STEP
+        even = torch.ones(rows, dtype=torch.bool, device=dev)
+        even[peak] = False
+        assert (logp[even] + np.log(2)).abs().max().item() < 8 * STEP and (ent[even] - np.log(2)).abs().max().item() < 16 * STEP
+        assert (grad[even] - torch.tensor([-0.5, 0.5], device=dev)).abs().max().item() < 8 * STEP
+        p = np.exp(lp1)
+        assert (grad[peak] - torch.tensor([p - 1, 1 - p], device=dev, dtype=torch.float32)).abs().max().item() < 8 * STEP
+        del x, ids, logp, ent, ls, tl, ti, m, grad, w, even
+        torch.cuda.empty_cache()
+        # lookup of many wide rows: one workgroup a row
+        n, dim = (1 << 23) + 3, 300
+        T = torch.arange(7 * dim, dtype=torch.int64, device=dev).view(7, dim)
+        ids = torch.arange(n, device=dev) % 7
+        E = i64(n, dim)
+        ctx.call("ring_embed", T, None, 7, dim, ids, n, 1, 0, E, None)
+        for a in range(0, n, 1 << 21):
+            assert torch.equal(E[a:a + (1 << 21)], T[ids[a:a + (1 << 21)]])
+        del E
+        torch.cuda.empty_cache()
+        # the gradient of a table of many rows
+        vocab, dim, n = (1 << 23) + 9, 300, 40
+        D, G = i64(vocab, dim), torch.arange(n * dim, dtype=torch.int64, device=dev).view(n, dim) + 1
+        ids = torch.full((n,), vocab - 1, dtype=torch.int64, device=dev)
+        ids[:3] = torch.tensor([0, 5 << 20, vocab - 2], device=dev)
+        ws = torch.empty(ctx.scratch_bytes("ring_embed_grad", n, vocab, dim), dtype=torch.uint8, device=dev)
+        D.fill_(-1)
+        ctx.call("ring_embed_grad", G, None, ids, n, vocab, dim, 2, 0, 0, ws, D, None)
+        for k in range(3):
+            assert torch.equal(D[ids[k]], 2 * G[k])
+        assert torch.equal(D[vocab - 1], 2 * G[3:].sum(0))
+        D[ids] = 0
+        assert not any(D[a:a + (1 << 20)].any().item() for a in range(0, vocab, 1 << 20))
+        del D, ws
+        torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------------ together
 def secure_step(be, w, E, W, ids, targets, rows, vocab, dim, frac):
     """One step of a private next-token model (table E, head W, both shared) on public text: lookup, product with the head,

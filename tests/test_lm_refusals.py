@@ -103,7 +103,7 @@ def lp(a=X, b=X, c=X, rows=3, vocab=5, frac=16, ids=X, per_row=1, top=2, scratch
 
 
 @pytest.mark.parametrize("args,text", [
-    (lp(vocab=0), "vocabulary"), (lp(vocab=1 << 31), "vocabulary"), (lp(rows=1 << 31), "too large"),
+    (lp(vocab=0), "vocabulary"), (lp(vocab=1 << 31), "vocabulary"), (lp(rows=1 << 60), "too large"),
     (lp(rows=1 << 20, per_row=1 << 50), "too large"), (lp(frac=63), "fractional"), (lp(frac=-1), "fractional"),
     (lp(top=33, vocab=100), "alternatives"), (lp(top=6), "alternatives"), (lp(b=N), "third share"),
     (lp(a=N), "NULL"), (lp(ids=N), "NULL"), (lp(logp=N), "NULL"), (lp(scratch=N), "NULL"), (lp(top_ids=N), "NULL"),
@@ -120,10 +120,57 @@ def lg(a=X, b=X, c=X, rows=3, vocab=5, frac=16, ids=X, per_row=1, d_logp=X, d_en
 
 
 @pytest.mark.parametrize("args,text", [
-    (lg(vocab=0), "vocabulary"), (lg(vocab=1 << 31), "vocabulary"), (lg(rows=1 << 31), "too large"), (lg(frac=63), "fractional"),
+    (lg(vocab=0), "vocabulary"), (lg(vocab=1 << 31), "vocabulary"), (lg(rows=1 << 60), "too large"), (lg(frac=63), "fractional"),
     (lg(grad_frac=63), "fractional"), (lg(grad_frac=-1), "fractional"), (lg(b=N), "third share"), (lg(a=N), "NULL"),
     (lg(ids=N), "NULL"), (lg(d_logp=N), "NULL"), (lg(row_max=N), "NULL"), (lg(log_sum=N), "NULL"), (lg(entropy=N), "NULL"),
     (lg(grad=N, words=N), "NULL"),
 ])
 def test_logprobs_grad(lib, args, text):
     refused(lib, "mpcx_reveal_logprobs_grad", args, text)
+
+
+class Sized:
+    def __init__(self, n):
+        self.size = n
+
+
+def test_backend_refuses_arrays_that_do_not_fit_the_shapes():
+    """The Python backends know the lengths of their arrays and check them before anything is uploaded."""
+    from mpc_amd.backends import GpuBackend
+    be = object.__new__(GpuBackend)  # without a context
+    A = Sized
+    calls = [
+        lambda: be.ring_embed(A(11), None, 3, 4, A(2)),
+        lambda: be.ring_embed(A(12), A(13), 3, 4, A(2)),
+        lambda: be.ring_embed_grad(A(9), None, A(2), 3, 4),
+        lambda: be.ring_embed_grad(A(8), A(7), A(2), 3, 4),
+        lambda: be.aby3_sqnorm_local([A(3)], [A(4)], 1, 0, 2, 0),
+        lambda: be.aby3_sqnorm_local([A(3)], [A(3), A(1)], 1, 0, 2, 0),
+        lambda: be.aby3_clip_local(0, [A(3)], [A(2)], A(1), A(1), A(1), 1, 16, 1, 0),
+        lambda: be.aby3_clip_local(0, [A(3)], [A(3)], A(1), A(2), A(1), 1, 16, 1, 0),
+        lambda: be.reveal_logprobs(A(12), A(12), A(11), 3, 4, 16, A(3)),
+        lambda: be.reveal_logprobs(A(12), None, None, 3, 4, 16, A(4)),
+        lambda: be.reveal_logprobs_grad(A(12), None, None, 3, 4, 16, A(3), A(2), None, A(3), A(3), None, 16),
+        lambda: be.reveal_logprobs_grad(A(12), None, None, 3, 4, 16, A(3), A(3), None, A(3), A(2), None, 16),
+        lambda: be.reveal_logprobs_grad(A(12), None, None, 3, 4, 16, A(3), A(3), A(3), A(3), A(3), A(1), 16),
+    ]
+    for k, f in enumerate(calls):
+        with pytest.raises(ValueError, match="elements where|first shares"):
+            f()
+
+
+def test_binding_refuses_tensors_of_another_device():
+    import torch
+    from mpc_amd import MpcxError
+    from mpc_amd.lib import _word
+    host = torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(MpcxError, match="context on device 0"):
+        _word(host, 0, [])
+    with pytest.raises(MpcxError, match="context on device 0"):
+        _word([host, host], 0, [])
+    with pytest.raises(TypeError):
+        _word(1.5, 0, [])
+    keep = []
+    assert _word(-3, 0, keep) == -3 and _word(None, 0, keep) == 0 and not keep
+    _word([1, 2, -1], 0, keep)
+    assert list(keep[0]) == [1, 2, 2 ** 64 - 1]
