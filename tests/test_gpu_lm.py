@@ -672,7 +672,7 @@ def test_two_contexts_at_once(resident):
 def test_clip_of_tensors_on_both_sides_of_the_fused_size(gpu):
     """Party 1 takes long tensors one by one and short ones together."""
     rng = np.random.default_rng(77)
-    lens = [(1 << 18) - 1, 5, 1 << 18, 0, 1, (1 << 18) + 4097, 300, 0]
+    lens = [(1 << 23) - 1, 5, 1 << 23, 0, 1, (1 << 23) + 4097, 300, 0]
     X0, X1 = [rnd(rng, n) for n in lens], [rnd(rng, n) for n in lens]
     z = [np.array([v], np.int64) for v in (25 << 32, 0, 0)]
     c = ref.clip_factor(25 << 32, 1 << 16, 16)
