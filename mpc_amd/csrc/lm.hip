@@ -1021,12 +1021,12 @@ template <int SH> __global__ __launch_bounds__(JOIN_THREADS) void logprobs_join_
     logprobs_finish(in, A, row, s, buf, tid, THREADS, id, at_id);
 }
 
-// The gradient.  A workgroup takes `chunk` words of a row, 16 bytes of each share per load and GRAD_PAIRS of them together;
+// The gradient.  TPR threads (a workgroup, or one wavefront of it for short rows) take `chunk` words of a row, 16 bytes of each share per load and GRAD_PAIRS of them together;
 // the words of the given ids are written again at the end with their own terms added, so that the pass itself knows no
 // ids and every word is rounded once.
 constexpr u32 GRAD_PAIRS = 8;
 struct LogprobGradArgs {
-    u64 vocab, chunk;
+    u64 rows, vocab, chunk;
     u32 splits;
     float unit, words; // 2^-frac, 2^grad_frac
     const i64 *ids;
@@ -1039,23 +1039,28 @@ struct LogprobGradArgs {
 };
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef f32x2 f32x2u __attribute__((aligned(4)));
-template <int SH, bool STREAM> __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, LogprobGradArgs A) {
+template <int SH, bool STREAM, u32 TPR>
+__global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, LogprobGradArgs A) {
     __shared__ float ws[4];
-    const u32 tid = threadIdx.x;
-    const u64 row = blockIdx.x / A.splits, split = blockIdx.x % A.splits, base = row * A.vocab;
+    const u32 tid = threadIdx.x % TPR;
+    const u64 group = (u64)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const u64 row = group / A.splits, split = group % A.splits, base = row * A.vocab;
+    if (row >= A.rows) return; // TPR = 64: no barrier follows
     const u64 j0 = split * A.chunk, j1 = j0 + A.chunk < A.vocab ? j0 + A.chunk : A.vocab;
     const i64 m = A.row_max[row];
     const float ls = A.log_sum[row], h = A.d_entropy ? A.d_entropy[row] : 0.0f, H = A.d_entropy ? A.entropy[row] : 0.0f;
     const i64 *ids = A.ids + row * A.per_row;
     const float *dl = A.d_logp + row * A.per_row;
     float w = 0;
-    for (u64 t = tid; t < A.per_row; t += 256)
+    for (u64 t = tid; t < A.per_row; t += TPR)
         if ((u64)ids[t] < A.vocab) w += dl[t];
     if (A.per_row > 1) {
         for (u32 d = 32; d; d >>= 1) w += __shfl_xor(w, (int)d);
-        if ((tid & 63) == 0) ws[tid >> 6] = w;
-        __syncthreads();
-        w = ws[0] + ws[1] + ws[2] + ws[3];
+        if (TPR > 64) {
+            if ((tid & 63) == 0) ws[tid >> 6] = w;
+            __syncthreads();
+            w = ws[0] + ws[1] + ws[2] + ws[3];
+        }
     } else if (A.per_row) {
         w = (u64)ids[0] < A.vocab ? dl[0] : 0.0f;
     }
@@ -1077,7 +1082,7 @@ template <int SH, bool STREAM> __global__ __launch_bounds__(256) void logprobs_g
         if (A.grad_words) st2<STREAM>((u64 *)A.grad_words + at, u64x2{(u64)nearest_word(g.x * A.words), (u64)nearest_word(g.y * A.words)});
     };
     u64 tile = j0;
-    for (; tile + 512 * GRAD_PAIRS <= j1; tile += 512 * GRAD_PAIRS) {
+    for (; TPR > 64 && tile + 512 * GRAD_PAIRS <= j1; tile += 512 * GRAD_PAIRS) {
         const u64 at = base + tile + 2 * tid;
         u64x2 x[GRAD_PAIRS];
 #pragma unroll
@@ -1085,15 +1090,16 @@ template <int SH, bool STREAM> __global__ __launch_bounds__(256) void logprobs_g
 #pragma unroll
         for (u32 k = 0; k < GRAD_PAIRS; k++) put2(at + 512 * k, x[k]);
     }
-    for (u64 j = tile + 2 * tid; j < j1; j += 512) {
+    for (u64 j = tile + 2 * tid; j < j1; j += 2 * TPR) {
         if (j + 1 < j1) put2(base + j, in.at2(base + j));
         else put1(base + j, part((u64)in.at(base + j)));
     }
     if (A.per_row == 0) return;
     // a word of an id is written by another lane now: the stores above have to be done
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (u64 t = tid; t < A.per_row; t += 256) {
+    if (TPR > 64) __syncthreads();
+    else prg_wave_sync();
+    for (u64 t = tid; t < A.per_row; t += TPR) {
         const u64 id = (u64)ids[t];
         if (id < j0 || id >= j1) continue;
         float g = 0; // equal ids write the same value
@@ -1107,6 +1113,7 @@ template <int SH, bool STREAM> __global__ __launch_bounds__(256) void logprobs_g
 constexpr u64 LP_GROUPS = 1024; // workgroups that fill the chip: four on each CU
 constexpr u64 LP_CHUNK = 2048;  // words: one tile for each of four wavefronts
 constexpr u64 LP_WAVE_ROW = 1024; // rows up to this length are read by one wavefront each
+constexpr u64 LP_GRAD_WAVE_ROW = 768; // the same for the gradient: 8192 rows of 500 21 us against 27, of 1000 38 against 38
 template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, LogprobArgs A) {
     const u64 all = A.rows;
     for (u64 r0 = 0; r0 < all; r0 += LM_MAX_BLOCKS) { // rows of one launch; more than one launch: nothing is split
@@ -1373,10 +1380,12 @@ int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b,
     A.ids = ids, A.per_row = per_row, A.d_logp = d_logp, A.d_entropy = d_entropy;
     A.row_max = row_max, A.log_sum = log_sum, A.entropy = entropy, A.grad = grad, A.grad_words = grad_words;
     const bool stream = rows * vocab * ((c ? 24 : b ? 16 : 8) + (grad ? 4 : 0) + (grad_words ? 8 : 0)) > STREAM_BYTES;
+    const bool one_wave = A.splits == 1 && vocab <= LP_GRAD_WAVE_ROW;
     auto run = [&](auto kernel, auto in) -> int {
         for (u64 r0 = 0; r0 < rows; r0 += LM_MAX_BLOCKS) { // rows of one launch; more than one launch: nothing is split
             const u64 now = rows - r0 < LM_MAX_BLOCKS ? rows - r0 : LM_MAX_BLOCKS;
-            hipLaunchKernelGGL(kernel, dim3((u32)(now * A.splits)), dim3(256), 0, ctx->stream, in, A);
+            A.rows = now;
+            hipLaunchKernelGGL(kernel, dim3((u32)ceil_div(now * A.splits, one_wave ? 4 : 1)), dim3(256), 0, ctx->stream, in, A);
             MPCX_LAUNCH_CHECK();
             in.skip(now * vocab);
             auto skip = [&](auto *&p, u64 n) { p = p ? p + n : p; };
@@ -1386,9 +1395,10 @@ int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b,
         return 0;
     };
     const u64 *pa = (const u64 *)a, *pb = (const u64 *)b, *pc = (const u64 *)c;
-    if (c) return run(stream ? logprobs_grad_kernel<3, true> : logprobs_grad_kernel<3, false>, LogitIn<3>{pa, pb, pc});
-    if (b) return run(stream ? logprobs_grad_kernel<2, true> : logprobs_grad_kernel<2, false>, LogitIn<2>{pa, pb, nullptr});
-    return run(stream ? logprobs_grad_kernel<1, true> : logprobs_grad_kernel<1, false>, LogitIn<1>{pa, nullptr, nullptr});
+    auto pick = [&](auto in, auto whole, auto streaming, auto wave) { return run(one_wave ? wave : stream ? streaming : whole, in); };
+    if (c) return pick(LogitIn<3>{pa, pb, pc}, logprobs_grad_kernel<3, false, 256>, logprobs_grad_kernel<3, true, 256>, logprobs_grad_kernel<3, false, 64>);
+    if (b) return pick(LogitIn<2>{pa, pb, nullptr}, logprobs_grad_kernel<2, false, 256>, logprobs_grad_kernel<2, true, 256>, logprobs_grad_kernel<2, false, 64>);
+    return pick(LogitIn<1>{pa, nullptr, nullptr}, logprobs_grad_kernel<1, false, 256>, logprobs_grad_kernel<1, true, 256>, logprobs_grad_kernel<1, false, 64>);
 }
 
 } // extern "C"
