@@ -32,7 +32,10 @@ constexpr u64 STREAM_BYTES = 256ull << 20;
 
 // ---- lookup.  A row is copied by 2^lg lanes (8 .. 256) of a workgroup, 16 bytes of each share per lane and step; the
 // four steps of a lane are all requested before the first is used.
-constexpr u32 EMB_STEPS = 4;
+#ifndef LM_ES
+#define LM_ES 4
+#endif
+constexpr u32 EMB_STEPS = LM_ES;
 template <bool TWO, bool STREAM>
 __global__ __launch_bounds__(256) void embed_kernel(const u64 *__restrict__ T0, const u64 *__restrict__ T1, u64 vocab, u64 dim,
                                                     const i64 *__restrict__ ids, u64 n, u64 scale, int shift,
@@ -476,13 +479,13 @@ __global__ __launch_bounds__(64 * HEAVY_WAVES) void grad_heavy_kernel(GradArgs A
 // kernel's own arguments, so nothing is copied to the device and a captured call keeps its descriptors.  A workgroup
 // finds the tensor of a tile by one comparison per lane and a population count.
 constexpr u32 LM_TENSORS = 96;    // descriptors of 40 bytes: the arguments stay below 4 KiB
-constexpr u64 LM_TILE = 4096;     // words
+constexpr u64 LM_TILE = 1024;     // words
 // From this many words on party 1's segment of a tensor is one launch that consumes the stream's words where they are
 // regenerated (24 bytes of traffic a word); shorter tensors go together, scaled by one launch and masked by a second (40
 // bytes), since a launch that regenerates words takes 35 us however few they are.  2^26 words in 8 tensors: 452 us against
 // 552, in 16: 768 against 552.
 constexpr u64 CLIP_FUSED_WORDS = 1 << 23;
-constexpr u32 LM_GRID = 2048;     // eight workgroups of four waves on each of 256 CUs
+constexpr u32 LM_GRID = 1024;     // of the norm: four workgroups of four waves on each of 256 CUs (2048: 3 % slower)
 struct TensorRef {
     const u64 *x0, *x1;
     u64 n, out, tile0; // words, first word in the call's output, first tile
@@ -1034,7 +1037,7 @@ template <int SH> __global__ __launch_bounds__(JOIN_THREADS) void logprobs_join_
 // The gradient.  TPR threads (a workgroup, or one wavefront of it for short rows) take `chunk` words of a row, 16 bytes of each share per load and GRAD_PAIRS of them together;
 // the words of the given ids are written again at the end with their own terms added, so that the pass itself knows no
 // ids and every word is rounded once.
-constexpr u32 GRAD_PAIRS = 8;
+constexpr u32 GRAD_PAIRS = 4;
 struct LogprobGradArgs {
     u64 rows, vocab, chunk;
     u32 splits;
@@ -1123,6 +1126,9 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, Logp
 constexpr u64 LP_GROUPS = 1024; // workgroups that fill the chip: four on each CU
 constexpr u64 LP_CHUNK = 2048;  // words: one tile for each of four wavefronts
 constexpr u64 LP_WAVE_ROW = 1024; // rows up to this length are read by one wavefront each
+// Words of a row that a workgroup of the gradient takes: one tile.  2048 rows of 32768 words of three shares: 331 us with
+// 2048 words (5.7 TB/s), 344 with 4096, 372 with whole rows.
+constexpr u64 LP_GRAD_CHUNK = 512 * GRAD_PAIRS;
 constexpr u64 LP_GRAD_WAVE_ROW = 768; // the same for the gradient: 8192 rows of 500 21 us against 27, of 1000 38 against 38
 template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, LogprobArgs A) {
     const u64 all = A.rows;
@@ -1326,12 +1332,12 @@ int mpcx_aby3_clip_local(mpcx_ctx *ctx, int party, const int64_t *const *X0, con
         const TensorTable tab = tensor_table(X0, party == 1 ? X1 : nullptr, lens, count, party == 1 ? CLIP_FUSED_WORDS : ~0ull, i, out);
         if (tab.count == 0) continue;
         if (party == 1) {
-            hipLaunchKernelGGL(clip_kernel<true>, dim3(tensor_grid(tab)), dim3(256), 0, ctx->stream, tab, A, coef, Y);
+            hipLaunchKernelGGL(clip_kernel<true>, dim3((u32)lm_blocks(tab.tiles)), dim3(256), 0, ctx->stream, tab, A, coef, Y);
             MPCX_LAUNCH_CHECK();
             u64 *y = Y + first;
             MPCX_TRY(prg_map1(ctx, seed12, PRG_POP_T0 + pop12 + first, out - first, [=] __device__(u64 j, u64 w) { y[j] -= w; }));
         } else {
-            hipLaunchKernelGGL(clip_kernel<false>, dim3(tensor_grid(tab)), dim3(256), 0, ctx->stream, tab, A, coef, Y);
+            hipLaunchKernelGGL(clip_kernel<false>, dim3((u32)lm_blocks(tab.tiles)), dim3(256), 0, ctx->stream, tab, A, coef, Y);
         }
         MPCX_LAUNCH_CHECK();
     }
@@ -1385,15 +1391,16 @@ int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b,
                  "mpcx_reveal_logprobs_grad: NULL pointer");
     MPCX_REQUIRE(ctx, "mpcx_reveal_logprobs_grad: the context is NULL");
     LogprobGradArgs A{};
-    A.vocab = vocab, A.chunk = logprob_chunk(rows, vocab), A.splits = (u32)ceil_div(vocab, A.chunk);
+        A.vocab = vocab, A.chunk = LP_GRAD_CHUNK, A.splits = (u32)ceil_div(vocab, A.chunk);
     A.unit = ldexpf(1.0f, -frac), A.words = ldexpf(1.0f, grad_words ? grad_frac : 0);
     A.ids = ids, A.per_row = per_row, A.d_logp = d_logp, A.d_entropy = d_entropy;
     A.row_max = row_max, A.log_sum = log_sum, A.entropy = entropy, A.grad = grad, A.grad_words = grad_words;
     const bool stream = rows * vocab * ((c ? 24 : b ? 16 : 8) + (grad ? 4 : 0) + (grad_words ? 8 : 0)) > STREAM_BYTES;
     const bool one_wave = A.splits == 1 && vocab <= LP_GRAD_WAVE_ROW;
     auto run = [&](auto kernel, auto in) -> int {
-        for (u64 r0 = 0; r0 < rows; r0 += LM_MAX_BLOCKS) { // rows of one launch; more than one launch: nothing is split
-            const u64 now = rows - r0 < LM_MAX_BLOCKS ? rows - r0 : LM_MAX_BLOCKS;
+        const u64 batch = LM_MAX_BLOCKS / A.splits; // rows of one launch
+        for (u64 r0 = 0; r0 < rows; r0 += batch) {
+            const u64 now = rows - r0 < batch ? rows - r0 : batch;
             A.rows = now;
             hipLaunchKernelGGL(kernel, dim3((u32)ceil_div(now * A.splits, one_wave ? 4 : 1)), dim3(256), 0, ctx->stream, in, A);
             MPCX_LAUNCH_CHECK();
