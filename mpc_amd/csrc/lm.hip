@@ -30,16 +30,15 @@ template <bool STREAM = false> __device__ inline void st2(u64 *p, u64x2 v) {
 }
 constexpr u64 STREAM_BYTES = 256ull << 20;
 
-// ---- lookup.  A row is copied by 2^lg lanes (8 .. 256) of a workgroup, 16 bytes of each share per lane and step; the
-// four steps of a lane are all requested before the first is used.
-#ifndef LM_ES
-#define LM_ES 4
-#endif
-constexpr u32 EMB_STEPS = LM_ES;
+// ---- lookup: a copy of rows, bound by memory traffic (16384 rows of 4096 words of two shares, 6800 different ones: 1.5 GB
+// in 270 us).  A row is copied by 2^lg lanes (8 .. 256) of a workgroup; a lane has two 16-byte loads under way, one of each
+// share or two of the one (two of each: 280 us; one of a single share: 168 us against 127 for that half).
+constexpr u32 emb_steps(bool two) { return two ? 1 : 2; }
 template <bool TWO, bool STREAM>
 __global__ __launch_bounds__(256) void embed_kernel(const u64 *__restrict__ T0, const u64 *__restrict__ T1, u64 vocab, u64 dim,
                                                     const i64 *__restrict__ ids, u64 n, u64 scale, int shift,
                                                     u64 *__restrict__ E0, u64 *__restrict__ E1, u32 lg) {
+    constexpr u32 EMB_STEPS = emb_steps(TWO);
     const u32 lane = threadIdx.x & ((1u << lg) - 1), rows = 256u >> lg;
     const u64 col0 = 2 * (((u64)blockIdx.y * EMB_STEPS << lg) + lane);
     for (u64 t = (u64)blockIdx.x * rows + (threadIdx.x >> lg); t < n; t += (u64)gridDim.x * rows) {
@@ -1224,7 +1223,7 @@ int mpcx_ring_embed(mpcx_ctx *ctx, const int64_t *T0, const int64_t *T1, uint64_
     MPCX_REQUIRE(ids && E0 && (T0 || vocab == 0), "mpcx_ring_embed: NULL pointer");
     MPCX_REQUIRE(ctx, "mpcx_ring_embed: the context is NULL");
     const u32 lg = lanes_log2(dim);
-    const u64 slices = ceil_div(dim, 2 * EMB_STEPS << lg);
+    const u64 slices = ceil_div(dim, 2 * emb_steps(T1) << lg);
     MPCX_REQUIRE(slices < 65536, "mpcx_ring_embed: rows of %llu words", (unsigned long long)dim);
     const dim3 grid((u32)lm_blocks(ceil_div(n, 256u >> lg)), (u32)slices), block(256);
     const bool stream = n * dim * (T1 ? 32 : 16) > STREAM_BYTES;
