@@ -84,9 +84,11 @@ inline u32 lanes_log2(u64 dim) { // lanes for a row: enough for its 16-byte piec
     return lg;
 }
 
-// ---- gradient of the lookup.  Rows of G whose tokens are equal are added; a wavefront (or 2^lg lanes of it) owns a slice
-// of a row of the table, NS 16-byte pieces of each share per lane, and adds NT tokens at a time: NS NT loads of each share
-// are under way together.
+// ---- gradient of the lookup.  Rows of G whose tokens are equal are added; every word of G is read once and every word of
+// the table written once, so memory traffic is the bound.  A wavefront (or 2^lg lanes of it) owns 128 columns of a row of
+// the table, a 16-byte piece of each share per lane (NS = 1), and adds NT tokens at a time, whose loads are under way
+// together.  65536 tokens, 65536 rows of 1024 words of two shares (2.15 GB): 450 us, 410 of them in the additions (5.2 TB/s,
+// what a copy reaches); four pieces per lane take 490, atomic additions into the table 1300.
 struct GradArgs {
     const u64 *G0, *G1;
     const i64 *ids;
@@ -502,7 +504,8 @@ __device__ inline u32 tensor_of(const TensorTable &tab, u64 tile) {
     return __builtin_amdgcn_readfirstlane(k);
 }
 
-// sum of x0 (x0 + 2 x1) over the tiles of a workgroup -> part[workgroup]
+// sum of x0 (x0 + 2 x1) = x0^2 + x0 x1 + x1 x0 over the tiles of a workgroup -> part[workgroup]: one 64-bit product for 16
+// bytes read, bound by the reads (2e8 words in 293 tensors: 505-535 us in all, 6.0-6.3 TB/s)
 __global__ __launch_bounds__(256) void sqnorm_kernel(TensorTable tab, u64 *__restrict__ part) {
     __shared__ u64 ws[4];
     const u32 tid = threadIdx.x;
@@ -564,7 +567,8 @@ __device__ inline i64 nearest_word(float f) {
     return r == r ? (i64)r : 0;
 }
 
-// the largest c in [0, 2^f] with c^2 S <= R^2
+// the largest c in [0, 2^f] with c^2 S <= R^2: an estimate in 64-bit floats, off by one at most (c < 2^32), put right in
+// 128-bit integers, so that all parties and all roundings agree on it
 __device__ inline u64 clip_factor(u64 S, u64 R, int f) {
     const u64 one = 1ull << f;
     if (S == 0) return one;
@@ -583,8 +587,9 @@ struct ClipArgs {
     int number;
     __device__ u64 factor() const { return clip_factor(*za + *zb + *zc, R, number); }
 };
-// SUM = false: y = (c x0) >> number (party 0); SUM = true: y = (c (x0 + x1)) >> number (party 1).  Every workgroup forms the
-// factor, which saves a launch.
+// SUM = false: y = (c x0) >> number (party 0); SUM = true: y = (c (x0 + x1)) >> number (party 1).  A copy with a product,
+// bound by memory traffic (2e8 words in 293 tensors: 575 us, 5.6 TB/s), best with one small tile per workgroup (4096 words
+// and a looping grid: 655 us).  Every workgroup forms the factor, which saves a launch.
 template <bool SUM>
 __global__ __launch_bounds__(256) void clip_kernel(TensorTable tab, ClipArgs A, i64 *__restrict__ coef, u64 *__restrict__ Y) {
     const u32 tid = threadIdx.x;
@@ -753,7 +758,10 @@ __device__ inline void top_first(WaveTop &t, const i64 (&x)[N], const u32 (&idx)
     const i64 m = wave_max(lane_max);
     float near[N / 2];
 #pragma unroll
-    for (u32 k = 0; k < N / 2; k++) near[k] = valid[2 * k] ? word_dist(m, valid[2 * k + 1] && x[2 * k + 1] > x[2 * k] ? x[2 * k + 1] : x[2 * k]) : -1.0f;
+    for (u32 k = 0; k < N / 2; k++) {
+        const i64 best = valid[2 * k + 1] && x[2 * k + 1] > x[2 * k] ? x[2 * k + 1] : x[2 * k];
+        near[k] = valid[2 * k] ? word_dist(m, best) : -1.0f;
+    }
     const float border = top_border<N / 2>(near, t.top, guess);
     bool in[N];
     u32 at[N], n = 0;
@@ -854,10 +862,12 @@ __device__ inline void logprobs_finish(const LogitIn<SH> &in, const LogprobArgs 
     }
 }
 
-// W wavefronts of a workgroup of four read `chunk` words of a row, in tiles of 64 x 8 words each.  A lane keeps its own
-// maximum and sums and moves them when a tile raises its maximum; nothing is exchanged between lanes before the end but
-// the ballots that look for new entries of the top list.  SPLIT: several workgroups read a row, and every wavefront
-// leaves its own part for logprobs_join_kernel.
+// One pass over the logits: maximum, sum of exponentials, entropy sum and top list together, bound by the reads (4096 rows of
+// 32771 words of three shares, 3.2 GB: 539 us, 6.0 TB/s; about 30 vector instructions a word).  W wavefronts of a workgroup
+// of four read `chunk` words of a row, in tiles of 64 x 8 words each.  A lane keeps its own maximum and sums and moves
+// them when a tile raises its maximum; nothing is exchanged between lanes before the end but the ballots that look for new
+// entries of the top list.  SPLIT: several workgroups read a row, and every wavefront leaves its own part for
+// logprobs_join_kernel.
 template <u32 W, bool SPLIT, int SH> __global__ __launch_bounds__(256) void logprobs_kernel(LogitIn<SH> in, LogprobArgs A) {
     constexpr u32 U = 4, N = 2 * U, TILE = 64 * N;
     __shared__ TopEntry buf[4][64];
@@ -950,7 +960,8 @@ template <u32 W, bool SPLIT, int SH> __global__ __launch_bounds__(256) void logp
     logprobs_finish(in, A, row, s, merged, tid, 256);
 }
 constexpr u32 JOIN_THREADS = 512; // 256 / 512 / 1024: 9.4 / 8.2 / 8.1 us for one row of 131072 with 20 alternatives
-// Joins the parts of a row: one workgroup per row.  What counts is the time of one such call, so parts and lists are asked
+// Joins the parts of a row: one workgroup per row.  What counts is the time of one such call (one row of 131072 with 20
+// alternatives: 13.5 us in all, 6.3 of them in the pass, 8.2 here, of which a launch and two trips to memory are 5), so parts and lists are asked
 // for together and every wavefront forms the maximum and the border (from the lanes' maxima over four interleaved sets of
 // parts each) for itself; its entries within the border go to LDS, and after the one barrier the first wavefront sorts
 // them.
@@ -1033,9 +1044,11 @@ template <int SH> __global__ __launch_bounds__(JOIN_THREADS) void logprobs_join_
     logprobs_finish(in, A, row, s, buf, tid, THREADS, id, at_id);
 }
 
-// The gradient.  TPR threads (a workgroup, or one wavefront of it for short rows) take `chunk` words of a row, 16 bytes of each share per load and GRAD_PAIRS of them together;
-// the words of the given ids are written again at the end with their own terms added, so that the pass itself knows no
-// ids and every word is rounded once.
+// The gradient: reads the logits once and writes its floats or words, bound by that traffic (2048 rows of 32768 words of
+// three shares into floats, 1.9 GB: 331 us, 5.7 TB/s).  TPR threads (a workgroup, or one wavefront of it for short rows)
+// take `chunk` words of a row, 16 bytes of each share per load and GRAD_PAIRS of them together; the words of the given
+// ids are written again at the end with their own terms added, so that the pass itself knows no ids and every word is
+// rounded once.
 constexpr u32 GRAD_PAIRS = 4;
 struct LogprobGradArgs {
     u64 rows, vocab, chunk;
@@ -1122,9 +1135,14 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, Logp
     }
 }
 
-constexpr u64 LP_GROUPS = 1024; // workgroups that fill the chip: four on each CU
-constexpr u64 LP_CHUNK = 2048;  // words: one tile for each of four wavefronts
-constexpr u64 LP_WAVE_ROW = 1024; // rows up to this length are read by one wavefront each
+// How a call is cut.  Fewer than LP_ROWS rows: a row is split over workgroups, LP_GROUPS of them in all (four on each CU),
+// as long as each has LP_CHUNK words, one tile for each of its wavefronts (one row of 131072, 20 alternatives: 14 us, with
+// 4096 words 19; 64 rows of 32000: 20 us, with 512 groups 33; 300 rows of 20000: 39 us against 31 unsplit, of 200000: 281
+// against 289).  A row of up to 1024 words, or of up to LP_WAVE_ROW where the rows fill the chip, is read by one wavefront
+// (8192 rows of 1500: 57 us against 108 with four; 2048 rows of 8000: 75 against 81, of 16000: 143 against 141; 1024
+// rows of 1500: 16.5 against 14.5).
+constexpr u64 LP_ROWS = 256, LP_GROUPS = 1024, LP_CHUNK = 2048, LP_WAVE_ROW = 8192;
+bool lp_one_wave(u64 rows, u64 vocab) { return vocab <= 1024 || (vocab <= LP_WAVE_ROW && rows >= 2048); }
 // Words of a row that a workgroup of the gradient takes: one tile.  2048 rows of 32768 words of three shares: 331 us with
 // 2048 words (5.7 TB/s), 344 with 4096, 372 with whole rows.
 constexpr u64 LP_GRAD_CHUNK = 512 * GRAD_PAIRS;
@@ -1135,7 +1153,7 @@ template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, LogprobArgs A)
         A.rows = all - r0 < LM_MAX_BLOCKS ? all - r0 : LM_MAX_BLOCKS;
         if (A.splits > 1)
             hipLaunchKernelGGL((logprobs_kernel<4, true, SH>), dim3((u32)(A.rows * A.splits)), dim3(256), 0, ctx->stream, in, A);
-        else if (A.vocab <= LP_WAVE_ROW)
+        else if (lp_one_wave(all, A.vocab))
             hipLaunchKernelGGL((logprobs_kernel<1, false, SH>), dim3((u32)ceil_div(A.rows, 4)), dim3(256), 0, ctx->stream, in, A);
         else
             hipLaunchKernelGGL((logprobs_kernel<4, false, SH>), dim3((u32)A.rows), dim3(256), 0, ctx->stream, in, A);
@@ -1343,9 +1361,9 @@ int mpcx_aby3_clip_local(mpcx_ctx *ctx, int party, const int64_t *const *X0, con
     return 0;
 }
 
-// Groups that share a row: enough that the launch has LP_GROUPS workgroups of work, as long as each reads LP_CHUNK words.
+// words of a row that one workgroup reads
 static u64 logprob_chunk(u64 rows, u64 vocab) {
-    u64 splits = rows >= LP_GROUPS ? 1 : LP_GROUPS / (rows ? rows : 1);
+    u64 splits = rows >= LP_ROWS ? 1 : LP_GROUPS / (rows ? rows : 1);
     if (splits > ceil_div(vocab, LP_CHUNK)) splits = ceil_div(vocab, LP_CHUNK);
     return ceil_div(ceil_div(vocab, splits ? splits : 1), 2048) * 2048;
 }
