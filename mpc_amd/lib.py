@@ -106,11 +106,14 @@ def _word(x, device, keep):
     if isinstance(x, DeviceArray):
         return x.ptr
     if isinstance(x, (list, tuple)):  # a host array: of device addresses (arrays, tensors) or of counts
-        try:
-            words = [e.data_ptr() if e.get_device() == device else _word(e, device, keep) for e in x]  # tensors: the short way
+        try:  # the short ways: all tensors, all counts
+            words = [e.data_ptr() if e.get_device() == device else _word(e, device, keep) for e in x]
         except AttributeError:
-            words = [(e if type(e) is int else _word(e, device, keep)) & 0xFFFFFFFFFFFFFFFF for e in x]
-        host = array.array("Q", words or [0])
+            words = x
+        try:
+            host = array.array("Q", words or [0])
+        except (TypeError, OverflowError):
+            host = array.array("Q", [_word(e, device, keep) & 0xFFFFFFFFFFFFFFFF for e in x])
         keep.append(host)
         return host.buffer_info()[0]
     raise TypeError(f"cannot pass {t} to the C ABI")
