@@ -868,7 +868,7 @@ __device__ inline void logprobs_finish(const LogitIn<SH> &in, const LogprobArgs 
 // them when a tile raises its maximum; nothing is exchanged between lanes before the end but the ballots that look for new
 // entries of the top list.  SPLIT: several workgroups read a row, and every wavefront leaves its own part for
 // logprobs_join_kernel.
-template <u32 W, bool SPLIT, int SH> __global__ __launch_bounds__(256) void logprobs_kernel(LogitIn<SH> in, LogprobArgs A) {
+template <u32 W, bool SPLIT, int SH> __global__ __launch_bounds__(256, W == 1 ? 5 : 1) void logprobs_kernel(LogitIn<SH> in, LogprobArgs A) {
     constexpr u32 U = 4, N = 2 * U, TILE = 64 * N;
     __shared__ TopEntry buf[4][64];
     __shared__ TopEntry merged[32];
@@ -892,11 +892,14 @@ template <u32 W, bool SPLIT, int SH> __global__ __launch_bounds__(256) void logp
 #pragma unroll
             for (u32 k = 0; k < N; k++) x[k] = (i64)(k & 1 ? p[k / 2].y : p[k / 2].x), valid[k] = true;
         } else {
+            const u32 left = (u32)(j1 - tile);
 #pragma unroll
-            for (u32 k = 0; k < N; k++) {
-                const u64 j = tile + 128 * (k / 2) + 2 * lane + (k & 1);
-                valid[k] = j < j1;
-                x[k] = valid[k] ? in.at(base + j) : INT64_MIN;
+            for (u32 u = 0; u < U; u++) {
+                const u32 j = 128 * u + 2 * lane;
+                u64x2 p = {1ull << 63, 1ull << 63}; // the lowest word
+                if (j + 1 < left) p = in.at2(base + tile + j);
+                else if (j < left) p.x = (u64)in.at(base + tile + j);
+                x[2 * u] = (i64)p.x, x[2 * u + 1] = (i64)p.y, valid[2 * u] = j < left, valid[2 * u + 1] = j + 1 < left;
             }
         }
         i64 m = x[0];
