@@ -279,9 +279,9 @@ struct GradChunk {
     }
 };
 // The whole sort in one launch: a workgroup owns `rows` rows of the table and looks through all ids twice, counting its
-// tokens in LDS (and those of the rows before, which gives its first place), then placing them.  Up to GRAD_SCAN_N tokens:
-// with 1000 rows of 256, 32768 tokens take 55 us in all against 74 with the histogram in memory below (four launches),
-// 65536 take 76 against 71.
+// tokens in LDS (and those of the rows before, which gives its first place), then placing them.  Up to GRAD_SCAN_N tokens,
+// where it comes level with the histogram in memory below, four launches (1000 rows of 256: 32768 tokens take 46 us in
+// all either way, 49152 take 65 against 57; 32768 rows of 256: 74 against 76, 81 against 77).
 constexpr u32 GRAD_SCAN_ROWS = 4096, GRAD_SCAN_THREADS = 1024;
 constexpr u64 GRAD_SCAN_N = 32768;
 __global__ __launch_bounds__(1024) void grad_scan_kernel(const i64 *__restrict__ ids, u32 n, u64 vocab, u32 rows, GradWork W) {
@@ -292,12 +292,18 @@ __global__ __launch_bounds__(1024) void grad_scan_kernel(const i64 *__restrict__
     for (u32 r = tid; r < GRAD_SCAN_ROWS; r += GRAD_SCAN_THREADS) cnt[r] = 0;
     __syncthreads();
     u32 below = 0;
+    auto look = [&](auto token) { // token(t, v) for every id, two by two
 #pragma unroll 4
-    for (u32 t = tid; t < n; t += GRAD_SCAN_THREADS) {
-        const u64 v = (u64)ids[t];
+        for (u32 t = 2 * tid; t + 1 < n; t += 2 * GRAD_SCAN_THREADS) {
+            const u64x2 v = ld2((const u64 *)ids + t);
+            token(t, v.x), token(t + 1, v.y);
+        }
+        if (tid == 0 && (n & 1)) token(n - 1, (u64)ids[n - 1]);
+    };
+    look([&](u32, u64 v) {
         below += v < v0;
         if (v - v0 < own) atomicAdd(&cnt[v - v0], 1u);
-    }
+    });
     __syncthreads();
     u32 c[4], s = 0; // four rows of a thread
 #pragma unroll
@@ -326,11 +332,9 @@ __global__ __launch_bounds__(1024) void grad_scan_kernel(const i64 *__restrict__
     }
     __syncthreads();
     if (mine)
-#pragma unroll 4
-        for (u32 t = tid; t < n; t += GRAD_SCAN_THREADS) {
-            const u64 r = (u64)ids[t] - v0;
-            if (r < own) W.place(atomicAdd(&cnt[r], 1u), t, (u32)(v0 + r));
-        }
+        look([&](u32 t, u64 v) {
+            if (v - v0 < own) W.place(atomicAdd(&cnt[v - v0], 1u), t, (u32)v);
+        });
 }
 __global__ __launch_bounds__(256) void grad_clear_kernel(u32 *p, u64 n) {
     for (u64 i = (u64)blockIdx.x * 256 + threadIdx.x; i < n; i += (u64)gridDim.x * 256) p[i] = 0;
