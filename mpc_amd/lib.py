@@ -33,8 +33,6 @@ def load_library():
         _lib.mpcx_last_error.restype = ctypes.c_char_p
         _lib.mpcx_last_error.argtypes = [ctypes.c_void_p]
         _lib.mpcx_get_stream.restype = ctypes.c_void_p
-        for name in ("ring_embed_grad", "aby3_sqnorm", "reveal_logprobs"):
-            getattr(_lib, f"mpcx_{name}_scratch").restype = ctypes.c_uint64
     return _lib
 
 
@@ -160,7 +158,9 @@ class Context:
 
     def scratch_bytes(self, name, *sizes):
         """Bytes of scratch memory that the caller of ``mpcx_<name>`` hands over (mpcx_<name>_scratch)."""
-        return getattr(self.lib, f"mpcx_{name}_scratch")(*[ctypes.c_uint64(s) for s in sizes])
+        fn = getattr(self.lib, f"mpcx_{name}_scratch")
+        fn.restype = ctypes.c_uint64
+        return fn(*[ctypes.c_uint64(s) for s in sizes])
 
     def sync(self):
         self._call("mpcx_sync")
