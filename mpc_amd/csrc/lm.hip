@@ -196,9 +196,9 @@ template <bool TWO, u32 WAVES> __device__ inline void join_waves(RowAcc<TWO, 1> 
 
 // Few tokens: one launch.  A workgroup owns GRAD_ROWS rows of the table, 128 columns of them: it looks through all ids,
 // sorts its own tokens by row in LDS, and adds them -- a row of few tokens by one wavefront, a row of many by all four.
-// Taken up to GRAD_SMALL_N tokens (1000 rows of 256: 2048 tokens 14 us against 18 of the other form, 4096: 29 against 22) and
-// up to GRAD_SMALL_SCAN ids read by all workgroups together (8000 rows of 512: 1024 tokens 21 us against 27, 2000: 30
-// against 30).
+// Taken up to GRAD_SMALL_N tokens (1000 rows of 256: 2048 tokens 13 us against 18 of the other form, 4096: 25 against 20) and
+// up to GRAD_SMALL_SCAN ids read by all workgroups together (8000 rows of 512: 1024 tokens 21 us against 29, 2000: 30.7
+// against 30.3).
 constexpr u32 GRAD_ROWS = 8, GRAD_SMALL_N = 2048, GRAD_ALONE = 8;
 constexpr u64 GRAD_SMALL_SCAN = 1 << 23;
 template <bool TWO> __global__ __launch_bounds__(256) void embed_grad_small_kernel(GradArgs A) {
@@ -485,11 +485,6 @@ __global__ __launch_bounds__(64 * HEAVY_WAVES) void grad_heavy_kernel(GradArgs A
 // finds the tensor of a tile by one comparison per lane and a population count.
 constexpr u32 LM_TENSORS = 96;    // descriptors of 40 bytes: the arguments stay below 4 KiB
 constexpr u64 LM_TILE = 1024;     // words
-// From this many words on party 1's segment of a tensor is one launch that consumes the stream's words where they are
-// regenerated (24 bytes of traffic a word); shorter tensors go together, scaled by one launch and masked by a second (40
-// bytes), since a launch that regenerates words takes 35 us however few they are.  2^26 words in 8 tensors: 452 us against
-// 552, in 16: 768 against 552.
-constexpr u64 CLIP_FUSED_WORDS = 1 << 23;
 constexpr u32 LM_GRID = 1024;     // of the norm: four workgroups of four waves on each of 256 CUs (2048: 3 % slower)
 struct TensorRef {
     const u64 *x0, *x1;
@@ -500,12 +495,19 @@ struct TensorTable {
     u32 count;
     u64 tiles;
 };
-__device__ inline u32 tensor_of(const TensorTable &tab, u64 tile) {
-    const u32 lane = threadIdx.x & 63;
-    const bool a = lane < tab.count && tab.t[lane].tile0 <= tile;
-    const bool b = lane + 64 < tab.count && tab.t[lane + 64 < LM_TENSORS ? lane + 64 : 0].tile0 <= tile;
+__device__ inline i64 lane_word(i64 v, u32 lane) {
+    const u32 lo = (u32)__builtin_amdgcn_readlane((int)(u32)v, (int)lane), hi = (u32)__builtin_amdgcn_readlane((int)((u64)v >> 32), (int)lane);
+    return (i64)((u64)hi << 32 | lo);
+}
+// the last of `count` descriptors that begins(k) holds for (it does for the first, and for none behind one without)
+template <class F> __device__ inline u32 last_below(u32 count, F begins) {
+    const u32 lane = threadIdx.x & 63, far = lane + 64 < LM_TENSORS ? lane + 64 : 0;
+    const bool a = lane < count && begins(lane), b = lane + 64 < count && begins(far);
     const u32 k = (u32)(__popcll(__ballot(a)) + __popcll(__ballot(b))) - 1;
     return __builtin_amdgcn_readfirstlane(k);
+}
+__device__ inline u32 tensor_of(const TensorTable &tab, u64 tile) {
+    return last_below(tab.count, [&](u32 k) { return tab.t[k].tile0 <= tile; });
 }
 
 // sum of x0 (x0 + 2 x1) = x0^2 + x0 x1 + x1 x0 over the tiles of a workgroup -> part[workgroup]: one 64-bit product for 16
@@ -591,10 +593,9 @@ struct ClipArgs {
     int number;
     __device__ u64 factor() const { return clip_factor(*za + *zb + *zc, R, number); }
 };
-// SUM = false: y = (c x0) >> number (party 0); SUM = true: y = (c (x0 + x1)) >> number (party 1).  A copy with a product,
-// bound by memory traffic (2e8 words in 293 tensors: 575 us, 5.6 TB/s), best with one small tile per workgroup (4096 words
-// and a looping grid: 655 us).  Every workgroup forms the factor, which saves a launch.
-template <bool SUM>
+// y = (c x0) >> number (party 0).  A copy with a product, bound by memory traffic (2e8 words in 293 tensors: 575 us, 5.6
+// TB/s), best with one small tile per workgroup (4096 words and a looping grid: 655 us).  Every workgroup forms the factor,
+// which saves a launch.
 __global__ __launch_bounds__(256) void clip_kernel(TensorTable tab, ClipArgs A, i64 *__restrict__ coef, u64 *__restrict__ Y) {
     const u32 tid = threadIdx.x;
     const u64 c = A.factor();
@@ -603,25 +604,90 @@ __global__ __launch_bounds__(256) void clip_kernel(TensorTable tab, ClipArgs A, 
     for (u64 tile = blockIdx.x; tile < tab.tiles; tile += gridDim.x) {
         const u32 k = tensor_of(tab, tile);
         const u64 at = (tile - tab.t[k].tile0) * LM_TILE, n = tab.t[k].n - at;
-        const u64 *x0 = tab.t[k].x0 + at, *x1 = SUM ? tab.t[k].x1 + at : nullptr;
+        const u64 *x0 = tab.t[k].x0 + at;
         u64 *y = Y + tab.t[k].out + at;
         if (n >= LM_TILE) {
 #pragma unroll
             for (u32 u = 0; u < LM_TILE / 512; u++) {
                 const u32 i = 512 * u + 2 * tid;
-                u64x2 a = ld2(x0 + i);
-                if (SUM) a += ld2(x1 + i);
-                a *= c;
+                const u64x2 a = ld2(x0 + i) * c;
                 st2(y + i, u64x2{(u64)((i64)a.x >> sh), (u64)((i64)a.y >> sh)});
             }
         } else {
-            for (u64 i = tid; i < n; i += 256) {
-                const u64 r = (u64)((i64)((SUM ? x0[i] + x1[i] : x0[i]) * c) >> sh);
-                y[i] = r;
-            }
+            for (u64 i = tid; i < n; i += 256) y[i] = (u64)((i64)(x0[i] * c) >> sh);
         }
     }
 }
+// y = ((c (x0 + x1)) >> number) - w (party 1), w the stream's words, consumed where they are regenerated: 24 bytes of traffic
+// a word, the bound of long tensors (2^26 words in 1, 4 or 16 tensors: 310 us, 5.2 TB/s).  The 32 words of a lane's 16 visits
+// are asked for before the stream's are generated, which hides their way from memory (90 tensors of 5000 words: 25 us against
+// 33).  A wavefront (4096 words) that lies in one tensor finds it once; another goes, at every visit, from tensor to tensor.
+// Scaling all tensors by one launch and masking them by a second takes 542 us for 16 tensors, 30 for 90 of 5000 words, and 26
+// for 90 of 100 words, where this takes 41.
+struct ClipMasked {
+    struct wavefront;
+    TensorTable tab;
+    const i64 *coef;
+    int number;
+    u64 *y;
+    struct Part { // of the launch's words: those below `end`, x0 and x1 at the launch's word 0
+        u64 end;
+        const u64 *x0, *x1;
+    };
+    struct Wave {
+        const ClipMasked &f;
+        Part near, far; // the lane's two tensors
+        Part one;       // the tensor of all words; x0 NULL: there are several
+        u64 c;
+        __device__ static Part of_lane(const Part &p, u32 lane) {
+            return Part{(u64)lane_word((i64)p.end, lane), (const u64 *)lane_word((i64)p.x0, lane), (const u64 *)lane_word((i64)p.x1, lane)};
+        }
+        __device__ Part part(u64 at) const {
+            const u32 k = (u32)(__popcll(__ballot(near.end <= at)) + __popcll(__ballot(far.end <= at)));
+            return k < 64 ? of_lane(near, k) : of_lane(far, k - 64);
+        }
+        struct Ask {
+            u64 a[PRG_VISITS], b[PRG_VISITS];
+        };
+        __device__ Ask ask(u64 rel, u64 count) const {
+            Ask s;
+#pragma unroll
+            for (u32 k = 0; k < PRG_VISITS; k++, rel += PRG_VISIT_STEP) {
+                Part p = one;
+                if (!one.x0) {
+                    const u64 todo = __ballot(rel < count);
+                    for (u64 left = todo; left;) { // a lane's word lies behind those of the lanes before it
+                        const u32 first = (u32)__builtin_ctzll(left);
+                        const Part t = part((u64)lane_word((i64)rel, first));
+                        if ((threadIdx.x & 63) >= first) p = t;
+                        left = todo & ~__ballot(rel < t.end);
+                    }
+                }
+                s.a[k] = s.b[k] = 0;
+                if (rel < count) s.a[k] = p.x0[rel], s.b[k] = p.x1[rel];
+            }
+            return s;
+        }
+        __device__ void put(u64 rel, const u64 (&w)[PRG_VISITS], const Ask &s, u64 count) const {
+#pragma unroll
+            for (u32 k = 0; k < PRG_VISITS; k++, rel += PRG_VISIT_STEP)
+                if (rel < count) f.y[rel] = (u64)((i64)((s.a[k] + s.b[k]) * c) >> f.number) - w[k];
+        }
+    };
+    __device__ Part part_of(u32 k) const {
+        if (k >= tab.count) return Part{~0ull, nullptr, nullptr};
+        const TensorRef &t = tab.t[k];
+        return Part{t.out + t.n, t.x0 - t.out, t.x1 - t.out};
+    }
+    __device__ Wave wave(u64 first, u64 end) const {
+        const u32 lane = threadIdx.x & 63;
+        Wave w{*this, part_of(lane), part_of(lane + 64), Part{0, nullptr, nullptr}, (u64)*coef};
+        if (first >= end) return w;
+        const Part p = w.part(first);
+        if (end <= p.end) w.one = p;
+        return w;
+    }
+};
 __global__ void clip_factor_kernel(ClipArgs A, i64 *coef) { *coef = (i64)A.factor(); }
 
 // ---- opened logits.  A word x = a + b + c stands for the logit x 2^-frac; distances from a maximum are differences of
@@ -649,10 +715,6 @@ __device__ inline float word_dist(i64 hi, i64 lo) {
 }
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); } // v_exp_f32, within one step
 
-__device__ inline i64 lane_word(i64 v, u32 lane) {
-    const u32 lo = (u32)__builtin_amdgcn_readlane((int)(u32)v, (int)lane), hi = (u32)__builtin_amdgcn_readlane((int)((u64)v >> 32), (int)lane);
-    return (i64)((u64)hi << 32 | lo);
-}
 __device__ inline i64 wave_max(i64 v) {
     for (u32 d = 32; d; d >>= 1) {
         const i64 o = (i64)__shfl_xor((long long)v, (int)d);
@@ -968,10 +1030,10 @@ template <u32 W, bool SPLIT, int SH> __global__ __launch_bounds__(256, W == 1 ? 
 }
 constexpr u32 JOIN_THREADS = 512; // 256 / 512 / 1024: 9.4 / 8.2 / 8.1 us for one row of 131072 with 20 alternatives
 // Joins the parts of a row: one workgroup per row.  What counts is the time of one such call (one row of 131072 with 20
-// alternatives: 13.5 us in all, 6.3 of them in the pass, 8.2 here, of which a launch and two trips to memory are 5), so parts and lists are asked
-// for together and every wavefront forms the maximum and the border (from the lanes' maxima over four interleaved sets of
-// parts each) for itself; its entries within the border go to LDS, and after the one barrier the first wavefront sorts
-// them.
+// alternatives: 13.5 us in all, 6.3 of them in the pass, 8.2 here, of which a launch and two trips to memory are 5), so parts
+// and lists are asked for together and every wavefront forms the maximum and the border (from the lanes' maxima over four
+// interleaved sets of parts each) for itself; its entries within the border go to LDS, and after the one barrier the first
+// wavefront sorts them.
 template <int SH> __global__ __launch_bounds__(JOIN_THREADS) void logprobs_join_kernel(LogitIn<SH> in, LogprobArgs A) {
     constexpr u32 K = 4, THREADS = JOIN_THREADS, E = 8192 / THREADS;
     __shared__ TopEntry buf[64];
@@ -1145,9 +1207,10 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, Logp
 // How a call is cut.  Fewer than LP_ROWS rows: a row is split over workgroups, LP_GROUPS of them in all (four on each CU),
 // as long as each has LP_CHUNK words, one tile for each of its wavefronts (one row of 131072, 20 alternatives: 14 us, with
 // 4096 words 19; 64 rows of 32000: 20 us, with 512 groups 33; 300 rows of 20000: 39 us against 31 unsplit, of 200000: 281
-// against 289).  A row of up to 1024 words, or of up to LP_WAVE_ROW where the rows fill the chip, is read by one wavefront
-// (8192 rows of 1500: 57 us against 108 with four; 2048 rows of 8000: 75 against 81, of 16000: 143 against 141; 1024
-// rows of 1500: 16.5 against 14.5).
+// against 289).  A row of up to 1024 words, or of up to LP_WAVE_ROW where the rows fill the chip, is read by one wavefront,
+// others by four (300 rows of 500: 7.4 us against 8.8, of 1000: 9.7 against 8.8; 1024 rows of 1000: 10.6 against 11.2, of
+// 1500: 14.8 against 12.8; 8192 rows of 500: 26 against 75, of 1500: 53 against 97; 2048 rows of 1500: 18.6 against 26, of
+// 8000: 74 against 78, of 16000: 137 against 140).
 constexpr u64 LP_ROWS = 256, LP_GROUPS = 1024, LP_CHUNK = 2048, LP_WAVE_ROW = 8192;
 bool lp_one_wave(u64 rows, u64 vocab) { return vocab <= 1024 || (vocab <= LP_WAVE_ROW && rows >= 2048); }
 // Words of a row that a workgroup of the gradient takes: one tile.  2048 rows of 32768 words of three shares: 331 us with
@@ -1276,11 +1339,11 @@ int mpcx_ring_embed_grad(mpcx_ctx *ctx, const int64_t *G0, const int64_t *G1, co
 }
 
 // the next tensors of a call, from tensor `i` on, as one launch's table; advances i and out
-static TensorTable tensor_table(const int64_t *const *X0, const int64_t *const *X1, const uint64_t *lens, u64 count, u64 limit,
-                                u64 &i, u64 &out) {
+static TensorTable tensor_table(const int64_t *const *X0, const int64_t *const *X1, const uint64_t *lens, u64 count, u64 &i,
+                                u64 &out) {
     TensorTable tab;
     tab.count = 0, tab.tiles = 0;
-    for (; i < count && tab.count < LM_TENSORS && lens[i] < limit; i++) {
+    for (; i < count && tab.count < LM_TENSORS; i++) {
         if (lens[i] == 0) continue;
         tab.t[tab.count++] = TensorRef{X0 ? (const u64 *)X0[i] : nullptr, X1 ? (const u64 *)X1[i] : nullptr, lens[i], out, tab.tiles};
         tab.tiles += ceil_div(lens[i], LM_TILE);
@@ -1306,7 +1369,7 @@ int mpcx_aby3_sqnorm_local(mpcx_ctx *ctx, const int64_t *const *X0, const int64_
     MPCX_TRY(mpcx_prg_table(ctx, seed_prev, 0, tB + 1, &ckB));
     u64 *part = (u64 *)scratch, parts = 0, out = 0;
     for (u64 i = 0; i < count;) {
-        const TensorTable tab = tensor_table(X0, X1, lens, count, ~0ull, i, out);
+        const TensorTable tab = tensor_table(X0, X1, lens, count, i, out);
         if (tab.count == 0) continue;
         const u32 grid = tensor_grid(tab);
         hipLaunchKernelGGL(sqnorm_kernel, dim3(grid), dim3(256), 0, ctx->stream, tab, part + parts);
@@ -1343,27 +1406,16 @@ int mpcx_aby3_clip_local(mpcx_ctx *ctx, int party, const int64_t *const *X0, con
     if (party == 2) return at ? prg_fill_words(ctx, seed12, 0, PRG_POP_T0 + pop12, at, 1, Y0, nullptr) : 0;
     u64 out = 0;
     for (u64 i = 0; i < count;) {
-        if (party == 1 && lens[i] >= CLIP_FUSED_WORDS) {
-            const u64 *x0 = (const u64 *)X0[i], *x1 = (const u64 *)X1[i];
-            u64 *y = Y + out;
-            MPCX_TRY(prg_map1(ctx, seed12, PRG_POP_T0 + pop12 + out, lens[i], [=] __device__(u64 j, u64 w) {
-                y[j] = (u64)((i64)((x0[j] + x1[j]) * (u64)*coef) >> number) - w;
-            }));
-            out += lens[i++];
-            continue;
-        }
         const u64 first = out;
-        const TensorTable tab = tensor_table(X0, party == 1 ? X1 : nullptr, lens, count, party == 1 ? CLIP_FUSED_WORDS : ~0ull, i, out);
+        TensorTable tab = tensor_table(X0, party == 1 ? X1 : nullptr, lens, count, i, out);
         if (tab.count == 0) continue;
         if (party == 1) {
-            hipLaunchKernelGGL(clip_kernel<true>, dim3((u32)lm_blocks(tab.tiles)), dim3(256), 0, ctx->stream, tab, A, coef, Y);
-            MPCX_LAUNCH_CHECK();
-            u64 *y = Y + first;
-            MPCX_TRY(prg_map1(ctx, seed12, PRG_POP_T0 + pop12 + first, out - first, [=] __device__(u64 j, u64 w) { y[j] -= w; }));
+            for (u32 k = 0; k < tab.count; k++) tab.t[k].out -= first;
+            MPCX_TRY(prg_map1(ctx, seed12, PRG_POP_T0 + pop12 + first, out - first, ClipMasked{tab, coef, number, Y + first}));
         } else {
-            hipLaunchKernelGGL(clip_kernel<false>, dim3((u32)lm_blocks(tab.tiles)), dim3(256), 0, ctx->stream, tab, A, coef, Y);
+            hipLaunchKernelGGL(clip_kernel, dim3((u32)lm_blocks(tab.tiles)), dim3(256), 0, ctx->stream, tab, A, coef, Y);
+            MPCX_LAUNCH_CHECK();
         }
-        MPCX_LAUNCH_CHECK();
     }
     return 0;
 }
@@ -1415,7 +1467,7 @@ int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b,
                  "mpcx_reveal_logprobs_grad: NULL pointer");
     MPCX_REQUIRE(ctx, "mpcx_reveal_logprobs_grad: the context is NULL");
     LogprobGradArgs A{};
-        A.vocab = vocab, A.chunk = LP_GRAD_CHUNK, A.splits = (u32)ceil_div(vocab, A.chunk);
+    A.vocab = vocab, A.chunk = LP_GRAD_CHUNK, A.splits = (u32)ceil_div(vocab, A.chunk);
     A.unit = ldexpf(1.0f, -frac), A.words = ldexpf(1.0f, grad_words ? grad_frac : 0);
     A.ids = ids, A.per_row = per_row, A.d_logp = d_logp, A.d_entropy = d_entropy;
     A.row_max = row_max, A.log_sum = log_sum, A.entropy = entropy, A.grad = grad, A.grad_words = grad_words;

@@ -9,6 +9,7 @@
 // the waves of a workgroup drift apart: some generate while others store.
 #pragma once
 #include "mpcx_internal.h"
+#include <type_traits>
 
 // orders the LDS traffic of one wavefront for the compiler; the hardware already runs it in program order
 __device__ inline void prg_wave_sync() {
@@ -72,13 +73,21 @@ __device__ inline void mod67_run(const PrgCk c, int zero_to_one, u32 (&w)[PRG_CK
     }
 }
 
+// A functor with a member type `wavefront` is prepared once per wavefront, f.wave(first, end) for the words [first, end) of it
+// (none when first >= end), and asked for what goes with the PRG_VISITS words rel, rel + PRG_VISIT_STEP, .. of each lane
+// before these are generated: all lanes call `ask = own.ask(rel, count)`, then `own.put(rel, v, ask, count)`.
+constexpr u32 PRG_VISITS = 16; // steps between two visits (8: 64-byte runs, 32: half the waves per CU; both measured slower)
+constexpr u64 PRG_VISIT_STEP = 64 / PRG_VISITS * PRG_CK;
+template <class F, class = void> struct PrgAsks : std::false_type {};
+template <class F> struct PrgAsks<F, std::void_t<typename F::wavefront>> : std::true_type {};
+
 // f(rel, v) for rel in [0, count) with v = g(A[tA + rel], B[tB + rel]) (TWO streams) or v = A[tA + rel] (one).
 // g runs in the producing lane (registers only); f runs in memory order.  A lane starts from the checkpoint below
 // its first word and discards the words in between (the same number for every lane).
 template <bool TWO, class G, class F>
 __global__ __launch_bounds__(256) void prg_map_kernel(const PrgCk *__restrict__ ckA, const PrgCk *__restrict__ ckB,
                                                       u64 tA, u64 tB, u64 count, G g, F f) {
-    constexpr u32 CH = 16; // steps between two visits (8: 64-byte runs, 32: half the waves per CU; both measured slower)
+    constexpr u32 CH = PRG_VISITS;
     __shared__ u64 tile[256 * (CH + 1)];
     const u32 tid = threadIdx.x;
     const u64 blk_r0 = (u64)blockIdx.x * 256; // first run of PRG_CK words of this workgroup
@@ -97,21 +106,45 @@ __global__ __launch_bounds__(256) void prg_map_kernel(const PrgCk *__restrict__ 
     for (u32 i = 0; i < skipA; i++) prv_step(sa, la, ha);
     if (TWO)
         for (u32 i = 0; i < skipB; i++) prv_step(sb, lb, hb);
-    for (u32 it = 0; it < PRG_CK / CH; it++) {
+    // the word of this lane's j-th visit, and its place in the tile
+    auto place = [&](u32 it, u32 j, u64 &rel) {
+        const u32 idx = j * 64 + (tid & 63);
+        const u32 row = (tid & ~63u) + idx / CH, col = idx % CH;
+        rel = (blk_r0 + row) * PRG_CK + it * CH + col;
+        return row * (CH + 1) + col;
+    };
+    auto generate = [&] {
 #pragma unroll
         for (u32 k = 0; k < CH; k++) {
             const u64 wa = prv_step(sa, la, ha);
             tile[tid * (CH + 1) + k] = TWO ? g(wa, prv_step(sb, lb, hb)) : wa;
         }
         prg_wave_sync();
-#pragma unroll 4
-        for (u32 j = 0; j < CH; j++) {
-            const u32 idx = j * 64 + (tid & 63);
-            const u32 row = (tid & ~63u) + idx / CH, col = idx % CH;
-            const u64 rel = (blk_r0 + row) * PRG_CK + it * CH + col;
-            if (rel < count) f(rel, tile[row * (CH + 1) + col]);
+    };
+    if constexpr (PrgAsks<F>::value) {
+        const u64 first = (blk_r0 + (tid & ~63u)) * PRG_CK;
+        const auto own = f.wave(first, first + 64 * PRG_CK < count ? first + 64 * PRG_CK : count);
+        for (u32 it = 0; it < PRG_CK / CH; it++) {
+            u64 rel, v[CH];
+            const u32 at = place(it, 0, rel);
+            const auto ask = own.ask(rel, count);
+            generate();
+#pragma unroll
+            for (u32 j = 0; j < CH; j++) v[j] = tile[at + j * (64 / CH) * (CH + 1)];
+            own.put(rel, v, ask, count);
+            prg_wave_sync();
         }
-        prg_wave_sync();
+    } else {
+        for (u32 it = 0; it < PRG_CK / CH; it++) {
+            generate();
+#pragma unroll 4
+            for (u32 j = 0; j < CH; j++) {
+                u64 rel;
+                const u32 at = place(it, j, rel);
+                if (rel < count) f(rel, tile[at]);
+            }
+            prg_wave_sync();
+        }
     }
 }
 

@@ -140,6 +140,53 @@ def test_embed_and_gradient_at_unaligned_addresses(gpu):
         assert np.array_equal(D1.to_host(), ref.embed_grad(G, ids, vocab, dim, 3, 0))
 
 
+def test_scratch_memory_may_begin_at_any_word(gpu):
+    """Scratch memory 8 bytes behind a 16-byte boundary, and the words behind its end are left as they were."""
+    ctx = gpu.ctx
+    rng = np.random.default_rng(31)
+
+    def scratch(name, *sizes):
+        size = ctx.scratch_bytes(name, *sizes)
+        assert size % 8 == 0
+        whole = ctx.to_device(np.full(size // 8 + 9, 0x5A5A, np.int64))
+        return whole, whole.view(1, size // 8), size // 8
+
+    def untouched(whole, words):
+        h = whole.to_host()
+        return h[0] == 0x5A5A and (h[1 + words:] == 0x5A5A).all()
+
+    for vocab, dim, n in ((9000, 33, 3000), (70, 130, 5000), (40000, 64, 40000)):
+        ids, G = tokens(rng, n, vocab), [rnd(rng, n * dim) for _ in range(2)]
+        whole, ws, words = scratch("ring_embed_grad", n, vocab, dim)
+        D = [ctx.empty(np.int64, vocab * dim) for _ in range(2)]
+        dG, dI = [ctx.to_device(g) for g in G], ctx.to_device(ids)
+        ctx.call("ring_embed_grad", dG[0], dG[1], dI, n, vocab, dim, 3, 0, 0, ws, D[0], D[1])
+        ctx.sync()
+        for k in range(2):
+            assert np.array_equal(D[k].to_host(), ref.embed_grad(G[k], ids, vocab, dim, 3, 0))
+        assert untouched(whole, words)
+    for rows, vocab, top in ((1, 50000, 7), (5, 9001, 0), (300, 700, 3)):
+        x = (rng.normal(size=(rows, vocab)) * 65536).astype(np.int64)
+        whole, ws, words = scratch("reveal_logprobs", rows, vocab, top)
+        dX, m, ti, tl = ctx.to_device(x), ctx.empty(np.int64, rows), ctx.empty(np.int64, rows * max(top, 1)), ctx.empty(np.float32, rows * max(top, 1))
+        ctx.call("reveal_logprobs", dX, None, None, rows, vocab, 16, None, 0, top, ws, None, None, ti if top else None,
+                 tl if top else None, m, None)
+        ctx.sync()
+        assert np.array_equal(m.to_host(), x.max(1))
+        if top:
+            assert np.array_equal(ti.to_host().reshape(rows, top), np.argsort(-x, axis=1, kind="stable")[:, :top])
+        assert untouched(whole, words)
+    X = [rnd(rng, 5000 + k) for k in range(200)]
+    dX = [ctx.to_device(x) for x in X]
+    whole, ws, words = scratch("aby3_sqnorm", 200)
+    z = ctx.empty(np.int64, 1)
+    ctx.call("aby3_sqnorm_local", dX, dX, [x.size for x in X], 200, KEY12, 3, KEY12, 3, ws, z)
+    ctx.sync()
+    with np.errstate(over="ignore"):
+        assert int(z.to_host()[0]) == int(sum((3 * x * x).sum() for x in X))  # the two masks are the same word
+    assert untouched(whole, words)
+
+
 def test_embed_gradient_is_the_lookups_adjoint(gpu):
     """sum(G * embed(T)) = sum(embed_grad(G) * T) mod 2^64, and the difference quotient of the lookup in a direction is its
     value there (the map is linear, so the quotient is exact)."""
@@ -669,10 +716,11 @@ def test_two_contexts_at_once(resident):
     other.close()
 
 
-def test_clip_of_tensors_on_both_sides_of_the_fused_size(gpu):
-    """Party 1 takes long tensors one by one and short ones together."""
+@pytest.mark.parametrize("lens", [[(1 << 23) - 1, 5, 1 << 23, 0, 1, (1 << 23) + 4097, 300, 0], [4096] * 20 + [1] * 70 + [64, 4095, 0, 8192] * 30,
+                                  [17, 47, 63, 65, 1, 4031] * 40], ids=["long", "aligned", "odd"])
+def test_clip_of_tensors_that_begin_and_end_anywhere(gpu, lens):
+    """Party 1 finds the tensor of a word per wavefront of 4096 words, or per visit of 64."""
     rng = np.random.default_rng(77)
-    lens = [(1 << 23) - 1, 5, 1 << 23, 0, 1, (1 << 23) + 4097, 300, 0]
     X0, X1 = [rnd(rng, n) for n in lens], [rnd(rng, n) for n in lens]
     z = [np.array([v], np.int64) for v in (25 << 32, 0, 0)]
     c = ref.clip_factor(25 << 32, 1 << 16, 16)
