@@ -29,65 +29,82 @@ template <bool STREAM = false> __device__ inline void st2(u64 *p, u64x2 v) {
         *(u64x2u *)p = v;
 }
 constexpr u64 STREAM_BYTES = 256ull << 20;
+// How a row of dim words is cut: 2^lg lanes (8 .. 2^max_lg, no more than a row needs) take 2 steps << lg words of it, `slices`
+// such pieces.  In calls that stream, the pieces of an output row that does not begin on a 128-byte line are moved forward
+// (`lines`) so that each of them does: a line that two wavefronts write a part of costs the memory more than a whole one.  The
+// first piece then holds up to 15 words less -- a column of it may lie before the row, below 0, as a u64 beyond every column
+// -- and the last one more, so this is done where it takes an eighth more pieces at most (two shares; lookup of 16384 x 4095:
+// 290 us against 306, 65536 x 500 would go from one piece to two: 155 against 126; gradient of 15 tokens, 21447 rows of 3129:
+// 194 us against 253).
+constexpr u32 LINE_WORDS = 16;
+struct RowCut {
+    u32 lg;
+    u64 slices;
+    bool lines;
+    RowCut() = default;
+    RowCut(u64 dim, u32 max_lg, u32 steps, bool stream, const void *out) : lg(3), lines(false) {
+        while (lg < max_lg && (2ull * steps << lg) < dim) lg++;
+        const u64 width = 2ull * steps << lg, whole = ceil_div(dim, width), moved = ceil_div(dim + LINE_WORDS - 1, width);
+        if (stream && ((u64)out % (8 * LINE_WORDS) || dim % LINE_WORDS)) lines = 8 * moved <= 9 * whole;
+        slices = lines ? moved : whole;
+    }
+    // the first column of lane `lane` of slice `slice` of the row that is written at `row`
+    __device__ u64 column(u64 slice, u32 lane, const u64 *row, u32 steps = 1) const {
+        return 2 * ((slice * steps << lg) + lane) - (lines ? (u64)row / 8 % LINE_WORDS : 0);
+    }
+};
+// the two words from p on, of which the row holds those that are asked for
+__device__ inline u64x2 ld_part(const u64 *p, bool lo, bool hi) {
+    if (lo && hi) return ld2(p);
+    u64x2 v = {0, 0};
+    if (lo) v.x = p[0];
+    if (hi) v.y = p[1];
+    return v;
+}
+template <bool STREAM> __device__ inline void st_part(u64 *p, u64x2 v, bool lo, bool hi) {
+    if (lo && hi) return st2<STREAM>(p, v);
+    if (lo) p[0] = v.x;
+    if (hi) p[1] = v.y;
+}
 
 // ---- lookup: a copy of rows, bound by memory traffic (16384 rows of 4096 words of two shares, 6800 different ones: 1.5 GB
-// in 270 us).  A row is copied by 2^lg lanes (8 .. 256) of a workgroup; a lane has two 16-byte loads under way, one of each
+// in 275 us).  A row is copied by 2^lg lanes (8 .. 256) of a workgroup; a lane has two 16-byte loads under way, one of each
 // share or two of the one (two of each: 280 us; one of a single share: 168 us against 127 for that half).
 constexpr u32 emb_steps(bool two) { return two ? 1 : 2; }
 template <bool TWO, bool STREAM>
 __global__ __launch_bounds__(256) void embed_kernel(const u64 *__restrict__ T0, const u64 *__restrict__ T1, u64 vocab, u64 dim,
                                                     const i64 *__restrict__ ids, u64 n, u64 scale, int shift,
-                                                    u64 *__restrict__ E0, u64 *__restrict__ E1, u32 lg) {
+                                                    u64 *__restrict__ E0, u64 *__restrict__ E1, RowCut cut) {
     constexpr u32 EMB_STEPS = emb_steps(TWO);
-    const u32 lane = threadIdx.x & ((1u << lg) - 1), rows = 256u >> lg;
-    const u64 col0 = 2 * (((u64)blockIdx.y * EMB_STEPS << lg) + lane);
+    const u32 lg = cut.lg, lane = threadIdx.x & ((1u << lg) - 1), rows = 256u >> lg;
     for (u64 t = (u64)blockIdx.x * rows + (threadIdx.x >> lg); t < n; t += (u64)gridDim.x * rows) {
         const u64 v = (u64)ids[t];
         const bool ok = v < vocab;
         const u64 *r0 = T0 + v * dim, *r1 = TWO ? T1 + v * dim : nullptr;
-        u64x2 a[EMB_STEPS] = {}, b[EMB_STEPS] = {};
+        const u64 first = cut.column(blockIdx.y, lane, E0 + t * dim, EMB_STEPS);
+        u64x2 a[EMB_STEPS], b[EMB_STEPS];
 #pragma unroll
         for (u32 u = 0; u < EMB_STEPS; u++) {
-            const u64 c = col0 + ((u64)(2 * u) << lg);
-            if (!ok || c >= dim) continue;
-            if (c + 1 < dim) {
-                a[u] = ld2(r0 + c);
-                if (TWO) b[u] = ld2(r1 + c);
-            } else {
-                a[u].x = r0[c];
-                if (TWO) b[u].x = r1[c];
-            }
+            const u64 c = first + ((u64)(2 * u) << lg);
+            const bool lo = ok && c < dim, hi = ok && c + 1 < dim;
+            a[u] = ld_part(r0 + c, lo, hi);
+            if (TWO) b[u] = ld_part(r1 + c, lo, hi);
         }
 #pragma unroll
         for (u32 u = 0; u < EMB_STEPS; u++) {
-            const u64 c = col0 + ((u64)(2 * u) << lg);
-            if (c >= dim) continue;
-            u64x2 x, y;
-            if (TWO) {
-                x = a[u] * scale, y = b[u] * scale;
-            } else {
-                x.x = (u64)((i64)(a[u].x * scale) >> shift), x.y = (u64)((i64)(a[u].y * scale) >> shift);
-            }
-            if (c + 1 < dim) {
-                st2<STREAM>(E0 + t * dim + c, x);
-                if (TWO) st2<STREAM>(E1 + t * dim + c, y);
-            } else {
-                E0[t * dim + c] = x.x;
-                if (TWO) E1[t * dim + c] = y.x;
-            }
+            const u64 c = first + ((u64)(2 * u) << lg);
+            const bool lo = c < dim, hi = c + 1 < dim;
+            u64x2 x = a[u] * scale;
+            if (!TWO) x.x = (u64)((i64)x.x >> shift), x.y = (u64)((i64)x.y >> shift);
+            st_part<STREAM>(E0 + t * dim + c, x, lo, hi);
+            if (TWO) st_part<STREAM>(E1 + t * dim + c, b[u] * scale, lo, hi);
         }
     }
 }
-inline u32 lanes_log2(u64 dim) { // lanes for a row: enough for its 16-byte pieces, 8 .. 256
-    u32 lg = 3;
-    while (lg < 8 && (2ull << lg) < dim) lg++;
-    return lg;
-}
-
 // ---- gradient of the lookup.  Rows of G whose tokens are equal are added; every word of G is read once and every word of
 // the table written once, so memory traffic is the bound.  A wavefront (or 2^lg lanes of it) owns 128 columns of a row of
-// the table, a 16-byte piece of each share per lane (NS = 1), and adds NT tokens at a time, whose loads are under way
-// together.  65536 tokens, 65536 rows of 1024 words of two shares (2.15 GB): 450 us, 410 of them in the additions (5.2 TB/s,
+// the table, a 16-byte piece of each share per lane, and adds NT tokens at a time, whose loads are under way
+// together.  65536 tokens, 65536 rows of 1024 words of two shares (2.15 GB): 440 us, 400 of them in the additions (5.4 TB/s,
 // what a copy reaches); four pieces per lane take 490, atomic additions into the table 1300.
 struct GradArgs {
     const u64 *G0, *G1;
@@ -96,111 +113,68 @@ struct GradArgs {
     int shift, accumulate;
     u64 *D0, *D1;
 };
-template <bool TWO, u32 NS> struct RowAcc {
-    u64x2 a[NS], b[TWO ? NS : 1];
-    __device__ RowAcc() {
-#pragma unroll
-        for (u32 u = 0; u < NS; u++) {
-            a[u] = 0;
-            if (TWO) b[u] = 0;
-        }
-    }
-    // adds columns c0 + u cs (two words each) of one row of each share
-    __device__ void add(const u64 *r0, const u64 *r1, u64 c0, u64 cs, u64 dim) {
-#pragma unroll
-        for (u32 u = 0; u < NS; u++) {
-            const u64 c = c0 + u * cs;
-            if (c + 1 < dim) {
-                a[u] += ld2(r0 + c);
-                if (TWO) b[u] += ld2(r1 + c);
-            } else if (c < dim) {
-                a[u].x += r0[c];
-                if (TWO) b[u].x += r1[c];
-            }
-        }
-    }
-    // adds the rows row(i) of p0 / p1, i = i0, i0 + step, .. below i1, NT at a time, what is left NT / 2 at a time and so on
+template <bool TWO> struct RowAcc {
+    u64x2 a = 0, b = 0;
+    // adds columns c and c + 1 of the rows row(i) of p0 / p1, i = i0, i0 + step, .. below i1, NT at a time, what is left NT / 2
+    // at a time and so on
     template <u32 NT, class F>
-    __device__ void add_rows(F row, const u64 *p0, const u64 *p1, u32 i0, u32 i1, u32 step, u64 c0, u64 cs, u64 dim) {
+    __device__ void add_rows(F row, const u64 *p0, const u64 *p1, u32 i0, u32 i1, u32 step, u64 c, u64 dim) {
+        const bool lo = c < dim, hi = c + 1 < dim;
         u32 i = i0;
-        for (; NT > 1 && i + (NT - 1) * step < i1; i += NT * step) {
+        for (; i + (NT - 1) * step < i1; i += NT * step) {
             u64 at[NT];
-            u64x2 x[NT * NS], y[TWO ? NT * NS : 1];
+            u64x2 x[NT], y[NT];
 #pragma unroll
-            for (u32 q = 0; q < NT; q++) at[q] = row(i + q * step);
+            for (u32 q = 0; q < NT; q++) at[q] = row(i + q * step) + c;
 #pragma unroll
-            for (u32 u = 0; u < NS; u++) {
-                const u64 c = c0 + u * cs;
-#pragma unroll
-                for (u32 q = 0; q < NT; q++) {
-                    x[u * NT + q] = 0;
-                    if (TWO) y[u * NT + q] = 0;
-                    if (c + 1 < dim) {
-                        x[u * NT + q] = ld2(p0 + at[q] + c);
-                        if (TWO) y[u * NT + q] = ld2(p1 + at[q] + c);
-                    } else if (c < dim) {
-                        x[u * NT + q].x = p0[at[q] + c];
-                        if (TWO) y[u * NT + q].x = p1[at[q] + c];
-                    }
-                }
+            for (u32 q = 0; q < NT; q++) {
+                x[q] = ld_part(p0 + at[q], lo, hi);
+                if (TWO) y[q] = ld_part(p1 + at[q], lo, hi);
             }
 #pragma unroll
-            for (u32 u = 0; u < NS; u++)
-#pragma unroll
-                for (u32 q = 0; q < NT; q++) {
-                    a[u] += x[u * NT + q];
-                    if (TWO) b[u] += y[u * NT + q];
-                }
+            for (u32 q = 0; q < NT; q++) {
+                a += x[q];
+                if (TWO) b += y[q];
+            }
         }
-        if (NT > 1) return add_rows<(NT > 1 ? NT / 2 : 1)>(row, p0, p1, i, i1, step, c0, cs, dim);
-        for (; i < i1; i += step) {
-            const u64 at = row(i);
-            add(p0 + at, TWO ? p1 + at : nullptr, c0, cs, dim);
-        }
+        if constexpr (NT > 1) add_rows<NT / 2>(row, p0, p1, i, i1, step, c, dim);
     }
-    template <bool STREAM> __device__ static void put(u64 *p, u64x2 v, bool pair, int accumulate) {
-        if (pair) {
-            if (accumulate) v += ld2(p);
-            st2<STREAM>(p, v);
-        } else {
-            *p = accumulate ? *p + v.x : v.x;
-        }
+    template <bool STREAM> __device__ static void put(u64 *p, u64x2 v, bool lo, bool hi, int accumulate) {
+        if (accumulate) v += ld_part(p, lo, hi);
+        st_part<STREAM>(p, v, lo, hi);
     }
-    template <bool STREAM> __device__ void write(const GradArgs &A, u64 row, u64 c0, u64 cs) {
-#pragma unroll
-        for (u32 u = 0; u < NS; u++) {
-            const u64 c = c0 + u * cs;
-            if (c >= A.dim) continue;
-            u64x2 x = a[u] * A.scale;
-            if (!TWO) x.x = (u64)((i64)x.x >> A.shift), x.y = (u64)((i64)x.y >> A.shift);
-            put<STREAM>(A.D0 + row * A.dim + c, x, c + 1 < A.dim, A.accumulate);
-            if (TWO) put<STREAM>(A.D1 + row * A.dim + c, b[u] * A.scale, c + 1 < A.dim, A.accumulate);
-        }
+    template <bool STREAM> __device__ void write(const GradArgs &A, u64 row, u64 c) const {
+        const bool lo = c < A.dim, hi = c + 1 < A.dim;
+        u64x2 x = a * A.scale;
+        if (!TWO) x.x = (u64)((i64)x.x >> A.shift), x.y = (u64)((i64)x.y >> A.shift);
+        put<STREAM>(A.D0 + row * A.dim + c, x, lo, hi, A.accumulate);
+        if (TWO) put<STREAM>(A.D1 + row * A.dim + c, b * A.scale, lo, hi, A.accumulate);
     }
 };
 // the sums of WAVES wavefronts in the first one (one 16-byte piece of each share per lane); all threads call it
-template <bool TWO, u32 WAVES> __device__ inline void join_waves(RowAcc<TWO, 1> &acc, u64x2 *lds) {
+template <bool TWO, u32 WAVES> __device__ inline void join_waves(RowAcc<TWO> &acc, u64x2 *lds) {
     const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
     if (wave) {
-        lds[(wave - 1) * 64 + lane] = acc.a[0];
-        if (TWO) lds[(WAVES - 1 + wave - 1) * 64 + lane] = acc.b[0];
+        lds[(wave - 1) * 64 + lane] = acc.a;
+        if (TWO) lds[(WAVES - 1 + wave - 1) * 64 + lane] = acc.b;
     }
     __syncthreads();
     if (wave == 0)
         for (u32 w = 0; w < WAVES - 1; w++) {
-            acc.a[0] += lds[w * 64 + lane];
-            if (TWO) acc.b[0] += lds[(WAVES - 1 + w) * 64 + lane];
+            acc.a += lds[w * 64 + lane];
+            if (TWO) acc.b += lds[(WAVES - 1 + w) * 64 + lane];
         }
 }
 
 // Few tokens: one launch.  A workgroup owns GRAD_ROWS rows of the table, 128 columns of them: it looks through all ids,
 // sorts its own tokens by row in LDS, and adds them -- a row of few tokens by one wavefront, a row of many by all four.
-// Taken up to GRAD_SMALL_N tokens (1000 rows of 256: 2048 tokens 13 us against 18 of the other form, 4096: 25 against 20) and
-// up to GRAD_SMALL_SCAN ids read by all workgroups together (8000 rows of 512: 1024 tokens 21 us against 29, 2000: 30.7
-// against 30.3).
+// Taken up to GRAD_SMALL_N tokens (1000 rows of 256: 2048 tokens 12 us against 18 of the other form, 4096: 25 against 20),
+// up to GRAD_SMALL_SCAN ids read by all workgroups together (8000 rows of 512: 500 tokens 17 us against 25, 2000: 23 against
+// 26; of 1024: 2000 tokens 38 us against 32) and up to GRAD_SMALL_BLOCKS workgroups (64 tokens, 8000 rows of 1024: 25 us
+// against 26; one token, 131072 rows of 64: 38 us against 23; 15 tokens, 21447 rows of 3129: 350 us against 190).
 constexpr u32 GRAD_ROWS = 8, GRAD_SMALL_N = 2048, GRAD_ALONE = 8;
-constexpr u64 GRAD_SMALL_SCAN = 1 << 23;
+constexpr u64 GRAD_SMALL_SCAN = 1 << 23, GRAD_SMALL_BLOCKS = 8192;
 template <bool TWO> __global__ __launch_bounds__(256) void embed_grad_small_kernel(GradArgs A) {
     __shared__ u16 list[GRAD_SMALL_N];
     __shared__ u32 cnt[GRAD_ROWS + 1], off[GRAD_ROWS + 1];
@@ -238,16 +212,16 @@ template <bool TWO> __global__ __launch_bounds__(256) void embed_grad_small_kern
     for (u32 r = wave; r < rows; r += 4) {
         const u32 k = off[r + 1] - off[r];
         if (k > GRAD_ALONE || (k == 0 && A.accumulate)) continue;
-        RowAcc<TWO, 1> acc;
-        acc.template add_rows<4>(row, A.G0, A.G1, off[r], off[r + 1], 1, c0, 0, A.dim);
-        acc.template write<false>(A, v0 + r, c0, 0);
+        RowAcc<TWO> acc;
+        acc.template add_rows<4>(row, A.G0, A.G1, off[r], off[r + 1], 1, c0, A.dim);
+        acc.template write<false>(A, v0 + r, c0);
     }
     for (u32 r = 0; r < rows; r++) {
         if (off[r + 1] - off[r] <= GRAD_ALONE) continue;
-        RowAcc<TWO, 1> acc;
-        acc.template add_rows<8>(row, A.G0, A.G1, off[r] + wave, off[r + 1], 4, c0, 0, A.dim);
+        RowAcc<TWO> acc;
+        acc.template add_rows<8>(row, A.G0, A.G1, off[r] + wave, off[r + 1], 4, c0, A.dim);
         join_waves<TWO, 4>(acc, lds);
-        if (wave == 0) acc.template write<false>(A, v0 + r, c0, 0);
+        if (wave == 0) acc.template write<false>(A, v0 + r, c0);
     }
 }
 
@@ -259,23 +233,17 @@ template <bool TWO> __global__ __launch_bounds__(256) void embed_grad_small_kern
 constexpr u32 GRAD_TOGETHER = 4, GRAD_CHUNK = 32;
 struct GradWork {
     u32 *total; // places of the order: tokens inside the vocabulary
-    u32 *count, *start, *rank, *order;
-    u32 *ends;    // the rows of the first and the last place of each full chunk
-    u64 *partial; // two sums of each chunk: dim words of each share
-    __device__ void place(u32 at, u32 t, u32 v) const {
-        order[at] = t;
-        const u32 p = at % GRAD_CHUNK;
-        if (p == 0) ends[2 * (at / GRAD_CHUNK)] = v;
-        if (p == GRAD_CHUNK - 1) ends[2 * (at / GRAD_CHUNK) + 1] = v;
-    }
+    u32 *count, *start, *rank;
+    u32 *order, *row; // of each place: the token and its row
+    u64 *partial;     // two sums of each chunk: dim words of each share
+    __device__ void place(u32 at, u32 t, u32 v) const { order[at] = t, row[at] = v; }
 };
 // chunk k: its places, and the rows of the first and the last one
 struct GradChunk {
     u32 p0, p1, va, vb;
-    __device__ GradChunk(const GradWork &W, const i64 *ids, u32 total, u32 k) {
+    __device__ GradChunk(const GradWork &W, u32 total, u32 k) {
         p0 = k * GRAD_CHUNK, p1 = total - p0 < GRAD_CHUNK ? total : p0 + GRAD_CHUNK;
-        va = W.ends[2 * k];
-        vb = p1 - p0 == GRAD_CHUNK ? W.ends[2 * k + 1] : (u32)ids[W.order[p1 - 1]];
+        va = W.row[p0], vb = W.row[p1 - 1];
     }
 };
 // The whole sort in one launch: a workgroup owns `rows` rows of the table and looks through all ids twice, counting its
@@ -401,42 +369,51 @@ __global__ __launch_bounds__(256) void grad_order_kernel(const i64 *__restrict__
     const u64 v = (u64)ids[t];
     if (v < vocab) W.place(W.start[v] + W.rank[t], t, (u32)v);
 }
-// The first `heavy_blocks` workgroups add the chunks' parts of heavy rows into scratch memory, 128 columns per wavefront;
-// the others one row of the table, 128 columns or less, per 2^lg lanes.
+// The first `heavy` workgroups add the chunks' parts of heavy rows into scratch memory, 128 columns per wavefront; the others
+// one row of the table, 128 columns or less, per 2^lg lanes.  Where rows without tokens stay as they are, the rows are found
+// at the first of their places, else by looking at all of them.
+struct GradCut {
+    u32 heavy, slices; // slices of 128 columns, of heavy rows
+    bool by_place;
+    RowCut row; // of the other rows
+};
 template <bool TWO, bool STREAM>
-__global__ __launch_bounds__(256) void grad_rows_kernel(GradArgs A, GradWork W, u32 heavy_blocks, u32 lg, u32 slices) {
-    RowAcc<TWO, 1> acc;
-    if (blockIdx.x < heavy_blocks) {
+__global__ __launch_bounds__(256) void grad_rows_kernel(GradArgs A, GradWork W, GradCut cut) {
+    RowAcc<TWO> acc;
+    if (blockIdx.x < cut.heavy) {
+        const u32 slices = cut.slices;
         const u32 total = *W.total;
         const u64 items = (u64)((total + GRAD_CHUNK - 1) / GRAD_CHUNK) * slices;
-        for (u64 it = (u64)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += (u64)heavy_blocks * 4) {
+        for (u64 it = (u64)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += (u64)cut.heavy * 4) {
             const u64 k = it / slices, c0 = (it % slices) * 128 + 2 * (threadIdx.x & 63);
-            const GradChunk ch(W, A.ids, total, (u32)k);
+            const GradChunk ch(W, total, (u32)k);
             for (u32 side = 0; side < (ch.va == ch.vb ? 1u : 2u); side++) {
                 const u32 v = side ? ch.vb : ch.va, c = W.count[v], first = W.start[v];
                 if (c <= GRAD_CHUNK) continue;
                 const u32 i0 = first > ch.p0 ? first : ch.p0, i1 = first + c < ch.p1 ? first + c : ch.p1;
-                acc = RowAcc<TWO, 1>();
-                acc.template add_rows<GRAD_TOGETHER>([&](u32 i) { return (u64)W.order[i] * A.dim; }, A.G0, A.G1, i0, i1, 1, c0, 0, A.dim);
-                if (c0 >= A.dim) continue;
+                acc = RowAcc<TWO>();
+                acc.template add_rows<GRAD_TOGETHER>([&](u32 i) { return (u64)W.order[i] * A.dim; }, A.G0, A.G1, i0, i1, 1, c0, A.dim);
                 u64 *p = W.partial + (2 * k + side) * 2 * A.dim + c0;
-                acc.template put<false>(p, acc.a[0], c0 + 1 < A.dim, 0);
-                if (TWO) acc.template put<false>(p + A.dim, acc.b[0], c0 + 1 < A.dim, 0);
+                st_part<false>(p, acc.a, c0 < A.dim, c0 + 1 < A.dim);
+                if (TWO) st_part<false>(p + A.dim, acc.b, c0 < A.dim, c0 + 1 < A.dim);
             }
         }
         return;
     }
-    const u64 step = (u64)(gridDim.x - heavy_blocks) * 256 >> lg;
-    for (u64 item = ((u64)(blockIdx.x - heavy_blocks) * 256 + threadIdx.x) >> lg;; item += step) {
-        const u64 v = item / slices;
-        if (v >= A.vocab) return;
+    const u32 lg = cut.row.lg;
+    const u64 slices = cut.row.slices, n = cut.by_place ? *W.total : A.vocab, step = (u64)(gridDim.x - cut.heavy) * 256 >> lg;
+    for (u64 item = ((u64)(blockIdx.x - cut.heavy) * 256 + threadIdx.x) >> lg; item < n * slices; item += step) {
+        u64 v = item / slices;
+        const u32 place = (u32)v;
+        if (cut.by_place) v = W.row[place];
         const u32 c = W.count[v];
         if (c > GRAD_CHUNK || (c == 0 && A.accumulate)) continue;
-        const u64 c0 = (item % slices) * 128 + 2 * (threadIdx.x & ((1u << lg) - 1));
-        const u32 *list = W.order + (c ? W.start[v] : 0);
-        acc = RowAcc<TWO, 1>();
-        acc.template add_rows<GRAD_TOGETHER>([&](u32 i) { return (u64)list[i] * A.dim; }, A.G0, A.G1, 0, c, 1, c0, 0, A.dim);
-        acc.template write<STREAM>(A, v, c0, 0);
+        const u32 first = c ? W.start[v] : 0;
+        if (cut.by_place && first != place) continue;
+        const u64 c0 = cut.row.column(item % slices, threadIdx.x & ((1u << lg) - 1), A.D0 + v * A.dim);
+        acc = RowAcc<TWO>();
+        acc.template add_rows<GRAD_TOGETHER>([&](u32 i) { return (u64)W.order[first + i] * A.dim; }, A.G0, A.G1, 0, c, 1, c0, A.dim);
+        acc.template write<STREAM>(A, v, c0);
     }
 }
 // 128 columns of the heavy rows that begin in eight chunks (one at most does in each): a wavefront looks at one chunk and
@@ -452,30 +429,30 @@ __global__ __launch_bounds__(64 * HEAVY_WAVES) void grad_heavy_kernel(GradArgs A
         const u64 c0 = (it % slices) * 128 + 2 * lane;
         u32 n = 0, b = 0, v = 0;
         if ((u64)k * GRAD_CHUNK < total) {
-            const GradChunk ch(W, A.ids, total, k);
+            const GradChunk ch(W, total, k);
             const u32 c = W.count[ch.vb], first = W.start[ch.vb];
             if (c > GRAD_CHUNK && first >= ch.p0) n = (first + c - 1) / GRAD_CHUNK - k + 1;
             b = 2 * k + (ch.va != ch.vb), v = ch.vb;
         }
         // the first chunk's sum is the one of its last row, every other chunk's that of its first row
-        auto add = [&](RowAcc<TWO, 1> &acc, u32 b, u32 i0, u32 n, u32 step) {
+        auto add = [&](RowAcc<TWO> &acc, u32 b, u32 i0, u32 n, u32 step) {
             acc.template add_rows<8>([&](u32 i) { return (u64)(i ? (b & ~1u) + 2 * i : b) * 2 * A.dim; }, W.partial,
-                                     W.partial + A.dim, i0, n, step, c0, 0, A.dim);
+                                     W.partial + A.dim, i0, n, step, c0, A.dim);
         };
         __syncthreads(); // the lists of the item before have been read
         if (lane == 0) begin[wave] = b, rows[wave] = v, chunks[wave] = n > HEAVY_ALONE ? n : 0;
         if (n && n <= HEAVY_ALONE) {
-            RowAcc<TWO, 1> acc;
+            RowAcc<TWO> acc;
             add(acc, b, 0, n, 1);
-            acc.template write<false>(A, v, c0, 0);
+            acc.template write<false>(A, v, c0);
         }
         __syncthreads();
         for (u32 q = 0; q < HEAVY_WAVES; q++) {
             if (chunks[q] == 0) continue;
-            RowAcc<TWO, 1> acc;
+            RowAcc<TWO> acc;
             add(acc, begin[q], wave, chunks[q], HEAVY_WAVES);
             join_waves<TWO, HEAVY_WAVES>(acc, lds);
-            if (wave == 0) acc.template write<false>(A, rows[q], c0, 0);
+            if (wave == 0) acc.template write<false>(A, rows[q], c0);
         }
     }
 }
@@ -1242,7 +1219,7 @@ template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, LogprobArgs A)
 
 // scratch memory of the many-token form, in 8-byte words from its start
 struct GradLayout {
-    u64 total, count, start, rank, order, ends, partial, words, rows, n;
+    u64 total, count, start, rank, order, row, partial, words, rows, n;
     bool scan() const { return n <= GRAD_SCAN_N && rows <= GRAD_SCAN_ROWS; } // sorted by one launch, `rows` rows a workgroup
     GradLayout(u64 n_, u64 vocab, u64 dim) : rows(ceil_div(vocab, 256) < GRAD_ROWS ? GRAD_ROWS : ceil_div(vocab, 256)), n(n_) {
         u64 at = 0;
@@ -1252,7 +1229,7 @@ struct GradLayout {
         take(start, 4 * vocab);
         take(rank, scan() ? 0 : 4 * n);
         take(order, 4 * n);
-        take(ends, n / GRAD_CHUNK * 8 + 8);
+        take(row, 4 * n);
         take(partial, n > GRAD_CHUNK ? ceil_div(n, GRAD_CHUNK) * 4 * dim * 8 : 0);
         words = at;
     }
@@ -1260,7 +1237,7 @@ struct GradLayout {
 template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *scratch) {
     const u64 slices = ceil_div(A.dim, 128);
     const u64 small_blocks = ceil_div(A.vocab, GRAD_ROWS) * slices;
-    if (A.n <= GRAD_SMALL_N && (A.n ? A.n : 1) * small_blocks <= GRAD_SMALL_SCAN && slices < 65536) {
+    if (A.n <= GRAD_SMALL_N && A.n * small_blocks <= GRAD_SMALL_SCAN && small_blocks <= GRAD_SMALL_BLOCKS) {
         hipLaunchKernelGGL(embed_grad_small_kernel<TWO>, dim3((u32)ceil_div(A.vocab, GRAD_ROWS), (u32)slices), dim3(256), 0,
                            ctx->stream, A);
         MPCX_LAUNCH_CHECK();
@@ -1269,12 +1246,14 @@ template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *s
     const GradLayout L(A.n, A.vocab, A.dim);
     u64 *w = (u64 *)scratch;
     const GradWork W{(u32 *)(w + L.total), (u32 *)(w + L.count), (u32 *)(w + L.start), (u32 *)(w + L.rank), (u32 *)(w + L.order),
-                     (u32 *)(w + L.ends), w + L.partial};
+                     (u32 *)(w + L.row), w + L.partial};
     const u32 n = (u32)A.n;
-    u32 lg = 3; // lanes of a row: up to a wavefront
-    while (lg < 6 && (2ull << lg) < A.dim) lg++;
-    const u64 heavy_blocks = n <= GRAD_CHUNK ? 0 : A.n > A.vocab ? 1024 : 512; // otherwise no row is heavy
-    const u64 blocks = lm_blocks(ceil_div(A.vocab * slices, 256u >> lg)) + heavy_blocks;
+    const u32 heavy_blocks = n <= GRAD_CHUNK ? 0 : A.n > A.vocab ? 1024 : 512; // otherwise no row is heavy
+    const bool stream = (A.n + A.vocab) * A.dim * (TWO ? 16 : 8) > STREAM_BYTES;
+    GradCut cut{};
+    cut.heavy = heavy_blocks, cut.slices = (u32)slices, cut.by_place = A.accumulate && A.n < A.vocab;
+    cut.row = RowCut(A.dim, 6, 1, stream, A.D0);
+    const u64 blocks = heavy_blocks + lm_blocks(ceil_div((cut.by_place ? A.n : A.vocab) * cut.row.slices, 256u >> cut.row.lg));
     const u64 heavy_items = ceil_div(ceil_div(n, GRAD_CHUNK), HEAVY_WAVES) * slices;
     MPCX_REQUIRE(slices < (1ull << 32), "mpcx_ring_embed_grad: rows of %llu words", (unsigned long long)A.dim);
     if (L.scan()) {
@@ -1287,9 +1266,9 @@ template <bool TWO> int embed_grad_run(mpcx_ctx *ctx, const GradArgs &A, void *s
         hipLaunchKernelGGL(grad_place_kernel, dim3(vb), dim3(256), 0, ctx->stream, (u32)A.vocab, W);
         if (n) hipLaunchKernelGGL(grad_order_kernel, dim3((u32)ceil_div(n, 256)), dim3(256), 0, ctx->stream, A.ids, n, A.vocab, W);
     }
-    const bool stream = (A.n + A.vocab) * A.dim * (TWO ? 16 : 8) > STREAM_BYTES;
-    hipLaunchKernelGGL((stream ? grad_rows_kernel<TWO, true> : grad_rows_kernel<TWO, false>), dim3((u32)blocks), dim3(256), 0,
-                       ctx->stream, A, W, (u32)heavy_blocks, lg, (u32)slices);
+    if (blocks)
+        hipLaunchKernelGGL((stream ? grad_rows_kernel<TWO, true> : grad_rows_kernel<TWO, false>), dim3((u32)blocks), dim3(256), 0,
+                           ctx->stream, A, W, cut);
     if (heavy_blocks)
         hipLaunchKernelGGL(grad_heavy_kernel<TWO>, dim3((u32)lm_blocks(heavy_items)), dim3(64 * HEAVY_WAVES), 0, ctx->stream, A, W,
                            (u32)slices, heavy_items);
@@ -1310,15 +1289,14 @@ int mpcx_ring_embed(mpcx_ctx *ctx, const int64_t *T0, const int64_t *T1, uint64_
     if (n == 0 || dim == 0) return 0;
     MPCX_REQUIRE(ids && E0 && (T0 || vocab == 0), "mpcx_ring_embed: NULL pointer");
     MPCX_REQUIRE(ctx, "mpcx_ring_embed: the context is NULL");
-    const u32 lg = lanes_log2(dim);
-    const u64 slices = ceil_div(dim, 2 * emb_steps(T1) << lg);
-    MPCX_REQUIRE(slices < 65536, "mpcx_ring_embed: rows of %llu words", (unsigned long long)dim);
-    const dim3 grid((u32)lm_blocks(ceil_div(n, 256u >> lg)), (u32)slices), block(256);
     const bool stream = n * dim * (T1 ? 32 : 16) > STREAM_BYTES;
+    const RowCut cut(dim, 8, emb_steps(T1), stream, E0);
+    MPCX_REQUIRE(cut.slices < 65536, "mpcx_ring_embed: rows of %llu words", (unsigned long long)dim);
+    const dim3 grid((u32)lm_blocks(ceil_div(n, 256u >> cut.lg)), (u32)cut.slices), block(256);
     const auto kernel = T1 ? (stream ? embed_kernel<true, true> : embed_kernel<true, false>)
                            : (stream ? embed_kernel<false, true> : embed_kernel<false, false>);
     hipLaunchKernelGGL(kernel, grid, block, 0, ctx->stream, (const u64 *)T0, (const u64 *)T1, vocab, dim, ids, n, (u64)scale, shift,
-                       (u64 *)E0, (u64 *)E1, lg);
+                       (u64 *)E0, (u64 *)E1, cut);
     MPCX_LAUNCH_CHECK();
     return 0;
 }

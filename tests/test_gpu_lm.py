@@ -224,6 +224,51 @@ def test_embed_reaches_rows_beyond_four_billion_words(resident):
         torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("dim,offset", [(1001, 0), (951, 3), (1024, 0), (1024, 1), (1024, 8), (250, 5)])
+@pytest.mark.parametrize("shares", [1, 2])
+def test_large_calls_at_any_line_offset(resident, dim, offset, shares):
+    """Calls beyond the last-level cache, whose stores go by whole lines: rows that begin anywhere in one, and the words
+    before the first row and behind the last stay as they were."""
+    ctx, torch, dev, _, side = resident
+    with torch.cuda.stream(side):
+        vocab, n = (300 << 20) // (8 * dim * shares), 37
+        big = vocab + 1111
+        words = lambda k: torch.randint(-2 ** 63, 2 ** 63 - 1, (k,), dtype=torch.int64, device=dev)
+        put = lambda x: torch.cat([torch.zeros(offset, dtype=torch.int64, device=dev), x])[offset:]
+        ids = torch.randint(0, vocab, (n,), dtype=torch.int64, device=dev)
+        ids[5], ids[6:20] = vocab, ids[20]
+        G = [words(n * dim) for _ in range(shares)]
+        D = [words(vocab * dim + offset + 40) for _ in range(shares)]
+        for accumulate in (0, 1):
+            old = [d.clone() for d in D]
+            ws = torch.empty(ctx.scratch_bytes("ring_embed_grad", n, vocab, dim), dtype=torch.uint8, device=dev)
+            ctx.call("ring_embed_grad", G[0], G[1] if shares == 2 else None, ids, n, vocab, dim, 5, 0, accumulate, ws, D[0][offset:],
+                     D[1][offset:] if shares == 2 else None)
+            ok = ids < vocab
+            for k in range(shares):
+                want = old[k].clone()
+                rows = want[offset:offset + vocab * dim].view(vocab, dim)
+                if not accumulate:
+                    rows.zero_()
+                rows.index_add_(0, ids[ok], G[k].view(n, dim)[ok] * 5)
+                assert torch.equal(D[k], want), (accumulate, k)
+        # every row of the table, and some again
+        some = torch.cat([torch.randperm(vocab, device=dev), torch.randint(0, vocab, (1111,), device=dev)])
+        some[77] = -1
+        E = [words(big * dim + offset + 40) for _ in range(shares)]
+        old = [e.clone() for e in E]
+        T = [put(d[:vocab * dim]) for d in D]
+        ctx.call("ring_embed", T[0], T[1] if shares == 2 else None, vocab, dim, some, big, 3, 0, E[0][offset:],
+                 E[1][offset:] if shares == 2 else None)
+        for k in range(shares):
+            rows = old[k][offset:offset + big * dim].view(big, dim)
+            rows.copy_(T[k].view(vocab, dim)[some.clamp(min=0)] * 3)
+            rows[77].zero_()
+            assert torch.equal(E[k], old[k]), k
+        del D, E, T, old, rows, want
+        torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------------ norm and clipping
 LENS = [[1], [5], [0], [0, 3, 0], [4096], [4097, 1, 70000], [1] * 7, list(range(1, 301)), [257] * 130 + [0] * 3 + [300001],
         [784 * 128, 128, 128 * 128, 128, 128 * 10, 10]]
