@@ -104,14 +104,17 @@ def _word(x, device, keep):
     if isinstance(x, DeviceArray):
         return x.ptr
     if isinstance(x, (list, tuple)):  # a host array: of device addresses (arrays, tensors) or of counts
-        try:  # the short ways: all tensors, all counts
-            words = [e.data_ptr() if e.get_device() == device else _word(e, device, keep) for e in x]
-        except AttributeError:
-            words = x
-        try:
-            host = array.array("Q", words or [0])
-        except (TypeError, OverflowError):
-            host = array.array("Q", [_word(e, device, keep) & 0xFFFFFFFFFFFFFFFF for e in x])
+        kinds, host = set(map(type, x)), None
+        kind = kinds.pop() if len(kinds) == 1 else None
+        if kind is int:  # the short ways: all counts, or all tensors on the device
+            try:
+                host = array.array("Q", x)
+            except OverflowError:
+                pass
+        elif hasattr(kind, "data_ptr") and set(map(kind.get_device, x)) == {device}:
+            host = array.array("Q", list(map(kind.data_ptr, x)))
+        if host is None:
+            host = array.array("Q", [_word(e, device, keep) & 0xFFFFFFFFFFFFFFFF for e in x] or [0])
         keep.append(host)
         return host.buffer_info()[0]
     raise TypeError(f"cannot pass {t} to the C ABI")

@@ -2,6 +2,7 @@
 these run without a GPU (no context)."""
 import ctypes
 
+import numpy as np
 import pytest
 
 U = ctypes.c_uint64
@@ -174,3 +175,10 @@ def test_binding_refuses_tensors_of_another_device():
     assert _word(-3, 0, keep) == -3 and _word(None, 0, keep) == 0 and not keep
     _word([1, 2, -1], 0, keep)
     assert list(keep[0]) == [1, 2, 2 ** 64 - 1]
+    _word((), 0, keep), _word([None, 2 ** 64 - 1, np.int64(5)], 0, keep)
+    assert list(keep[1]) == [0] and list(keep[2]) == [0, 2 ** 64 - 1, 5]
+    _word([host, host[1:]], -1, keep)
+    assert list(keep[3]) == [host.data_ptr(), host.data_ptr() + 8]
+    for wrong in ([host], [host, 7], [7, host[:1]], [host[:1], None], [torch.nn.Parameter(host.double()), host]):
+        with pytest.raises(MpcxError, match="context on device 0"):  # one word of a tensor is never taken for a number
+            _word(wrong, 0, [])
