@@ -370,8 +370,9 @@ __global__ __launch_bounds__(256) void grad_order_kernel(const i64 *__restrict__
     if (v < vocab) W.place(W.start[v] + W.rank[t], t, (u32)v);
 }
 // The first `heavy` workgroups add the chunks' parts of heavy rows into scratch memory, 128 columns per wavefront; the others
-// one row of the table, 128 columns or less, per 2^lg lanes.  Where rows without tokens stay as they are, the rows are found
-// at the first of their places, else by looking at all of them.
+// one row of the table, 128 columns or less, per 2^lg lanes.  Where rows without tokens stay as they are and the tokens are
+// fewer than the rows, the rows are found at the first of their places, else by looking at all of them (32768 rows of 1024,
+// accumulated: 3000 tokens 33 us against 51, 131072 rows of 128: 65536 tokens 69 us against 72).
 struct GradCut {
     u32 heavy, slices; // slices of 128 columns, of heavy rows
     bool by_place;
@@ -665,6 +666,7 @@ struct ClipMasked {
         return w;
     }
 };
+static_assert(sizeof(ClipMasked) <= 4096 - 64, "a kernel's arguments");
 __global__ void clip_factor_kernel(ClipArgs A, i64 *coef) { *coef = (i64)A.factor(); }
 
 // ---- opened logits.  A word x = a + b + c stands for the logit x 2^-frac; distances from a maximum are differences of
