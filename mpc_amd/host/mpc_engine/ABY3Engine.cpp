@@ -905,7 +905,7 @@ void ABY3Engine::clip_norm(const vector<VecPair> &X, uint64_t max_norm, size_t n
         lens.push_back(n);
         total += n;
     }
-    // round 1: the squared norm is opened
+    // first exchange: the squared norm is opened
     Dev<int64_t> zp(gpu, 1), z0(gpu, 1), zn(gpu, 1), coef(gpu, 1), y(gpu, total);
     Dev<uint8_t> scratch(gpu, mpcx_aby3_sqnorm_scratch(X.size()));
     GPU_OK(gpu, mpcx_aby3_sqnorm_local(gpu, x0.data(), x1.data(), lens.data(), X.size(), prgs[pe.next].init_seed, prgs[pe.next].pops,
@@ -918,7 +918,7 @@ void ABY3Engine::clip_norm(const vector<VecPair> &X, uint64_t max_norm, size_t n
     MSG_CHECK(message_recv[pe.prev].size() == sizeof(int64_t) && message_recv[pe.next].size() == sizeof(int64_t));
     upload_string(zp, message_recv[pe.prev]);
     upload_string(zn, message_recv[pe.next]);
-    // round 2: trunc's, of the scaled tensors
+    // second exchange: that of trunc, of the scaled tensors
     const size_t k = party_id == 1 ? 2 : 1; // parties 1 and 2 draw from the stream they share
     GPU_OK(gpu, mpcx_aby3_clip_local(gpu, (int)party_id, x0.data(), x1.data(), lens.data(), X.size(), zp, z0, zn, max_norm,
                                      (int)number, prgs[k].init_seed, prgs[k].pops, y, coef));
