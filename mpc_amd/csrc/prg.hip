@@ -97,7 +97,8 @@ struct Table {
     std::vector<PrgCk *> retired;
     u64 bg_target = 0;    // checkpoints the background walker has been asked for
     bool job_queued = false; // a job for this table is in the walker's queue or running
-    u64 last_need = 0;    // the previous request, for the rate at which the stream is consumed
+    u64 last_need = 0;    // the furthest request, for the rate at which the stream is consumed
+    u64 advanced = 0;     // checkpoints that the requests after the first have moved on by
     u64 loaded_from_disk = 0, saved_to_disk = 0;
     u64 disk_seen_size = 0, disk_seen_mtime = 0; // the cache file as ckpt_load last saw it
 };
@@ -741,6 +742,9 @@ __global__ __launch_bounds__(256) void prg_mod67_listed_kernel(const PrgCk *__re
 
 } // namespace
 
+// checkpoints that a walk in front of a call goes past the call's need, at least
+static const u64 CK_SPARE = 4096;
+
 // save_now: write a table that grew back to the disk cache before returning (mpcx_prg_ckpt_build: another rank of
 // the node may be waiting for the file); otherwise the background thread writes it, off the caller's path
 static int prg_table(mpcx_ctx *ctx, u64 seed, u64 lcg, u64 t_end, const PrgCk **dev, bool save_now) {
@@ -758,7 +762,7 @@ static int prg_table(mpcx_ctx *ctx, u64 seed, u64 lcg, u64 t_end, const PrgCk **
         // walk a little past the request (between 4 Ki and 64 Ki checkpoints) so that the device copy grows once in
         // many calls
         u64 ahead = need / 8;
-        ahead = ahead < 4096 ? 4096 : ahead > 65536 ? 65536 : ahead;
+        ahead = ahead < CK_SPARE ? CK_SPARE : ahead > 65536 ? 65536 : ahead;
         walk_to(T, need + ahead, seed, lcg, true);
         if (save_now || !walker_enabled())
             ckpt_save(T, seed, lcg);
@@ -770,12 +774,15 @@ static int prg_table(mpcx_ctx *ctx, u64 seed, u64 lcg, u64 t_end, const PrgCk **
     // previous request, within 16 Mi .. 256 Mi words, started when less than half of that is left.  Only a request
     // beyond everything asked before counts as consumption: the first one says nothing about a rate (and a table built
     // by mpcx_prg_ckpt_build has been given its length), and a stream that is read again from the start -- fresh engines
-    // with the same keys -- has its table already.
+    // with the same keys -- has its table already.  Nor does a stream that has moved on by less than the spare block of
+    // its first walk: a caller that draws a word a call (the norm's masks) is not worth a walk of millions, nor the
+    // upload beside its kernels.
     {
         const bool advancing = T.last_need != 0 && need > T.last_need && !save_now;
         const u64 step = advancing ? need - T.last_need : 0;
         if (need > T.last_need) T.last_need = need;
-        if (advancing) {
+        T.advanced += step;
+        if (advancing && T.advanced >= CK_SPARE) {
             u64 more = 4 * step;
             const u64 lo = (16ull << 20) / PRG_CK, hi = (256ull << 20) / PRG_CK;
             more = more < lo ? lo : more > hi ? hi : more;
