@@ -85,6 +85,8 @@ class CkVec {
     }
 };
 
+const u64 CKPT_CHUNK = 262144; // checkpoints (6 MB) of one upload, and that the background thread handles per hold of a lock
+
 struct Table {
     std::mutex mu; // walk and upload of THIS stream; streams are extended independently of one another
     std::atomic<int> waiters{0}; // engine calls waiting for mu: the background thread stays away while there are any
@@ -140,13 +142,21 @@ struct Key {
         return lcg < o.lcg;
     }
 };
+// What the uploads of a device's tables go through: a stream of their own, and pinned memory that is never freed or moved.
+// A table's pages move when it grows (CkVec) and go when a process ends while the background thread is at work, which
+// no handler sees after _exit or a signal: no copy engine is ever pointed at them.
+struct UploadLane {
+    std::mutex mu; // one chunk at a time; nothing else is taken while it is held
+    hipStream_t stream = nullptr;
+    PrgCk *stage = nullptr; // CKPT_CHUNK checkpoints
+};
 // The registry and the walker's queue are never destroyed: the background thread may still run at process exit.
 struct Registry {
     std::mutex mu; // guards the map itself (its nodes never move)
     std::map<Key, Table> tables;
     std::map<int, int> live_contexts; // per device
-    std::mutex smu; // guards upload_streams only; nothing else is taken while it is held
-    std::map<int, hipStream_t> upload_streams; // per device, never destroyed
+    std::mutex smu; // guards the map of lanes only (its nodes never move); nothing else is taken while it is held
+    std::map<int, UploadLane> upload_lanes; // per device, never destroyed
     // background walker: one thread, jobs = (table, device)
     std::mutex qmu;
     std::condition_variable qcv;
@@ -256,7 +266,6 @@ void ckpt_load(Table &T, u64 seed, u64 lcg) {
     }
     fclose(f);
 }
-const u64 CKPT_CHUNK = 262144; // checkpoints (6 MB) the background thread handles per hold of a table's lock
 // Writes the table to the cache.  background = false: the caller holds T.mu throughout.  background = true (the
 // background thread, T.mu not held): the lock is taken for one chunk at a time, so an engine call that needs the table
 // waits for a few megabytes at most; the entries being written never change (a table only grows), and `stopping`
@@ -432,22 +441,27 @@ void walk_to(Table &T, u64 want, u64 seed = 0, u64 lcg = 0, bool keyed = false) 
 }
 // Table uploads run on a stream of their own that does not synchronise with the null stream: an engine that works on
 // the null stream (torch's default) has kernels queued there, and a plain hipMemcpy would wait for all of them.
-hipError_t upload_stream(int device, hipStream_t *out) { // the device current
+hipError_t upload_lane(int device, UploadLane **out) { // the device current
     Registry &R = reg();
     std::lock_guard<std::mutex> g(R.smu);
-    auto it = R.upload_streams.find(device);
-    if (it == R.upload_streams.end()) {
-        hipStream_t s = nullptr;
-        hipError_t e = hipStreamCreateWithFlags(&s, hipStreamNonBlocking);
-        if (e != hipSuccess) return e;
-        it = R.upload_streams.emplace(device, s).first;
-    }
-    *out = it->second;
-    return hipSuccess;
+    UploadLane &L = R.upload_lanes[device];
+    hipError_t e = hipSuccess;
+    if (!L.stream) e = hipStreamCreateWithFlags(&L.stream, hipStreamNonBlocking);
+    if (e == hipSuccess && !L.stage) e = hipHostMalloc((void **)&L.stage, CKPT_CHUNK * sizeof(PrgCk), hipHostMallocDefault);
+    *out = &L;
+    return e;
 }
-hipError_t upload_copy(PrgCk *dst, const PrgCk *src, u64 count, hipStream_t s) {
-    hipError_t e = hipMemcpyAsync(dst, src, count * sizeof(PrgCk), hipMemcpyHostToDevice, s);
-    return e == hipSuccess ? hipStreamSynchronize(s) : e; // complete before anybody is told that the entries exist
+hipError_t upload_copy(PrgCk *dst, const PrgCk *src, u64 count, UploadLane &L) {
+    for (u64 done = 0; done < count;) {
+        const u64 n = count - done < CKPT_CHUNK ? count - done : CKPT_CHUNK;
+        std::lock_guard<std::mutex> g(L.mu);
+        mpcx_parallel_memcpy(L.stage, src + done, n * sizeof(PrgCk));
+        hipError_t e = hipMemcpyAsync(dst + done, L.stage, n * sizeof(PrgCk), hipMemcpyHostToDevice, L.stream);
+        if (e == hipSuccess) e = hipStreamSynchronize(L.stream); // complete before anybody is told that the entries exist
+        if (e != hipSuccess) return e;
+        done += n;
+    }
+    return hipSuccess;
 }
 // room of a device copy for `have` checkpoints: the first copy gets a sixteenth more than the request (a table built to a
 // stated length is often read a few words further); a table that outgrows a copy is a pop stream on the move and gets
@@ -460,8 +474,8 @@ u64 upload_capacity(const Table &T, u64 have) {
 hipError_t upload(Table &T, int device) {
     const u64 have = T.host.size();
     if (T.dev_count >= have) return hipSuccess;
-    hipStream_t s;
-    hipError_t e = upload_stream(device, &s);
+    UploadLane *lane;
+    hipError_t e = upload_lane(device, &lane);
     if (e != hipSuccess) return e;
     if (T.dev_cap < have) {
         const u64 cap = upload_capacity(T, have);
@@ -473,7 +487,7 @@ hipError_t upload(Table &T, int device) {
         T.dev_cap = cap;
         T.dev_count = 0;
     }
-    e = upload_copy(T.dev + T.dev_count, T.host.data() + T.dev_count, have - T.dev_count, s);
+    e = upload_copy(T.dev + T.dev_count, T.host.data() + T.dev_count, have - T.dev_count, *lane);
     if (e == hipSuccess) T.dev_count = have;
     return e;
 }
@@ -481,8 +495,8 @@ hipError_t upload(Table &T, int device) {
 // and a larger device copy is filled completely before the table points at it, so an engine call never waits for more
 // than a few megabytes and never sees a copy that is half there.  false = given up (error, or the process is ending).
 template <class Stop> bool upload_background(Table &T, int device, Stop stopping) {
-    hipStream_t s;
-    if (upload_stream(device, &s) != hipSuccess) return false;
+    UploadLane *lane;
+    if (upload_lane(device, &lane) != hipSuccess) return false;
     PrgCk *fresh = nullptr; // a larger copy in the making
     u64 fresh_cap = 0, filled = 0;
     for (;;) {
@@ -502,14 +516,14 @@ template <class Stop> bool upload_background(Table &T, int device, Stop stopping
             }
             if (!fresh && T.dev_cap >= have) { // room in the live copy: append a chunk
                 const u64 n = have - T.dev_count < CKPT_CHUNK ? have - T.dev_count : CKPT_CHUNK;
-                if (upload_copy(T.dev + T.dev_count, T.host.data() + T.dev_count, n, s) != hipSuccess) return false;
+                if (upload_copy(T.dev + T.dev_count, T.host.data() + T.dev_count, n, *lane) != hipSuccess) return false;
                 T.dev_count += n;
                 continue;
             }
             if (fresh) {
                 const u64 upto = have < fresh_cap ? have : fresh_cap;
                 const u64 n = upto - filled < CKPT_CHUNK ? upto - filled : CKPT_CHUNK;
-                if (n && upload_copy(fresh + filled, T.host.data() + filled, n, s) != hipSuccess) break;
+                if (n && upload_copy(fresh + filled, T.host.data() + filled, n, *lane) != hipSuccess) break;
                 filled += n;
                 if (filled == upto) { // caught up with the table: the new copy takes over
                     if (filled > T.dev_count) {

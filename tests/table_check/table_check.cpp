@@ -1,5 +1,5 @@
-// The checkpoint tables of the generator streams on the CPU (hip/hip_runtime.h beside this file): when the background
-// thread walks ahead, and that calls of several threads get the states of the streams.
+// The checkpoint tables of the generator streams on the CPU (hip/hip_runtime.h beside this file): what their uploads read,
+// when the background thread walks ahead, and that calls of several threads get the states of the streams.
 //   table_check <what> ; exit status 0: right
 #include <stdio.h>
 #include <unistd.h>
@@ -80,6 +80,12 @@ static void long_advances() {
         CHECK(right(dev, seed, walked < 40000 ? walked : 40000));
     }
 }
+// uploads, of calls and of the background thread, read pinned memory that stays: never the table's pages, which move
+static void upload_sources() {
+    long_advances();
+    CHECK(stub().copies > 0 && stub().copied > 0);
+    CHECK(stub().from_pageable == 0);
+}
 // several threads advance two streams at once
 static void threads() {
     std::vector<std::thread> th;
@@ -104,6 +110,7 @@ int main(int argc, char **argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     if (what == "short") short_advances();
     else if (what == "long") long_advances();
+    else if (what == "sources") upload_sources();
     else if (what == "threads") threads();
     else return 2;
     fflush(stderr);

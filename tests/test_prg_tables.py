@@ -20,7 +20,7 @@ def table_check(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("what", ["short", "long", "threads"])
+@pytest.mark.parametrize("what", ["short", "long", "sources", "threads"])
 def test_tables(table_check, what):
     env = dict(os.environ, MPCX_CKPT_CACHE="", MPCX_PRG_MARKS="", TSAN_OPTIONS="halt_on_error=1")
     r = subprocess.run([table_check, what], env=env, capture_output=True, text=True, timeout=240)
