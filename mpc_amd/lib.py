@@ -85,6 +85,11 @@ class DeviceArray:
             pass
 
 
+# entry points that take the address of host memory, and in which arguments
+_HOST_ARGS = {"h2d": (1,), "d2h": (0,), "h2d_bits": (1,), "d2h_bits": (0,), "h2d_u16": (1,), "d2h_u16": (0,),
+              "prg_state_at_pop": (3,)}
+
+
 def _word(x, device, keep):
     """One argument of the C ABI as the 64-bit word that carries it: an address, a size, or an int (whose callee reads the
     low half).  `keep` holds what must outlive the call."""
@@ -147,7 +152,7 @@ class Context:
 
     def call(self, name, *args):
         """Calls ``mpcx_<name>(ctx, *args)``; DeviceArrays, tensors on the context's device, ints and lists of these are
-        converted."""
+        converted, and tensors in host memory where the entry point takes a host address."""
         if not self.h:
             raise MpcxError(f"mpcx_{name}: the context is closed")
         fn = self._fns.get((name, len(args)))
@@ -156,6 +161,9 @@ class Context:
             fn.argtypes = [ctypes.c_void_p] + [ctypes.c_uint64] * len(args)
             self._fns[name, len(args)] = fn
         keep = []
+        host = _HOST_ARGS.get(name)
+        if host is not None:  # the address of a tensor in host memory is an int like any other
+            args = [x.data_ptr() if i in host and hasattr(x, "data_ptr") and x.get_device() < 0 else x for i, x in enumerate(args)]
         if fn(self.h, *[_word(x, self.device, keep) for x in args]):
             raise MpcxError(f"mpcx_{name}: {self.lib.mpcx_last_error(self.h).decode()}")
 
