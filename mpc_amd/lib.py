@@ -99,6 +99,8 @@ def _word(x, device, keep):
     if x is None:
         return 0
     if t is DeviceArray:
+        if x.ctx.device != device:
+            raise MpcxError(f"an array on device {x.ctx.device} was passed to a context on device {device}")
         return x.ptr
     if hasattr(x, "data_ptr"):  # torch tensor: kernels can take neither host memory nor another device's
         if x.get_device() != device:
@@ -106,8 +108,8 @@ def _word(x, device, keep):
         return x.data_ptr()
     if isinstance(x, (int, np.integer)):
         return int(x)
-    if isinstance(x, DeviceArray):
-        return x.ptr
+    if isinstance(x, DeviceArray):  # of a derived class
+        return _word(DeviceArray(x.ctx, x.dtype, x.n, ptr=x.ptr), device, keep)
     if isinstance(x, (list, tuple)):  # a host array: of device addresses (arrays, tensors) or of counts
         kinds, host = set(map(type, x)), None
         kind = kinds.pop() if len(kinds) == 1 else None

@@ -35,3 +35,18 @@ def test_host_tensors_where_a_host_address_is_taken(ctx, name, at, args):
     a[at], a[(at + 1) % args] = 4096, host  # and nowhere else
     with pytest.raises(MpcxError, match="context on device 0"):
         ctx.call(name, *a)
+
+
+def test_device_arrays_of_another_device_are_refused(ctx):
+    other = object.__new__(Context)
+    other.h, other.device = None, 1
+    here, there = DeviceArray(ctx, np.int64, 4, ptr=4096), DeviceArray(other, np.int64, 4, ptr=8192)
+
+    class Derived(DeviceArray):
+        pass
+
+    for bad in (there, Derived(other, np.int64, 4, ptr=8192), there.view(1, 2), [there, there], [here, there], (here, None, there.view(0, 4))):
+        with pytest.raises(MpcxError, match="an array on device 1 was passed to a context on device 0"):
+            ctx.call("xor_bools", here, bad, here, 4)
+    ctx.call("xor_bools", Derived(ctx, np.int64, 4, ptr=4096), here.view(1, 2), None, 4)
+    assert ctx._fns.seen == [("xor_bools", (4096, 4104, 0, 4))]
