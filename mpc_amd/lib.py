@@ -2,7 +2,9 @@
 :class:`DeviceArray` (mpcx_malloc) or borrowed from a torch tensor via its ``data_ptr()``."""
 import array
 import ctypes
+import operator
 import os
+import sys
 
 import numpy as np
 
@@ -25,7 +27,6 @@ def load_library():
                             "(hipcc --offload-arch=gfx950); there is no CPU fallback")
         # A process that also uses PyTorch must bring torch's bundled HIP runtime up first: once this library (linked
         # against the system ROCm) has initialised HIP, torch no longer finds the device.
-        import sys
         torch = sys.modules.get("torch")
         if torch is not None and torch.cuda.is_available():
             torch.cuda.init()
@@ -127,6 +128,122 @@ def _word(x, device, keep):
     raise TypeError(f"cannot pass {t} to the C ABI")
 
 
+# ---- The language-model operators say what their arguments have to hold, and it is checked: contiguous arrays of the right
+# type with as many elements as the sizes ask for (raw addresses are taken as they are).  A tensor that is right passes by
+# four questions, so that short calls stay short; everything else goes the long way, which finds the words for what is wrong.
+_I64 = _F32 = None  # torch's types, once an argument is a tensor
+
+
+def _array(x, kind, need, device):
+    """The address of one array of at least `need` elements: "w" 64-bit words, "f" 32-bit floats, "s" bytes of any type."""
+    global _I64, _F32
+    if x is None or isinstance(x, (int, np.integer)):
+        return _word(x, device, [])
+    word = _word(x, device, [])  # refuses what is no array, and other devices
+    if isinstance(x, DeviceArray):
+        right, have = x.dtype in (np.int64, np.uint64) if kind == "w" else x.dtype == np.float32, x.n
+    elif isinstance(x, (list, tuple)):
+        raise MpcxError("a list in the place of an array")
+    else:
+        torch = sys.modules["torch"]
+        _I64, _F32 = torch.int64, torch.float32
+        if not x.is_contiguous():
+            raise MpcxError(f"a tensor of shape {tuple(x.shape)} and strides {x.stride()} that is not contiguous")
+        right, have = x.dtype in ((_I64, torch.uint64) if kind == "w" else (_F32,)), x.numel()
+    if kind == "s":
+        have = x.nbytes
+    elif not right:
+        raise MpcxError(f"an array of {x.dtype} in the place of {'64-bit words' if kind == 'w' else '32-bit floats'}")
+    if have < need:
+        raise MpcxError(f"an array of {have} {'bytes' if kind == 's' else 'elements'} where the sizes ask for {need}")
+    return word
+
+
+def _w(x, need, device):
+    if x is None:
+        return 0
+    if getattr(x, "dtype", 0) is _I64 and x.numel() >= need and x.get_device() == device and x.is_contiguous():
+        return x.data_ptr()
+    return _array(x, "w", need, device)
+
+
+def _f(x, need, device):
+    if x is None:
+        return 0
+    if getattr(x, "dtype", 0) is _F32 and x.numel() >= need and x.get_device() == device and x.is_contiguous():
+        return x.data_ptr()
+    return _array(x, "f", need, device)
+
+
+def _counts(lens, count, keep):
+    """The address of the word counts of a call's tensors."""
+    if isinstance(lens, (list, tuple)) and len(lens) < count:
+        raise MpcxError(f"{len(lens)} counts of {count} tensors")
+    return _word(lens, None, keep)
+
+
+def _tensors(xs, lens, count, device, keep):
+    """The address of the addresses of `count` arrays of `lens` words each."""
+    if not isinstance(xs, (list, tuple)) or not isinstance(lens, (list, tuple)):
+        return _word(xs, device, keep)
+    if len(xs) < count:
+        raise MpcxError(f"{len(xs)} of {count} tensors")
+    kinds = set(map(type, xs))
+    kind = kinds.pop() if len(kinds) == 1 else None
+    if (hasattr(kind, "data_ptr") and len(xs) == len(lens) == count and set(map(kind.dtype.__get__, xs)) == {_I64}
+            and set(map(kind.get_device, xs)) == {device} and all(map(kind.is_contiguous, xs))
+            and all(map(operator.ge, map(kind.numel, xs), lens))):
+        host = array.array("Q", list(map(kind.data_ptr, xs)))
+    else:
+        host = array.array("Q", [_array(x, "w", n, device) & 0xFFFFFFFFFFFFFFFF for x, n in zip(xs[:count], lens)] or [0])
+    keep.append(host)
+    return host.buffer_info()[0]
+
+
+def _ring_embed(ctx, keep, T0, T1, vocab, dim, ids, n, scale, shift, E0, E1):
+    d, table, rows = ctx.device, vocab * dim, n * dim
+    return _w(T0, table, d), _w(T1, table, d), vocab, dim, _w(ids, n, d), n, scale, shift, _w(E0, rows, d), _w(E1, rows, d)
+
+
+def _ring_embed_grad(ctx, keep, G0, G1, ids, n, vocab, dim, scale, shift, accumulate, scratch, dT0, dT1):
+    d, table, rows = ctx.device, vocab * dim, n * dim
+    return (_w(G0, rows, d), _w(G1, rows, d), _w(ids, n, d), n, vocab, dim, scale, shift, accumulate,
+            _array(scratch, "s", ctx.scratch_bytes("ring_embed_grad", n, vocab, dim), d), _w(dT0, table, d), _w(dT1, table, d))
+
+
+def _aby3_sqnorm_local(ctx, keep, X0, X1, lens, count, seed_next, pop_next, seed_prev, pop_prev, scratch, z0):
+    d = ctx.device
+    return (_tensors(X0, lens, count, d, keep), _tensors(X1, lens, count, d, keep), _counts(lens, count, keep), count, seed_next,
+            pop_next, seed_prev, pop_prev, _array(scratch, "s", ctx.scratch_bytes("aby3_sqnorm", count), d), _w(z0, 1, d))
+
+
+def _aby3_clip_local(ctx, keep, party, X0, X1, lens, count, z_prev, z0, z1, max_norm, number, seed12, pop12, Y0, coef):
+    d = ctx.device
+    total = sum(lens[:count]) if isinstance(lens, (list, tuple)) else 0
+    # party 0 does not read the second shares, party 2 none
+    return (party, _tensors(X0, lens, count, d, keep) if party != 2 else 0, _tensors(X1, lens, count, d, keep) if party == 1 else 0,
+            _counts(lens, count, keep), count, _w(z_prev, 1, d), _w(z0, 1, d), _w(z1, 1, d), max_norm, number, seed12, pop12,
+            _w(Y0, total, d), _w(coef, 1, d))
+
+
+def _reveal_logprobs(ctx, keep, a, b, c, rows, vocab, frac, ids, per_row, top, scratch, logp, entropy, top_ids, top_logp, row_max, log_sum):
+    d, x, k, t = ctx.device, rows * vocab, rows * per_row, rows * top
+    return (_w(a, x, d), _w(b, x, d), _w(c, x, d), rows, vocab, frac, _w(ids, k, d), per_row, top,
+            _array(scratch, "s", ctx.scratch_bytes("reveal_logprobs", rows, vocab, top), d), _f(logp, k, d), _f(entropy, rows, d),
+            _w(top_ids, t, d), _f(top_logp, t, d), _w(row_max, rows, d), _f(log_sum, rows, d))
+
+
+def _reveal_logprobs_grad(ctx, keep, a, b, c, rows, vocab, frac, ids, per_row, d_logp, d_entropy, row_max, log_sum, entropy, grad,
+                          grad_words, grad_frac):
+    d, x, k = ctx.device, rows * vocab, rows * per_row
+    return (_w(a, x, d), _w(b, x, d), _w(c, x, d), rows, vocab, frac, _w(ids, k, d), per_row, _f(d_logp, k, d), _f(d_entropy, rows, d),
+            _w(row_max, rows, d), _f(log_sum, rows, d), _f(entropy, rows, d), _f(grad, x, d), _w(grad_words, x, d), grad_frac)
+
+
+_CHECKED = {f.__name__[1:]: f for f in (_ring_embed, _ring_embed_grad, _aby3_sqnorm_local, _aby3_clip_local, _reveal_logprobs,
+                                        _reveal_logprobs_grad)}
+
+
 class Context:
     """One mpcx context (one HIP stream, one scratch workspace) on one GPU."""
 
@@ -166,14 +283,25 @@ class Context:
         host = _HOST_ARGS.get(name)
         if host is not None:  # the address of a tensor in host memory is an int like any other
             args = [x.data_ptr() if i in host and hasattr(x, "data_ptr") and x.get_device() < 0 else x for i, x in enumerate(args)]
-        if fn(self.h, *[_word(x, self.device, keep) for x in args]):
+        checked = _CHECKED.get(name)
+        if checked is None:
+            words = [_word(x, self.device, keep) for x in args]
+        else:
+            try:
+                words = map(operator.index, checked(self, keep, *args))
+            except MpcxError as e:
+                raise MpcxError(f"mpcx_{name}: {e}") from None
+        if fn(self.h, *words):
             raise MpcxError(f"mpcx_{name}: {self.lib.mpcx_last_error(self.h).decode()}")
 
     def scratch_bytes(self, name, *sizes):
         """Bytes of scratch memory that the caller of ``mpcx_<name>`` hands over (mpcx_<name>_scratch)."""
-        fn = getattr(self.lib, f"mpcx_{name}_scratch")
-        fn.restype = ctypes.c_uint64
-        return fn(*[ctypes.c_uint64(s) for s in sizes])
+        fn = self._fns.get((name, "scratch"))
+        if fn is None:
+            fn = self.lib[f"mpcx_{name}_scratch"]
+            fn.argtypes, fn.restype = [ctypes.c_uint64] * len(sizes), ctypes.c_uint64
+            self._fns[name, "scratch"] = fn
+        return fn(*map(operator.index, sizes))
 
     def sync(self):
         self._call("mpcx_sync")
