@@ -468,7 +468,7 @@ int mpcx_aby3_clip_local(mpcx_ctx *ctx, int party, const int64_t *const *X0, con
  *   entropy    - sum p ln p
  *   top_ids / top_logp   the `top` likeliest ids (rows x top), equal words by the lower id, and their ln p
  * Differences of words are exact; the sums are kept in 32-bit floats.  top <= 32, top <= vocab, frac <= 62,
- * vocab < 2^31.  ids / logp may be NULL when per_row = 0, top_ids / top_logp when top = 0; entropy, row_max and log_sum
+ * 1 <= vocab < 2^31 (without rows there is nothing to do, whatever vocab and top).  ids / logp may be NULL when per_row = 0, top_ids / top_logp when top = 0; entropy, row_max and log_sum
  * may be NULL. */
 uint64_t mpcx_reveal_logprobs_scratch(uint64_t rows, uint64_t vocab, uint64_t top);
 int mpcx_reveal_logprobs(mpcx_ctx *ctx, const int64_t *a, const int64_t *b, const int64_t *c, uint64_t rows, uint64_t vocab,

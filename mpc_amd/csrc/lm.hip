@@ -1413,10 +1413,10 @@ uint64_t mpcx_reveal_logprobs_scratch(uint64_t rows, uint64_t vocab, uint64_t to
 int mpcx_reveal_logprobs(mpcx_ctx *ctx, const int64_t *a, const int64_t *b, const int64_t *c, uint64_t rows, uint64_t vocab,
                          int frac, const int64_t *ids, uint64_t per_row, uint64_t top, void *scratch, float *logp,
                          float *entropy, int64_t *top_ids, float *top_logp, int64_t *row_max, float *log_sum) {
-    MPCX_REQUIRE(vocab >= 1 && vocab < (1ull << 31), "mpcx_reveal_logprobs: vocabulary of %llu", (unsigned long long)vocab);
+    MPCX_REQUIRE((vocab >= 1 || rows == 0) && vocab < (1ull << 31), "mpcx_reveal_logprobs: vocabulary of %llu", (unsigned long long)vocab);
     MPCX_REQUIRE(lm_fits(rows, vocab) && lm_fits(rows, per_row), "mpcx_reveal_logprobs: sizes too large");
     MPCX_REQUIRE(frac >= 0 && frac <= 62, "mpcx_reveal_logprobs: %d fractional bits", frac);
-    MPCX_REQUIRE(top <= 32 && top <= vocab, "mpcx_reveal_logprobs: %llu alternatives", (unsigned long long)top);
+    MPCX_REQUIRE(top <= 32 && (top <= vocab || rows == 0), "mpcx_reveal_logprobs: %llu alternatives", (unsigned long long)top);
     MPCX_REQUIRE(b || !c, "mpcx_reveal_logprobs: the third share without the second");
     if (rows == 0) return 0;
     MPCX_REQUIRE(a && scratch && (per_row == 0 || (ids && logp)) && (top == 0 || (top_ids && top_logp)),
@@ -1437,7 +1437,7 @@ int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b,
                               uint64_t vocab, int frac, const int64_t *ids, uint64_t per_row, const float *d_logp,
                               const float *d_entropy, const int64_t *row_max, const float *log_sum, const float *entropy,
                               float *grad, int64_t *grad_words, int grad_frac) {
-    MPCX_REQUIRE(vocab >= 1 && vocab < (1ull << 31), "mpcx_reveal_logprobs_grad: vocabulary of %llu", (unsigned long long)vocab);
+    MPCX_REQUIRE((vocab >= 1 || rows == 0) && vocab < (1ull << 31), "mpcx_reveal_logprobs_grad: vocabulary of %llu", (unsigned long long)vocab);
     MPCX_REQUIRE(lm_fits(rows, vocab) && lm_fits(rows, per_row), "mpcx_reveal_logprobs_grad: sizes too large");
     MPCX_REQUIRE(frac >= 0 && frac <= 62, "mpcx_reveal_logprobs_grad: %d fractional bits", frac);
     MPCX_REQUIRE(!grad_words || (grad_frac >= 0 && grad_frac <= 62), "mpcx_reveal_logprobs_grad: %d fractional bits", grad_frac);

@@ -95,7 +95,8 @@ class ABY3Engine {
     void clip_norm(const vector<VecPair> &X, uint64_t max_norm, size_t number, vector<VecPair> &Y, int64_t *factor = nullptr);
     // Opens logits (the round of reveal_matrix) with `number` fractional bits and returns, on every party, what a caller
     // reads of each row: the log probability of ids[row] (0 for an id outside the columns), the entropy, and the `top`
-    // likeliest columns with their log probabilities (rows x top, best first, ties by the lower column).
+    // likeliest columns with their log probabilities (rows x top, best first, ties by the lower column); top <= 32 and <= the
+    // columns, unless there are no rows.
     struct LogProbs {
         vector<float> logp, entropy, top_logp;
         vector<int64_t> top_ids;

@@ -621,6 +621,36 @@ static void aby3_language_party(InProcHub *hub, size_t p) {
     CHECK(fabsf(out.top_logp[6] + logf(3 + 3 * expf(-1))) < 1e-6f);
 }
 
+// the same on matrices without rows or columns, and on no tensors at all
+static void aby3_language_empty_party(InProcHub *hub, size_t p) {
+    InProcMessenger msgr(hub, p);
+    ABY3Engine e(&msgr, p);
+    for (size_t dim : {(size_t)0, (size_t)5}) {
+        array<MatrixXl, 2> none{MatrixXl(0, dim), MatrixXl(0, dim)}, rows{MatrixXl(3, dim), MatrixXl(3, dim)}, out;
+        for (auto &m : rows)
+            for (size_t i = 0; i < 3; i++)
+                for (size_t j = 0; j < dim; j++) m(i, j) = 7;
+        e.embed(none, {0, 1}, 3, out); // a table without rows: every id lies outside
+        CHECK(out[0].rows() == 2 && out[1].rows() == 2 && (size_t)out[0].cols() == dim);
+        for (size_t j = 0; j < dim; j++) CHECK(out[0](0, j) == 0 && out[1](1, j) == 0);
+        e.embed(rows, {}, 3, out);
+        CHECK(out[0].rows() == 0 && (size_t)out[1].cols() == dim);
+        e.embed_grad(none, {}, 4, 3, out);
+        CHECK(out[0].rows() == 4 && (size_t)out[0].cols() == dim);
+        for (size_t j = 0; j < dim; j++) CHECK(out[0](3, j) == 0 && out[1](0, j) == 0);
+        e.embed_grad(rows, {0, 1, 2}, 0, 3, out);
+        CHECK(out[0].rows() == 0 && (size_t)out[1].cols() == dim);
+        ABY3Engine::LogProbs lp;
+        lp.logp = {1};
+        e.reveal_logprobs(none, 16, {}, 3, lp);
+        CHECK(lp.logp.empty() && lp.entropy.empty() && lp.top_ids.empty() && lp.top_logp.empty());
+    }
+    vector<array<VecI64, 2>> y(1);
+    int64_t factor = 0;
+    e.clip_norm({}, 1 << 16, 16, y, &factor);
+    CHECK(y.empty() && factor == 1 << 16);
+}
+
 template <class F> static void run3(F party) {
     InProcHub hub;
     std::thread t0(party, &hub, 0), t1(party, &hub, 1), t2(party, &hub, 2);
@@ -662,6 +692,7 @@ int main() {
     run3(snn_additions_party);
     run3(empty_inputs_party);
     run3(aby3_language_party);
+    run3(aby3_language_empty_party);
     if (failures.load()) {
         printf("host_selftest: %d check(s) FAILED\n", failures.load());
         return 1;

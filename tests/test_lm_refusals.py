@@ -182,3 +182,11 @@ def test_binding_refuses_tensors_of_another_device():
     for wrong in ([host], [host, 7], [7, host[:1]], [host[:1], None], [torch.nn.Parameter(host.double()), host]):
         with pytest.raises(MpcxError, match="context on device 0"):  # one word of a tensor is never taken for a number
             _word(wrong, 0, [])
+
+
+def test_logits_without_rows_are_no_error_whatever_their_columns(lib):
+    for vocab, top in ((0, 0), (0, 3), (2, 3)):
+        assert lib.mpcx_reveal_logprobs(N, X, N, N, U(0), U(vocab), I(16), X, U(1), U(top), X, X, N, X, X, N, N) == 0
+    assert lib.mpcx_reveal_logprobs_grad(N, X, N, N, U(0), U(0), I(16), X, U(1), X, N, X, X, N, X, N, I(0)) == 0
+    for args in (lp(rows=0, top=33), lp(rows=0, frac=63), lp(rows=0, vocab=1 << 31)):
+        assert lib.mpcx_reveal_logprobs(N, *args) != 0
