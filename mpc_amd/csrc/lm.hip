@@ -1137,10 +1137,10 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, Logp
     } else if (A.per_row) {
         w = (u64)ids[0] < A.vocab ? dl[0] : 0.0f;
     }
-    // - p w - h p (ln p + H)
+    // - p w - h p (ln p + H); 0 where p is, whatever h ln p comes to
     auto part = [&](u64 x) {
         const float lp = -(word_dist(m, (i64)x) * A.unit + ls), p = expf(lp);
-        return -p * (w + h * (lp + H));
+        return p == 0.0f ? 0.0f : -p * (w + h * (lp + H));
     };
     auto put1 = [&](u64 at, float g) {
         if (A.grad) A.grad[at] = g;
