@@ -1096,7 +1096,7 @@ template <int SH> __global__ __launch_bounds__(JOIN_THREADS) void logprobs_join_
 // three shares into floats, 1.9 GB: 331 us, 5.7 TB/s).  TPR threads (a workgroup, or one wavefront of it for short rows)
 // take `chunk` words of a row, 16 bytes of each share per load and GRAD_PAIRS of them together; the words of the given
 // ids are written again at the end with their own terms added, so that the pass itself knows no ids and every word is
-// rounded once.
+// rounded once; MANY: ids beyond a few dozen a row.
 constexpr u32 GRAD_PAIRS = 4;
 struct LogprobGradArgs {
     u64 rows, vocab, chunk;
@@ -1112,9 +1112,47 @@ struct LogprobGradArgs {
 };
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef f32x2 f32x2u __attribute__((aligned(4)));
-template <int SH, bool STREAM, u32 TPR>
+constexpr u64 LP_GRAD_CHUNK = 512 * GRAD_PAIRS; // words of a row that a workgroup takes: one tile, see below
+constexpr u64 LP_GRAD_WAVE_ROW = 768;           // longest row that one wavefront takes
+// The sums of d_logp of equal ids, for rows of many ids: a wavefront goes once through the row's ids, in their order, and
+// adds to a word of LDS for each of its words of the row.  64 ids at a time: where no two of them are the same (every lane
+// leaves its number at its id's word, and finds it there) the lanes add together, else one after the other.
+template <u32 WORDS> struct IdSums {
+    float sum[WORDS];
+    u32 lane_of[WORDS]; // the last lane that came by; NO_ID: no id at all
+    static constexpr u32 NO_ID = ~0u;
+    __device__ void clear(u32 t, u32 n) {
+        for (u32 i = t; i < WORDS; i += n) sum[i] = 0, lane_of[i] = NO_ID;
+    }
+    __device__ void add(const i64 *ids, const float *dl, u64 count, u64 j0, u64 j1) {
+        const u32 lane = threadIdx.x & 63;
+        u64 next = lane < count ? (u64)ids[lane] : j1;
+        float next_w = lane < count ? dl[lane] : 0.0f;
+        for (u64 k0 = 0; k0 < count; k0 += 64) {
+            const u64 id = next, k = k0 + 64 + lane;
+            const float w = next_w;
+            next = k < count ? (u64)ids[k] : j1, next_w = k < count ? dl[k] : 0.0f; // the next 64 are on their way
+            const bool in = id >= j0 && id < j1;
+            const u32 at = in ? (u32)(id - j0) : 0;
+            if (in) lane_of[at] = lane;
+            prg_wave_sync();
+            if (__ballot(in && lane_of[at] != lane) == 0) {
+                if (in) sum[at] += w;
+            } else {
+                for (u64 todo = __ballot(in); todo; todo &= todo - 1) {
+                    if (lane == (u32)__builtin_ctzll(todo)) sum[at] += w;
+                    prg_wave_sync();
+                }
+            }
+            prg_wave_sync();
+        }
+    }
+};
+template <int SH, bool STREAM, u32 TPR, bool MANY = false>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, LogprobGradArgs A) {
     __shared__ float ws[4];
+    constexpr u32 WORDS = MANY ? (TPR == 64 ? LP_GRAD_WAVE_ROW : LP_GRAD_CHUNK) : 1;
+    __shared__ IdSums<WORDS> sums[MANY ? 256 / TPR : 1];
     const u32 tid = threadIdx.x % TPR;
     const u64 group = (u64)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
     const u64 row = group / A.splits, split = group % A.splits, base = row * A.vocab;
@@ -1172,6 +1210,17 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, Logp
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (TPR > 64) __syncthreads();
     else prg_wave_sync();
+    if constexpr (MANY) {
+        auto &mine = sums[threadIdx.x / TPR];
+        mine.clear(tid, TPR);
+        if (TPR > 64) __syncthreads();
+        else prg_wave_sync();
+        if (tid < 64) mine.add(ids, dl, A.per_row, j0, j1);
+        if (TPR > 64) __syncthreads();
+        for (u32 i = tid; i < j1 - j0; i += TPR)
+            if (mine.lane_of[i] != mine.NO_ID) put1(base + j0 + i, mine.sum[i] + part((u64)in.at(base + j0 + i)));
+        return;
+    }
     for (u64 t = tid; t < A.per_row; t += TPR) {
         const u64 id = (u64)ids[t];
         if (id < j0 || id >= j1) continue;
@@ -1192,10 +1241,13 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogitIn<SH> in, Logp
 // 8000: 74 against 78, of 16000: 137 against 140).
 constexpr u64 LP_ROWS = 256, LP_GROUPS = 1024, LP_CHUNK = 2048, LP_WAVE_ROW = 8192;
 bool lp_one_wave(u64 rows, u64 vocab) { return vocab <= 1024 || (vocab <= LP_WAVE_ROW && rows >= 2048); }
-// Words of a row that a workgroup of the gradient takes: one tile.  2048 rows of 32768 words of three shares: 331 us with
-// 2048 words (5.7 TB/s), 344 with 4096, 372 with whole rows.
-constexpr u64 LP_GRAD_CHUNK = 512 * GRAD_PAIRS;
-constexpr u64 LP_GRAD_WAVE_ROW = 768; // the same for the gradient: 8192 rows of 500 21 us against 27, of 1000 38 against 38
+// LP_GRAD_CHUNK, one tile: 2048 rows of 32768 words of three shares take 331 us with 2048 words (5.7 TB/s), 344 with 4096, 372
+// with whole rows.  LP_GRAD_WAVE_ROW: 8192 rows of 500 21 us against 27 of a workgroup, of 1000 38 against 38.
+// LP_GRAD_MANY: rows of more ids collect them in LDS (IdSums); up to it every id looks through the row's ids by itself, whose
+// work grows with their square.  512 rows of 32768: 16 ids 37 us either way, 32 43 looking against 37, 256 264 against 49, 1024
+// 3.7 ms against 87 us; 512 rows of 700: 32 ids 10.7 us against 11.6, 64 15.7 against 14.0; as many ids as words, 512 rows of
+// 32768: 1.46 ms collected.
+constexpr u64 LP_GRAD_MANY = 32;
 template <int SH> int logprobs_run(mpcx_ctx *ctx, LogitIn<SH> in, LogprobArgs A) {
     const u64 all = A.rows;
     for (u64 r0 = 0; r0 < all; r0 += LM_MAX_BLOCKS) { // rows of one launch; more than one launch: nothing is split
@@ -1468,10 +1520,18 @@ int mpcx_reveal_logprobs_grad(mpcx_ctx *ctx, const int64_t *a, const int64_t *b,
         return 0;
     };
     const u64 *pa = (const u64 *)a, *pb = (const u64 *)b, *pc = (const u64 *)c;
-    auto pick = [&](auto in, auto whole, auto streaming, auto wave) { return run(one_wave ? wave : stream ? streaming : whole, in); };
-    if (c) return pick(LogitIn<3>{pa, pb, pc}, logprobs_grad_kernel<3, false, 256>, logprobs_grad_kernel<3, true, 256>, logprobs_grad_kernel<3, false, 64>);
-    if (b) return pick(LogitIn<2>{pa, pb, nullptr}, logprobs_grad_kernel<2, false, 256>, logprobs_grad_kernel<2, true, 256>, logprobs_grad_kernel<2, false, 64>);
-    return pick(LogitIn<1>{pa, nullptr, nullptr}, logprobs_grad_kernel<1, false, 256>, logprobs_grad_kernel<1, true, 256>, logprobs_grad_kernel<1, false, 64>);
+    const bool many = per_row > LP_GRAD_MANY;
+    auto pick = [&](auto in, auto whole, auto streaming, auto wave, auto many_whole, auto many_wave) {
+        return run(many ? (one_wave ? many_wave : many_whole) : one_wave ? wave : stream ? streaming : whole, in);
+    };
+    if (c)
+        return pick(LogitIn<3>{pa, pb, pc}, logprobs_grad_kernel<3, false, 256>, logprobs_grad_kernel<3, true, 256>,
+                    logprobs_grad_kernel<3, false, 64>, logprobs_grad_kernel<3, false, 256, true>, logprobs_grad_kernel<3, false, 64, true>);
+    if (b)
+        return pick(LogitIn<2>{pa, pb, nullptr}, logprobs_grad_kernel<2, false, 256>, logprobs_grad_kernel<2, true, 256>,
+                    logprobs_grad_kernel<2, false, 64>, logprobs_grad_kernel<2, false, 256, true>, logprobs_grad_kernel<2, false, 64, true>);
+    return pick(LogitIn<1>{pa, nullptr, nullptr}, logprobs_grad_kernel<1, false, 256>, logprobs_grad_kernel<1, true, 256>,
+                logprobs_grad_kernel<1, false, 64>, logprobs_grad_kernel<1, false, 256, true>, logprobs_grad_kernel<1, false, 64, true>);
 }
 
 } // extern "C"
