@@ -446,7 +446,8 @@ int mpcx_ring_embed_grad(mpcx_ctx *ctx, const int64_t *G0, const int64_t *G1, co
 /* This party's share of the squared norm of `count` shared tensors taken together, before the round: z0[0] = sum over all
  * words of X0*X0 + X0*X1 + X1*X0, plus pop(next) - pop(prev) (one word of each stream).  X0, X1 and lens are HOST arrays:
  * the device pointers of the tensors' shares and their word counts (0 allowed).  The sum of the three parties' z0 is the
- * squared norm with twice the tensors' fractional bits; it must stay below 2^64. */
+ * squared norm with twice the tensors' fractional bits, mod 2^64: the norm of the words has to stay below 2^32, that of the
+ * reals below 2^(32 - frac).  A larger one wraps, and nothing can be seen of that in the opened word. */
 uint64_t mpcx_aby3_sqnorm_scratch(uint64_t count);
 int mpcx_aby3_sqnorm_local(mpcx_ctx *ctx, const int64_t *const *X0, const int64_t *const *X1, const uint64_t *lens,
                            uint64_t count, uint64_t seed_next, uint64_t pop_next, uint64_t seed_prev, uint64_t pop_prev,
@@ -457,7 +458,11 @@ int mpcx_aby3_sqnorm_local(mpcx_ctx *ctx, const int64_t *const *X0, const int64_
  * the trunc segment (ABY3Engine.cpp:480-503) of c * X by `number` bits: the message to the previous party, the tensors
  * one after the other (the words that parties 1 and 2 pop run through them in the same order).  Party 0 reads X0 only,
  * party 1 both shares, party 2 none (its X0 / X1 may be NULL).  coef (one device word) receives c.  number <= 31,
- * max_norm < 2^(62 - number).  Party 0's segment is also the local clip of an additive share. */
+ * max_norm < 2^(62 - number); a bound of 2^32 and more never acts.
+ * The tensors' norm has to stay below 2^32 (65536 in reals of 16 fractional bits): with a larger one S has wrapped, and the
+ * factor, formed from what is left, lets the tensors pass too large.  Tensors that may be that large are truncated by k bits
+ * first (mpcx_aby3_trunc_local) and clipped to max_norm >> k with number - k fractional bits, which moves the limit to
+ * 2^(32 + k) and leaves the factor number - k bits.  Party 0's segment is also the local clip of an additive share. */
 int mpcx_aby3_clip_local(mpcx_ctx *ctx, int party, const int64_t *const *X0, const int64_t *const *X1, const uint64_t *lens,
                          uint64_t count, const int64_t *z_prev, const int64_t *z0, const int64_t *z1, uint64_t max_norm,
                          int number, uint64_t seed12, uint64_t pop12, int64_t *Y0, int64_t *coef);

@@ -386,14 +386,14 @@ class GpuBackend:
             _sized(what, a.size, b)
 
     def aby3_sqnorm_local(self, X0s, X1s, seed_next, pop_next, seed_prev, pop_prev):
-        """X0s, X1s: lists of the tensors' shares."""
+        """X0s, X1s: lists of the tensors' shares, whose norm (in words) has to stay below 2^32."""
         self._same_lengths("aby3_sqnorm_local", X0s, X1s)
         X0s, X1s = [_c(x, np.int64) for x in X0s], [_c(x, np.int64) for x in X1s]
         return self._go("aby3_sqnorm_local", X0s, X1s, [x.size for x in X0s], len(X0s), seed_next, pop_next, seed_prev, pop_prev,
                         self._scratch("aby3_sqnorm", len(X0s)), ("out", np.int64, 1))
 
     def aby3_clip_local(self, party, X0s, X1s, z_prev, z0, z1, max_norm, number, seed12, pop12):
-        """Returns the message (the tensors one after the other) and the factor."""
+        """Returns the message (the tensors one after the other) and the factor; for norms (in words) below 2^32."""
         self._same_lengths("aby3_clip_local", X0s, X1s)
         _sized("aby3_clip_local", 1, z_prev, z0, z1)
         lens = [x.size for x in X0s]

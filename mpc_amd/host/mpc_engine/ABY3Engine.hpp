@@ -92,6 +92,9 @@ class ABY3Engine {
     // Y = X clipped to the global norm max_norm of all tensors together (max_norm and X with `number` fractional bits): two
     // rounds, the opened squared norm (one word to each of the others) and trunc's.  One word popped from each pair stream,
     // then trunc's words.  factor receives the public factor (`number` fractional bits).  X and Y may be the same.
+    // The opened square is one word: the norm of X has to stay below 2^32 (65536 in reals of 16 fractional bits).  A larger one
+    // wraps without a sign of it and X passes too large; tensors that may be that large go through trunc by k bits first, and
+    // are clipped to max_norm >> k with number - k bits.
     void clip_norm(const vector<VecPair> &X, uint64_t max_norm, size_t number, vector<VecPair> &Y, int64_t *factor = nullptr);
     // Opens logits (the round of reveal_matrix) with `number` fractional bits and returns, on every party, what a caller
     // reads of each row: the log probability of ids[row] (0 for an id outside the columns), the entropy, and the `top`

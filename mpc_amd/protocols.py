@@ -188,7 +188,7 @@ def aby3_embed_grad(w, Gs, ids, vocab, dim, scale=1):
 
 def aby3_sqnorm(w, tensors):
     """tensors: list of share lists.  The three shares of the squared norm of all of them together; party j sends its own
-    to both others (the norm is opened)."""
+    to both others (the norm is opened).  The square is one word: a norm of 2^32 (in words) and more wraps unseen."""
     z = []
     for j in range(3):
         nx, pv = (j + 1) % 3, (j + 2) % 3
@@ -200,7 +200,8 @@ def aby3_sqnorm(w, tensors):
 
 def aby3_clip(w, tensors, max_norm, number):
     """Clips the tensors to the global norm max_norm (`number` fractional bits, as the tensors).  Two rounds: the opened
-    norm, then trunc's message.  Returns the clipped shares of all tensors as one vector, and the factor."""
+    norm, then trunc's message.  Returns the clipped shares of all tensors as one vector, and the factor.  Tensors whose norm
+    may reach 2^32 words go through aby3_trunc by k bits first, and are clipped to max_norm >> k with number - k bits."""
     z = aby3_sqnorm(w, tensors)
     total = sum(t[0][0].size for t in tensors)
     pops = [0, w.take(1, 2, total), w.take(2, 1, total)]

@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 
 import lm_reference as ref
+import protocols as pr
 from test_gpu_lm import KINDS, LOWEST, STEP, gpu, logprob_bounds, logit_rows, resident, rnd, share, tokens  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -235,3 +236,25 @@ def test_embed_grad_accumulates_few_tokens_of_many_rows(gpu, shares, vocab, dim,
         want = old[k].copy()
         want[:vocab * dim] = (ref.words(want[:vocab * dim]) + ref.words(add)).view(np.int64)
         assert np.array_equal(dT[k].to_host(), want), k
+
+
+def test_clipping_of_norms_beyond_the_opened_word(gpu, orc):
+    """A norm of 2^32 words and more wraps in the opened word; truncated by k bits first, the tensors are clipped as they should
+    be (the way that mpcx_aby3_clip_local and ABY3Engine::clip_norm name)."""
+    frac, k = 16, 8
+    rng = np.random.default_rng(3)
+    X = [rng.normal(size=n) * 9000 for n in (100, 7, 400)]  # reals of norm 2e5
+    X = [(x * 2 ** frac).astype(np.int64) for x in X]
+    assert sum(int(v) ** 2 for x in X for v in x) >= 2 ** 64
+    w = pr.World(gpu)
+    shares = [pr.aby3_trunc(w, pr.aby3_share(w, x, x.size), k) for x in X]
+    open3 = lambda S: (ref.words(S[0][0]) + ref.words(S[1][0]) + ref.words(S[2][0])).view(np.int64)
+    cut = np.concatenate([open3(s) for s in shares])
+    S = sum(int(v) ** 2 for v in cut)
+    assert S < 2 ** 64 and np.abs(cut - (np.concatenate(X) >> k)).max() <= 1
+    clipped, coef = pr.aby3_clip(w, shares, (20000 << frac) >> k, frac - k)  # to a norm of 20000
+    c = ref.clip_factor(S, 20000 << (frac - k), frac - k)
+    assert int(coef[0]) == c and 0 < c < 2 ** (frac - k)
+    got = open3(clipped)
+    assert np.abs(got - ((cut * c) >> (frac - k))).max() <= 2
+    assert np.sqrt((got.astype(np.float64) ** 2).sum()) <= (20000 << (frac - k)) + 2 * np.sqrt(got.size)
