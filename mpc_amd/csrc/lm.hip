@@ -1459,6 +1459,7 @@ static u64 logprob_chunk(u64 rows, u64 vocab) {
     return ceil_div(ceil_div(vocab, splits ? splits : 1), 2048) * 2048;
 }
 uint64_t mpcx_reveal_logprobs_scratch(uint64_t rows, uint64_t vocab, uint64_t top) {
+    if (vocab >= (1ull << 31)) return 16; // the call refuses it
     const u64 splits = vocab ? ceil_div(vocab, logprob_chunk(rows, vocab)) : 1;
     return splits > 1 ? rows * splits * 4 * (sizeof(RowPart) + (top ? LIST * sizeof(TopEntry) : 0)) : 16;
 }

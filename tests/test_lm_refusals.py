@@ -190,3 +190,17 @@ def test_logits_without_rows_are_no_error_whatever_their_columns(lib):
     assert lib.mpcx_reveal_logprobs_grad(N, X, N, N, U(0), U(0), I(16), X, U(1), X, N, X, X, N, X, N, I(0)) == 0
     for args in (lp(rows=0, top=33), lp(rows=0, frac=63), lp(rows=0, vocab=1 << 31)):
         assert lib.mpcx_reveal_logprobs(N, *args) != 0
+
+
+def test_scratch_sizes_of_calls_that_are_refused():
+    """The sizes can be asked for whatever the numbers are (in a process of its own: it must not end by a signal)."""
+    import os
+    import subprocess
+    import sys
+    numbers = (0, 1, 255, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 56, 2 ** 63, 2 ** 64 - 2048, 2 ** 64 - 1)
+    code = ("import ctypes, itertools\nfrom mpc_amd.lib import load_library\nlib = load_library()\n"
+            "for name, k in (('ring_embed_grad', 3), ('aby3_sqnorm', 1), ('reveal_logprobs', 3)):\n"
+            "    fn = getattr(lib, f'mpcx_{name}_scratch')\n"
+            f"    for v in itertools.product({numbers}, repeat=k): fn(*map(ctypes.c_uint64, v))\n")
+    root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..")
+    assert subprocess.run([sys.executable, "-c", code], cwd=root, timeout=100).returncode == 0
