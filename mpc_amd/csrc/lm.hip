@@ -104,8 +104,8 @@ __global__ __launch_bounds__(256) void embed_kernel(const u64 *__restrict__ T0, 
 // ---- gradient of the lookup.  Rows of G whose tokens are equal are added; every word of G is read once and every word of
 // the table written once, so memory traffic is the bound.  A wavefront (or 2^lg lanes of it) owns 128 columns of a row of
 // the table, a 16-byte piece of each share per lane, and adds NT tokens at a time, whose loads are under way
-// together.  65536 tokens, 65536 rows of 1024 words of two shares (2.15 GB): 440 us, 400 of them in the additions (5.4 TB/s,
-// what a copy reaches); four pieces per lane take 490, atomic additions into the table 1300.
+// together.  65536 tokens, 65536 rows of 1024 words of two shares (2.15 GB): 450 us, 410 of them in the additions (5.2 TB/s;
+// a copy reaches 5.1); four pieces per lane take 490, atomic additions into the table 1300.
 struct GradArgs {
     const u64 *G0, *G1;
     const i64 *ids;
@@ -597,7 +597,10 @@ __global__ __launch_bounds__(256) void clip_kernel(TensorTable tab, ClipArgs A, 
     }
 }
 // y = ((c (x0 + x1)) >> number) - w (party 1), w the stream's words, consumed where they are regenerated: 24 bytes of traffic
-// a word, the bound of long tensors (2^26 words in 1, 4 or 16 tensors: 310 us, 5.2 TB/s).  The 32 words of a lane's 16 visits
+// a word, the bound of long tensors of whole runs (2^26 words in 1, 4 or 16 tensors: 310 us, 5.2 TB/s).  Tensors of any length
+// cost more, 2e8 words in 293 take 1.52 ms (3.2 TB/s): the runs of 16 words that a visit reads lie across lines (the counters
+// show up to twice the reads, and a fifth more writes), and launches that begin between two checkpoints of the stream discard
+// up to 63 words a lane.  The 32 words of a lane's 16 visits
 // are asked for before the stream's are generated, which hides their way from memory (90 tensors of 5000 words: 25 us against
 // 33).  A wavefront (4096 words) that lies in one tensor finds it once; another goes, at every visit, from tensor to tensor.
 // Scaling all tensors by one launch and masking them by a second takes 542 us for 16 tensors, 30 for 90 of 5000 words, and 26
@@ -1093,10 +1096,10 @@ template <int SH> __global__ __launch_bounds__(JOIN_THREADS) void logprobs_join_
 }
 
 // The gradient: reads the logits once and writes its floats or words, bound by that traffic (2048 rows of 32768 words of
-// three shares into floats, 1.9 GB: 331 us, 5.7 TB/s).  TPR threads (a workgroup, or one wavefront of it for short rows)
-// take `chunk` words of a row, 16 bytes of each share per load and GRAD_PAIRS of them together; the words of the given
-// ids are written again at the end with their own terms added, so that the pass itself knows no ids and every word is
-// rounded once; MANY: ids beyond a few dozen a row.
+// three shares into floats, 1.9 GB: 331 us, 5.7 TB/s; into ring words, 2.1 GB: 371 us, 5.8 TB/s).  TPR threads (a workgroup, or
+// one wavefront of it for short rows) take `chunk` words of a row, 16 bytes of each share per load and GRAD_PAIRS of them
+// together; the words of the given ids are written again at the end with their own terms added, so that the pass itself knows
+// no ids and every word is rounded once; MANY: ids beyond a few dozen a row.
 constexpr u32 GRAD_PAIRS = 4;
 struct LogprobGradArgs {
     u64 rows, vocab, chunk;

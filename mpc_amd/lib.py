@@ -271,7 +271,8 @@ class Context:
 
     def call(self, name, *args):
         """Calls ``mpcx_<name>(ctx, *args)``; DeviceArrays, tensors on the context's device, ints and lists of these are
-        converted, and tensors in host memory where the entry point takes a host address."""
+        converted, and tensors in host memory where the entry point takes a host address.  Nothing is kept and nothing is
+        ordered here: tensors have to be ready on the context's stream, and live until it has passed."""
         if not self.h:
             raise MpcxError(f"mpcx_{name}: the context is closed")
         fn = self._fns.get((name, len(args)))
